@@ -26,7 +26,10 @@ EXP_DIR = os.path.join(HERE, '..', 'tools', 'experiments')
 SOURCES_EXP = SOURCES + [os.path.join(EXP_DIR, 'exp_se.hip'), os.path.join(EXP_DIR, 'exp_attn.hip')]
 HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_common.h'), os.path.join(CSRC, 'conv3p.h'), os.path.join(CSRC, 'conv3_knobs.h'),
            os.path.join(HERE, '..', 'include', 'mv2.h')]
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result']
+# packed fp32 arithmetic is switched off: some forms of v_pk_{add,mul,fma}_f32 that hipcc makes of ordinary float code have given wrong
+# results now and then on these chips (the host pass does not know the feature and says so: harmless)
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result', *NO_PACKED_FP32]
 
 
 def _hipcc():

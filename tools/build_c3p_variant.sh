@@ -8,7 +8,7 @@ TAG=${1:?tag}; SRC=${2:?source}; DEFS=$3
 R=$(cd "$(dirname "$0")/.." && pwd)
 P=$R/magvit2_pytorch_amd
 python3 -m magvit2_pytorch_amd.build --experiments >/dev/null || exit 1
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Wno-unused-result -DMV2_EXPERIMENTS $DEFS -I $P/csrc -c $R/$SRC -o $P/csrc/_obj_exp/conv3p_$TAG.o || exit 1
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -fno-gpu-rdc -Wno-unused-result -DMV2_EXPERIMENTS $DEFS -I $P/csrc -c $R/$SRC -o $P/csrc/_obj_exp/conv3p_$TAG.o || exit 1
 objs=$(ls $P/csrc/_obj_exp/*.o | grep -v "/conv3p\.o\|/conv3p_\|/conv3_\|/convg_" | tr '\n' ' ')
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $objs $P/csrc/_obj_exp/conv3p_$TAG.o -o $P/libmv2_hip_exp_$TAG.so || exit 1
 echo built $P/libmv2_hip_exp_$TAG.so

@@ -6,7 +6,7 @@ cd "$(dirname "$0")/../magvit2_pytorch_amd/csrc" || exit 1
 T=$(mktemp -d)
 for f in ${@:-conv3p.hip conv3.hip convin.hip convout.hip pwse.hip ff.hip conv.hip misc.hip attn.hip quant.hip}; do
   b=$(basename "$f" .hip)
-  hipcc -O3 -std=c++17 --offload-arch=gfx950 --cuda-device-only -S -I../../include "$b.hip" -o "$T/$b.s" 2>/dev/null || { echo "$b: compile failed"; continue; }
+  hipcc -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops --offload-arch=gfx950 --cuda-device-only -S -I../../include "$b.hip" -o "$T/$b.s" 2>/dev/null || { echo "$b: compile failed"; continue; }
   grep "\.name: \+_Z\|private_segment_fixed_size\|\.vgpr_count\|vgpr_spill" "$T/$b.s" |
     awk -v F="$b" '/\.name:/{n=$2} /private_segment_fixed_size/{p=$2} /\.vgpr_count/{v=$2} /vgpr_spill/{printf "%-12s %-70s vgpr=%-4s scratch=%-6s spills=%s\n", F, substr(n,1,70), v, p, $2}'
 done
