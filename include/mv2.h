@@ -382,6 +382,67 @@ int mv2_pad_ndhwc(const void* in, void* out, int B, int T, int H, int W, int64_t
  * out may alias residual. */
 int mv2_gateloop_scan(int dtype, const void* qkva, const void* residual, void* out, int B, int T, int64_t P, int C, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Gated linear recurrence along tokens, with states, padding, document starts and gradients: the general form of the scan inside
+ * 'gateloop_time' (mv2_gateloop_scan above: whole clips from an empty state, forward only).  Per sample b, pixel p and channel c
+ *     h_t = g_t h_{t-1} + kv_t,   g_t = sigmoid(a_t),   y_t = q_t h_t,        t = 0 .. T-1,  h_{-1} = h0 (NULL: 0)
+ * (gated linear recurrence with a real, data-dependent decay; T = 1 with h0 and h_last is the step of a decoder).
+ *   lengths  (B) int32, optional: tokens t >= lengths[b] (taken into [0, T]) do not exist: they are not read, y and the gradients
+ *            are zero there, h_last is the state behind the last token that exists (h0 where there is none).
+ *   resets   (B, T) bytes, optional: a token whose byte is not 0 starts a document: g_t = 0, whatever the state before it holds.
+ * q, kv, a share the strides in_* (elements), dq, dkv, da the strides grad_*; channels are contiguous, so the three may be the thirds of
+ * one (B, T, P, 3C) tensor.  y and dy are dense (B, T, P, C), h0 / h_last / dh_last / dh0 dense fp32 (B, P, C).  h_last may be
+ * h0 itself; otherwise outputs overlap neither inputs nor each other.  Storage is `dtype`; states, decays and sums are fp32.
+ * The backward pass starts from kept states: the forward call writes them to `states` if it is given (fp32,
+ * B * mv2_gateloop_states(d) * P * C floats).  dq / dkv / da are all written; dh_last and dh0 are optional.
+ * Any C and any strides are served; where C and the strides are whole 16-byte chunks and the pointers 16-byte aligned, rows are moved
+ * in such chunks. */
+typedef struct mv2_gateloop_desc {
+    int32_t dtype;
+    int32_t B, T, P, C;
+    int64_t in_b, in_t, in_p;          /* strides of q, kv, a */
+    int64_t grad_b, grad_t, grad_p;    /* strides of dq, dkv, da (backward) */
+} mv2_gateloop_desc;
+int64_t mv2_gateloop_states(const mv2_gateloop_desc* d);      /* kept states per sequence; < 0: MV2_E* */
+size_t mv2_gateloop_workspace_bytes(const mv2_gateloop_desc* d, int backward);
+int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, const void* kv, const void* a, const float* h0,
+                         const int32_t* lengths, const unsigned char* resets, void* y, float* h_last, float* states,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, const void* kv, const void* a, const float* h0,
+                          const int32_t* lengths, const unsigned char* resets, const float* states, const void* dy,
+                          const float* dh_last, void* dq, void* dkv, void* da, float* dh0, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The norms before and after a residual block, its gate and its scale, in one pass over the rows:
+ *     out = x + scale * act(gate) * N(branch; post_gamma),     normed = N(out; pre_gamma),
+ *     N(v; gamma) = v / max(|v|, 1e-12) * sqrt(C) * gamma                               (RMSNorm, reference M:258-276)
+ * out closes one block (Residual add, M:174), normed opens the next.  Each part is optional:
+ *   branch == NULL: no add (out is x; gate, post_gamma, scale must be NULL too);  post_gamma == NULL: branch enters as it is;
+ *   gate == NULL: 1;  scale == NULL: 1;  pre_gamma == NULL: no second norm.
+ * act: MV2_ACT_NONE (the gate itself), MV2_ACT_SILU or MV2_ACT_SIGMOID.  x, branch, gate are rows of C contiguous elements of `dtype` with
+ * row strides of their own (elements); every tensor the calls write is dense.  post_gamma, scale, pre_gamma: fp32 (C).  Norms and sums are
+ * fp32, and normed is taken from the unrounded out.  out may be x itself (same stride).  C <= 16384.
+ * rstd (optional output of the forward call, input of the backward call): fp32 (2, rows): 1 / max(|branch|, 1e-12), 1 / max(|out|, 1e-12).
+ * Backward: dout (gradient of out) and dn (of normed) may be NULL (zero); dx, dbranch, dgate (dense rows, dtype) and dpost, dscale, dpre (fp32 C)
+ * are each optional.  The column sums are taken in a fixed order: results are bitwise reproducible. */
+enum { MV2_ACT_SIGMOID = 5 };
+typedef struct mv2_block_norm_desc {
+    int32_t dtype;
+    int32_t C;
+    int64_t rows;
+    int64_t x_stride, branch_stride, gate_stride;
+    int32_t gate_act;
+    int32_t reserved;                  /* 0 */
+} mv2_block_norm_desc;
+size_t mv2_block_norm_workspace_bytes(const mv2_block_norm_desc* d);      /* of the backward call */
+int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post_gamma,
+                           const float* scale, const float* pre_gamma, void* out, void* normed, float* rstd, void* stream);
+int mv2_block_norm_backward(const mv2_block_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post_gamma,
+                            const float* scale, const float* pre_gamma, const float* rstd, const void* dout, const void* dn, void* dx,
+                            void* dbranch, void* dgate, float* dpost, float* dscale, float* dpre, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ResidualUnit tail at C = 128 / 256 / 512, bf16: the 1x1x1 conv + bias + ELU (reference M:937-938) and the SqueezeExcite
  * pooling records of its output (reference M:226-231) in ONE launch (replaces mv2_conv k = 1 + mv2_se_pool).  `wp` is the
  * C x C kernel in mv2_conv3's fragment-major order (the 1x1x1 kernel packed as mv2_conv does, then pack.py::to_frag_major).

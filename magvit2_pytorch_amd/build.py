@@ -18,13 +18,13 @@ CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, 'csrc', '_obj')
 LIB = os.path.join(HERE, 'libmv2_hip.so')
 # product library: no environment switches, no experimental kernels
-SOURCES = ['conv.hip', 'conv3.hip', 'conv3p.hip', 'convout.hip', 'convin.hip', 'pwse.hip', 'ff.hip', 'misc.hip', 'attn.hip', 'quant.hip', 'pack_host.hip']
+SOURCES = ['conv.hip', 'conv3.hip', 'conv3p.hip', 'convout.hip', 'convin.hip', 'pwse.hip', 'ff.hip', 'misc.hip', 'attn.hip', 'quant.hip', 'gateloop.hip', 'blocknorm.hip', 'pack_host.hip']
 # experiments library (tools/ only, -DMV2_EXPERIMENTS): the same sources with phase-clock profiling and the conv3 work-split knobs
 LIB_EXP = os.path.join(HERE, 'libmv2_hip_exp.so')
 # + kernels that exist only to be measured: they live with the other experiments under tools/experiments/, not in the product source directory
 EXP_DIR = os.path.join(HERE, '..', 'tools', 'experiments')
 SOURCES_EXP = SOURCES + [os.path.join(EXP_DIR, 'exp_se.hip'), os.path.join(EXP_DIR, 'exp_attn.hip')]
-HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_common.h'), os.path.join(CSRC, 'conv3p.h'), os.path.join(CSRC, 'conv3_knobs.h'),
+HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_common.h'), os.path.join(CSRC, 'conv3p.h'), os.path.join(CSRC, 'conv3_knobs.h'), os.path.join(CSRC, 'rowvec.h'),
            os.path.join(HERE, '..', 'include', 'mv2.h')]
 # packed fp32 arithmetic is switched off: some forms of v_pk_{add,mul,fma}_f32 that hipcc makes of ordinary float code have given wrong
 # results now and then on these chips (the host pass does not know the feature and says so: harmless)

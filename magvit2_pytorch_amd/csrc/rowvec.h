@@ -1,0 +1,23 @@
+// Row access of the kernels that serve any width and any strides: V elements of storage type E as one access - 16 bytes where the
+// rows, strides and addresses are whole 16-byte chunks (V = E::kVec), one element otherwise (V = 1).
+#pragma once
+#include "common.h"
+
+template <typename E, int V> struct RowVec {
+    static_assert(V == E::kVec, "a 16-byte chunk or one element");
+    i32x4 v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) { v = *(const i32x4*)((const typename E::T*)p + i); }
+    __device__ __forceinline__ void get(float* f) const { Chunk<E>::unpack(v, f); }
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { *(i32x4*)((typename E::T*)p + i) = Chunk<E>::pack(f); }
+};
+template <typename E> struct RowVec<E, 1> {
+    typename E::T v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) { v = ((const typename E::T*)p)[i]; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = ld_elem<E>(&v, 0); }
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { st_elem<E>(p, i, f[0]); }
+};
+
+static inline bool rows_aligned16(std::initializer_list<const void*> ps) {
+    for (const void* p : ps) if ((uintptr_t)p & 15) return false;
+    return true;
+}

@@ -31,6 +31,15 @@ class ConvDesc(C.Structure):
         'splitk')]
 
 
+class GateLoopDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ('dtype', 'B', 'T', 'P', 'C')] + [(n, C.c_int64) for n in ('in_b', 'in_t', 'in_p', 'grad_b', 'grad_t', 'grad_p')]
+
+
+class BlockNormDesc(C.Structure):
+    _fields_ = [('dtype', C.c_int32), ('C', C.c_int32)] + [(n, C.c_int64) for n in ('rows', 'x_stride', 'branch_stride', 'gate_stride')] + \
+               [('gate_act', C.c_int32), ('reserved', C.c_int32)]
+
+
 _SIGS = {
     'mv2_abi_version': (C.c_int, []),
     'mv2_device_cus': (C.c_int, []),
@@ -75,6 +84,13 @@ _SIGS = {
     'mv2_pack_conv3d': (C.c_int, [C.c_int, C.c_void_p] + [C.c_int] * 6 + [C.c_void_p, C.c_size_t]),
     'mv2_copy_frames': (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_void_p]),
     'mv2_gateloop_scan': (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_void_p]),
+    'mv2_gateloop_states': (C.c_int64, [C.POINTER(GateLoopDesc)]),
+    'mv2_gateloop_workspace_bytes': (C.c_size_t, [C.POINTER(GateLoopDesc), C.c_int]),
+    'mv2_gateloop_forward': (C.c_int, [C.POINTER(GateLoopDesc)] + [C.c_void_p] * 10 + [C.c_size_t, C.c_void_p]),
+    'mv2_gateloop_backward': (C.c_int, [C.POINTER(GateLoopDesc)] + [C.c_void_p] * 14 + [C.c_size_t, C.c_void_p]),
+    'mv2_block_norm_workspace_bytes': (C.c_size_t, [C.POINTER(BlockNormDesc)]),
+    'mv2_block_norm_forward': (C.c_int, [C.POINTER(BlockNormDesc)] + [C.c_void_p] * 10),
+    'mv2_block_norm_backward': (C.c_int, [C.POINTER(BlockNormDesc)] + [C.c_void_p] * 16 + [C.c_size_t, C.c_void_p]),
     'mv2_pad_ndhwc': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_void_p]),
     'mv2_cond_linear': (C.c_int, [C.c_void_p] * 4 + [C.c_int] * 4 + [C.c_float, C.c_void_p]),
     'mv2_scale_channels': (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_void_p]),
@@ -268,6 +284,40 @@ class HipOps:
     def gateloop_scan(self, dt, qkva, residual, out, B, T, Pn, Cc):
         fn, args = self.lib.mv2_gateloop_scan, (dt, _ptr(qkva), _ptr(residual), _ptr(out), B, T, Pn, Cc)
         return _mk(fn, args, 'mv2_gateloop_scan', (qkva, residual, out), [out])
+
+    # ---- gated recurrence and block norms (magvit2_pytorch_amd/functional.py); `d` is the filled descriptor, kept by the step
+    def gateloop_sizes(self, d: GateLoopDesc):
+        """(kept states per sequence, forward workspace bytes, backward workspace bytes) on this device"""
+        with torch.cuda.device(self.device):
+            n = int(self.lib.mv2_gateloop_states(C.byref(d)))
+            if n < 0:
+                raise Mv2Error(f'mv2_gateloop_states failed: {n}')
+            return n, int(self.lib.mv2_gateloop_workspace_bytes(C.byref(d), 0)), int(self.lib.mv2_gateloop_workspace_bytes(C.byref(d), 1))
+
+    def gateloop_forward(self, d, q, kv, a, h0, lengths, resets, y, h_last, states, ws):
+        args = (C.byref(d), _ptr(q), _ptr(kv), _ptr(a), _ptr(h0), _ptr(lengths), _ptr(resets), _ptr(y), _ptr(h_last), _ptr(states), _ptr(ws),
+                0 if ws is None else ws.numel() * ws.element_size())
+        return _mk(self.lib.mv2_gateloop_forward, args, 'mv2_gateloop_forward', (d, q, kv, a, h0, lengths, resets, y, h_last, states, ws), (y, h_last, states))
+
+    def gateloop_backward(self, d, q, kv, a, h0, lengths, resets, states, dy, dh_last, dq, dkv, da, dh0, ws):
+        args = (C.byref(d), _ptr(q), _ptr(kv), _ptr(a), _ptr(h0), _ptr(lengths), _ptr(resets), _ptr(states), _ptr(dy), _ptr(dh_last), _ptr(dq), _ptr(dkv),
+                _ptr(da), _ptr(dh0), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size())
+        return _mk(self.lib.mv2_gateloop_backward, args, 'mv2_gateloop_backward',
+                   (d, q, kv, a, h0, lengths, resets, states, dy, dh_last, dq, dkv, da, dh0, ws), (dq, dkv, da, dh0))
+
+    def block_norm_workspace_bytes(self, d: BlockNormDesc) -> int:
+        return int(self.lib.mv2_block_norm_workspace_bytes(C.byref(d)))
+
+    def block_norm_forward(self, d, x, branch, gate, post, scale, pre, out, normed, rstd):
+        args = (C.byref(d), _ptr(x), _ptr(branch), _ptr(gate), _ptr(post), _ptr(scale), _ptr(pre), _ptr(out), _ptr(normed), _ptr(rstd))
+        return _mk(self.lib.mv2_block_norm_forward, args, 'mv2_block_norm_forward', (d, x, branch, gate, post, scale, pre, out, normed, rstd), (out, normed, rstd))
+
+    def block_norm_backward(self, d, x, branch, gate, post, scale, pre, rstd, dout, dn, dx, dbranch, dgate, dpost, dscale, dpre, ws):
+        args = (C.byref(d), _ptr(x), _ptr(branch), _ptr(gate), _ptr(post), _ptr(scale), _ptr(pre), _ptr(rstd), _ptr(dout), _ptr(dn), _ptr(dx), _ptr(dbranch),
+                _ptr(dgate), _ptr(dpost), _ptr(dscale), _ptr(dpre), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size())
+        return _mk(self.lib.mv2_block_norm_backward, args, 'mv2_block_norm_backward',
+                   (d, x, branch, gate, post, scale, pre, rstd, dout, dn, dx, dbranch, dgate, dpost, dscale, dpre, ws),
+                   (dx, dbranch, dgate, dpost, dscale, dpre))
 
     def pad_ndhwc(self, x, out, B, T, H, W, row_bytes, pt, ph, pw, mode, tail_bytes):
         fn, args = self.lib.mv2_pad_ndhwc, (_ptr(x), _ptr(out), B, T, H, W, row_bytes, pt, ph, pw, mode, tail_bytes)

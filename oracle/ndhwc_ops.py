@@ -522,6 +522,109 @@ class CpuOps:
         step.what = 'gateloop_scan'
         return step
 
+    # ---- gated recurrence and block norms: token by token / row by row, from the header's formulas
+    def gateloop_sizes(self, d):
+        return max(d.T - 1, 0), 0, 0                     # one kept state per token but the first (the library keeps fewer)
+
+    @staticmethod
+    def _loop_view(t, d, grad=False):
+        st = (d.grad_b, d.grad_t, d.grad_p) if grad else (d.in_b, d.in_t, d.in_p)
+        return torch.as_strided(t, (d.B, d.T, d.P, d.C), (*st, 1), t.storage_offset())
+
+    def _loop_tables(self, d, a, lengths, resets):
+        """decay (B, T, P, C), and which tokens exist"""
+        g = torch.sigmoid(self._loop_view(a, d).to(self.acc))
+        n = torch.full((d.B,), d.T) if lengths is None else lengths.long().clamp(0, d.T)
+        live = torch.arange(d.T)[None] < n[:, None]
+        cut = torch.zeros(d.B, d.T, dtype=torch.bool) if resets is None else resets.bool()
+        return g, live[:, :, None, None], cut[:, :, None, None]
+
+    def gateloop_forward(self, d, q, kv, a, h0, lengths, resets, y, h_last, states, ws):
+        def step(stream):
+            g, live, cut = self._loop_tables(d, a, lengths, resets)
+            vq, vk = (self._loop_view(t, d).to(self.acc) for t in (q, kv))
+            h = torch.zeros(d.B, d.P, d.C, dtype=self.acc) if h0 is None else h0.reshape(d.B, d.P, d.C).to(self.acc)
+            o = torch.zeros(d.B, d.T, d.P, d.C, dtype=self.acc)
+            for t in range(d.T):
+                if states is not None and t > 0:
+                    states[:, t - 1].copy_(h)
+                new = vk[:, t] + torch.where(cut[:, t], torch.zeros_like(h), g[:, t] * h)
+                h = torch.where(live[:, t], new, h)
+                o[:, t] = torch.where(live[:, t], vq[:, t] * h, o[:, t])
+            y.reshape(o.shape).copy_(o)
+            if h_last is not None:
+                h_last.reshape(h.shape).copy_(h)
+        step.outs = [t for t in (y, h_last) if t is not None]
+        step.what = 'gateloop_forward'
+        return step
+
+    def gateloop_backward(self, d, q, kv, a, h0, lengths, resets, states, dy, dh_last, dq, dkv, da, dh0, ws):
+        def step(stream):
+            g, live, cut = self._loop_tables(d, a, lengths, resets)
+            vq, vk = (self._loop_view(t, d).to(self.acc) for t in (q, kv))
+            gy = dy.reshape(d.B, d.T, d.P, d.C).to(self.acc)
+            zero = torch.zeros(d.B, d.P, d.C, dtype=self.acc)
+            start = zero if h0 is None else h0.reshape(zero.shape).to(self.acc)
+            back = zero if dh_last is None else dh_last.reshape(zero.shape).to(self.acc)
+            for t in range(d.T - 1, -1, -1):
+                prev = start if t == 0 else states[:, t - 1].to(self.acc)
+                through = torch.where(cut[:, t], zero, g[:, t] * prev)
+                D = back + vq[:, t] * gy[:, t]
+                parts = ((vk[:, t] + through) * gy[:, t], D, torch.where(cut[:, t], zero, D * prev * g[:, t] * (1 - g[:, t])))
+                for out, v in zip((dq, dkv, da), parts):
+                    self._loop_view(out, d, grad=True)[:, t].copy_(torch.where(live[:, t], v, zero))
+                back = torch.where(live[:, t], torch.where(cut[:, t], zero, g[:, t] * D), back)
+            if dh0 is not None:
+                dh0.reshape(zero.shape).copy_(back)
+        step.outs = [t for t in (dq, dkv, da, dh0) if t is not None]
+        step.what = 'gateloop_backward'
+        return step
+
+    def block_norm_workspace_bytes(self, d):
+        return 4
+
+    def _block_norm(self, d, x, branch, gate, post, scale, pre, grad=False):
+        view = lambda t, s: None if t is None else torch.as_strided(t, (d.rows, d.C), (s, 1), t.storage_offset()).to(self.acc).requires_grad_(grad)
+        vec = lambda t: None if t is None else t.detach().to(self.acc).requires_grad_(grad)
+        ins = [view(x, d.x_stride), view(branch, d.branch_stride), view(gate, d.gate_stride), vec(post), vec(scale), vec(pre)]
+        vx, vb, vg, w1, sc, w2 = ins
+        norm = lambda v, w: v / v.norm(dim=-1, keepdim=True).clamp_min(1e-12) * math.sqrt(d.C) * w
+        out = vx
+        if vb is not None:
+            u = vb if w1 is None else norm(vb, w1)
+            if vg is not None:
+                s = torch.sigmoid(vg)
+                u = u * {0: vg, 2: vg * s, 5: s}[d.gate_act]
+            out = vx + (u if sc is None else u * sc)
+        return ins, out, None if w2 is None else norm(out, w2)
+
+    def block_norm_forward(self, d, x, branch, gate, post, scale, pre, out, normed, rstd):
+        def step(stream):
+            _, o, n = self._block_norm(d, x, branch, gate, post, scale, pre)
+            if branch is not None:
+                out.reshape(o.shape).copy_(o)
+            if n is not None:
+                normed.reshape(n.shape).copy_(n)
+        step.outs = [t for t in (out, normed) if t is not None]
+        step.what = 'block_norm_forward'
+        return step
+
+    def block_norm_backward(self, d, x, branch, gate, post, scale, pre, rstd, dout, dn, dx, dbranch, dgate, dpost, dscale, dpre, ws):
+        def step(stream):
+            with torch.enable_grad():
+                ins, o, n = self._block_norm(d, x, branch, gate, post, scale, pre, grad=True)
+            pairs = [(t, g.reshape(t.shape).to(self.acc)) for t, g in ((o, dout), (n, dn)) if g is not None]
+            live = [t for t in ins if t is not None]
+            got = torch.autograd.grad([p[0] for p in pairs], live, [p[1] for p in pairs], allow_unused=True)
+            by = {id(t): g for t, g in zip(live, got)}
+            for dst, t in zip((dx, dbranch, dgate, dpost, dscale, dpre), ins):
+                if dst is not None:
+                    g = by[id(t)]
+                    dst.reshape(t.shape).copy_(torch.zeros_like(t) if g is None else g)
+        step.outs = [t for t in (dx, dbranch, dgate, dpost, dscale, dpre) if t is not None]
+        step.what = 'block_norm_backward'
+        return step
+
     def pad_ndhwc(self, x, out, B, T, H, W, row_bytes, pt, ph, pw, mode, tail_bytes):
         """mv2_pad_ndhwc: F.pad(x, (pw, pw, ph, ph, pt, 0), mode) on an NDHWC tensor (mode 1 reflect / 2 replicate / 3 circular) + zero tail"""
         def step(stream):

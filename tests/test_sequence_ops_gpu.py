@@ -1,0 +1,557 @@
+"""The sequence operators (gated recurrence, block norms) on the GPU against the 64-bit references of tests/_sequence_ref.py, within the
+running error bounds derived there."""
+import pytest
+import torch
+
+from magvit2_pytorch_amd import functional as F
+from tests._sequence_ref import assert_within, block_norm_ref, gate_loop_ref
+
+pytestmark = pytest.mark.gpu
+DT = [torch.bfloat16, torch.float32]
+NAN, INF = float('nan'), float('inf')
+
+
+def rnd(*shape, seed=0, dtype=torch.float32, mean=0., std=1.):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std + mean).to(dtype)
+
+
+def loop_inputs(B, T, P, C, dtype, seed=0):
+    qkva = rnd(B, T, P, 3 * C, seed=seed, dtype=dtype)
+    qkva[..., 2 * C:] = qkva[..., 2 * C:] * 1.5 + 2
+    return qkva
+
+
+def check_loop(qkva, C, state=None, lengths=None, resets=None, train=True, fused=True):
+    """qkva (B, T, P, 3C) on the GPU, any strides; every output of forward and backward against the reference"""
+    dtype = qkva.dtype
+    B, T, P = qkva.shape[:3]
+    leaves = [qkva.detach().requires_grad_(train)] if fused else [t.detach().requires_grad_(train) for t in qkva.split(C, -1)]
+    st = None if state is None else state.cuda().requires_grad_(train)
+    cu = lambda t: None if t is None else t.cuda()
+    y, h = F.gate_loop(leaves[0] if fused else tuple(leaves), state=st, lengths=cu(lengths), resets=cu(resets), return_state=True)
+    parts = [t.cpu() for t in qkva.detach().split(C, -1)]
+    dy, dh = rnd(B, T, P, C, seed=90, dtype=dtype), rnd(B, P, C, seed=91)
+    ref = gate_loop_ref(*parts, state, lengths, resets, dy, dh, fast_exp=dtype == torch.bfloat16)
+    assert_within(y, ref['y'], dtype, 'y')
+    assert_within(h, ref['h'], torch.float32, 'h')
+    if not train:
+        return
+    grads = torch.autograd.grad((y, h), leaves + ([st] if st is not None else []), (dy.cuda(), dh.cuda()))
+    got = grads[0].split(C, -1) if fused else grads[:3]
+    for name, g in zip(('dq', 'dkv', 'da'), got):
+        assert_within(g, ref[name], dtype, name)
+    if st is not None:
+        assert_within(grads[-1], ref['dstate'], torch.float32, 'dstate')
+
+
+# lengths around the spans that the kernels keep, join and split along (8, 16, 32, 64, 256, 512 and their neighbours)
+LENGTHS = [1, 2, 7, 8, 9, 15, 17, 31, 33, 63, 64, 65, 255, 256, 257, 300, 511, 513, 1025]
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', LENGTHS)
+def test_gate_loop_lengths(T, dtype):
+    B, P, C = 2, 1, 72
+    check_loop(loop_inputs(B, T, P, C, dtype, T).cuda(), C, state=rnd(B, P, C, seed=1))
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('C', [1, 3, 4, 8, 12, 63, 64, 65, 130, 512, 1000])
+def test_gate_loop_widths(C, dtype):
+    B, T, P = 2, 70, 1
+    check_loop(loop_inputs(B, T, P, C, dtype, C).cuda(), C, state=rnd(B, P, C, seed=1))
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('B,T,P,C', [(2, 5, 16, 64), (1, 17, 9, 24), (3, 33, 5, 7), (2, 600, 3, 40), (1, 2, 1000, 8)])
+def test_gate_loop_pixels(B, T, P, C, dtype):
+    check_loop(loop_inputs(B, T, P, C, dtype, T).cuda(), C, state=rnd(B, P, C, seed=1))
+    check_loop(loop_inputs(B, T, P, C, dtype, T).cuda(), C, fused=False)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', [9, 300, 1100])
+@pytest.mark.parametrize('C', [64, 33])
+def test_padded_batch(T, C, dtype):
+    """lengths of zero, one, T, past T and below zero; what lies behind a sequence is never read (NaN), is zero in every result, and
+    a reset there changes nothing"""
+    lengths = torch.tensor([0, 1, T, T + 5, -3, T // 2, T - 1, 8])
+    B = len(lengths)
+    qkva = loop_inputs(B, T, 1, C, dtype, T)
+    clean = qkva.clone()
+    resets = rnd(B, T, seed=5) > 1.5
+    for b, n in enumerate(lengths.clamp(0, T).tolist()):
+        qkva[b, n:] = NAN
+        clean[b, n:] = 0
+        resets[b, n:] = True
+    state = rnd(B, 1, C, seed=1)
+    parts = clean.split(C, -1)
+    leaf, st = qkva.cuda().requires_grad_(), state.cuda().requires_grad_()
+    dy, dh = rnd(B, T, 1, C, seed=90, dtype=dtype), rnd(B, 1, C, seed=91)
+    dyn = dy.clone()
+    for b, n in enumerate(lengths.clamp(0, T).tolist()):
+        dyn[b, n:] = NAN                                  # nor are the gradients that arrive there
+    ref = gate_loop_ref(*parts, state, lengths, resets, dy, dh, fast_exp=dtype == torch.bfloat16)
+    for ln in (lengths, lengths.int()):
+        y, h = F.gate_loop(leaf, state=st, lengths=ln.cuda(), resets=resets.cuda(), return_state=True)
+        g, gs = torch.autograd.grad((y, h), (leaf, st), (dyn.cuda(), dh.cuda()))
+        assert_within(y, ref['y'], dtype, 'y')
+        assert_within(h, ref['h'], torch.float32, 'h')
+        for name, t in zip(('dq', 'dkv', 'da'), g.split(C, -1)):
+            assert_within(t, ref[name], dtype, name)
+        assert_within(gs, ref['dstate'], torch.float32, 'dstate')
+        for b, n in enumerate(lengths.clamp(0, T).tolist()):
+            assert not y[b, n:].any() and not g[b, n:].any()
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', [20, 700, 1500])
+def test_document_starts(T, dtype):
+    """every kind of start: the first token, the last, neighbours, none in a long run"""
+    B, C = 4, 40
+    resets = torch.zeros(B, T, dtype=torch.bool)
+    resets[0, 0] = resets[1, T - 1] = True
+    resets[2, T // 2: T // 2 + 3] = True
+    resets[3] = True
+    check_loop(loop_inputs(B, T, 1, C, dtype, T).cuda(), C, state=rnd(B, 1, C, seed=1), resets=resets)
+    check_loop(loop_inputs(B, T, 1, C, dtype, T).cuda(), C, state=rnd(B, 1, C, seed=1), resets=resets.to(torch.uint8) * 7, train=False)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', [24, 900])
+@pytest.mark.parametrize('poison', [NAN, INF, -INF])
+def test_nothing_crosses_a_document_start(T, dtype, poison):
+    """a document that holds infinities or NaN leaves its neighbours, forward and backward, as they are without it"""
+    B, C, cut, end = 1, 16, T // 3, 2 * T // 3
+    resets = torch.zeros(B, T, dtype=torch.bool)
+    resets[:, cut] = resets[:, end] = True
+    good = loop_inputs(B, T, 1, C, dtype, T)
+    bad = good.clone()
+    bad[:, cut:end] = poison
+    dy, dh = rnd(B, T, 1, C, seed=90, dtype=dtype).cuda(), rnd(B, 1, C, seed=91).cuda()
+    res = []
+    for z in (good, bad):
+        leaf = z.cuda().requires_grad_()
+        y, h = F.gate_loop(leaf, resets=resets.cuda(), return_state=True)
+        res.append((y, h, torch.autograd.grad((y, h), leaf, (dy, dh))[0]))
+    (y0, h0, g0), (y1, h1, g1) = res
+    assert torch.equal(h0, h1)
+    for s in (slice(0, cut), slice(end, T)):
+        assert torch.equal(y0[:, s], y1[:, s]) and torch.equal(g0[:, s], g1[:, s])
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', [12, 800])
+def test_extreme_decays(T, dtype):
+    """decays of exactly one and exactly zero (the type's largest and lowest values, infinities), and close to both"""
+    B, C = 2, 32
+    top = torch.finfo(dtype).max
+    qkva = loop_inputs(B, T, 1, C, dtype, T)
+    qkva[..., C:2 * C] *= 0.05                            # sums of T terms stay moderate
+    vals = torch.tensor([top, -top, INF, -INF, 30., -30., 12., -12.])
+    qkva[..., 2 * C:] = vals.to(dtype).repeat(C // 8)
+    check_loop(qkva.cuda(), C, state=rnd(B, 1, C, seed=1))
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_strides(dtype):
+    """batch and token axes exchanged, parts of wider rows, rows that start off a 16-byte boundary, repeated rows, transposed channels"""
+    B, T, P, C = 3, 70, 2, 16
+    base = loop_inputs(B, T, P, C, dtype)
+    for z in (loop_inputs(T, B, P, C, dtype, 1).cuda().transpose(0, 1),
+              loop_inputs(B, P, T, C, dtype, 2).cuda().transpose(1, 2),
+              torch.nn.functional.pad(base, (16, 24)).cuda()[..., 16:16 + 3 * C],
+              torch.nn.functional.pad(base, (1, 2)).cuda()[..., 1:1 + 3 * C],
+              base.cuda()[:1].expand(B, T, P, 3 * C),
+              base.cuda()[:, ::2],
+              base.cuda().transpose(2, 3).contiguous().transpose(2, 3)):
+        check_loop(z, C, state=rnd(B, P, C, seed=1))
+        check_loop(z, C, fused=False)
+    # three tensors whose strides differ
+    q, kv, a = (t.cuda() for t in base.split(C, -1))
+    y = F.gate_loop((q.contiguous(), kv, a.transpose(0, 1).contiguous().transpose(0, 1)))
+    assert torch.equal(y, F.gate_loop(base.cuda()))
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_rows_past_32_bit_offsets(dtype):
+    """two sequences more than 2^31 elements apart, and a token stride that leaves 32 bits"""
+    B, T, C = 2, 40, 32
+    far = (1 << 31) + 64
+    store = torch.zeros(far + T * 3 * C, dtype=dtype, device='cuda')
+    z = store.as_strided((B, T, 1, 3 * C), (far, 3 * C, 3 * C, 1))
+    z.copy_(loop_inputs(B, T, 1, C, dtype))
+    check_loop(z, C, state=rnd(B, 1, C, seed=1))
+    wide = 1 << 26                                        # 40 tokens: 2.7e9 elements
+    store = torch.zeros(T * wide + 3 * C, dtype=dtype, device='cuda')
+    z = store.as_strided((1, T, 1, 3 * C), (0, wide, 0, 1))
+    z.copy_(loop_inputs(1, T, 1, C, dtype))
+    check_loop(z, C)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T,C', [(20011, 8), (9000, 70), (33000, 3)])
+def test_long_sequences(T, C, dtype):
+    check_loop(loop_inputs(1, T, 1, C, dtype, T).cuda(), C, state=rnd(1, 1, C, seed=1))
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_steps_follow_the_whole_sequence(dtype):
+    """prefill, then token by token in place: states and outputs of the one call over all tokens"""
+    B, T, C, pre = 3, 40, 72, 29
+    z = loop_inputs(B, T, 1, C, dtype).squeeze(2).cuda()
+    parts = [t.cpu().unsqueeze(2) for t in z.split(C, -1)]
+    ref = gate_loop_ref(*parts, fast_exp=dtype == torch.bfloat16)
+    y, state = F.gate_loop(z[:, :pre], return_state=True)
+    ys = [y]
+    for t in range(pre, T):
+        if t % 2:
+            ys.append(F.gate_loop_step(z[:, t], state)[:, None])
+        else:
+            new = torch.full_like(state, NAN)
+            ys.append(F.gate_loop_step(tuple(z[:, t].split(C, -1)), state, state_out=new)[:, None])
+            state = new
+    assert_within(torch.cat(ys, 1), ref['y'], dtype, 'y')
+    assert_within(state, ref['h'], torch.float32, 'h')
+    pix = loop_inputs(2, 1, 6, 24, dtype).cuda()
+    s0 = rnd(2, 6, 24, seed=3).cuda()
+    y, h = F.gate_loop(pix, state=s0, return_state=True)
+    s = s0.clone()
+    assert torch.equal(F.gate_loop_step(pix[:, 0], s), y[:, 0]) and torch.equal(s, h)
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_last_state_written_over_the_first(dtype):
+    """the C ABI lets h_last be h0 itself, for any length"""
+    for B, T, C in ((2, 1, 64), (2, 600, 40), (1, 5000, 64), (1, 5000, 9)):
+        z = loop_inputs(B, T, 1, C, dtype).cuda()
+        ops = F._ops(z.device)
+        s0 = rnd(B, C, seed=2).cuda()
+        y, h = F.gate_loop(z, state=s0[:, None], return_state=True)
+        geo = F._loop_geometry(ops, {torch.bfloat16: 0, torch.float32: 1}[dtype], (B, T, 1, C), (z.stride(0) if B > 1 else 0, z.stride(1) if T > 1 else 0, 0), True)
+        s, y2 = s0.clone(), torch.empty_like(y)
+        ops.gateloop_forward(geo.desc, *z.split(C, -1), s, None, None, y2, s, None, F._bytes(ops, geo.ws_forward))(ops.current_stream())
+        assert torch.equal(s, h[:, 0]) and torch.equal(y2, y)
+
+
+def test_results_do_not_change_from_call_to_call():
+    z = loop_inputs(2, 5000, 1, 136, torch.bfloat16).cuda().requires_grad_()
+    w = [torch.ones(136, device='cuda', requires_grad=True) for _ in range(3)]
+    first = None
+    for _ in range(4):
+        y, h = F.gate_loop(z, return_state=True)
+        g = torch.autograd.grad((y, h), z, (torch.ones_like(y), torch.ones_like(h)))[0]
+        out, n = F.block_norm(y, y * 2, gate=y, post_gamma=w[0], scale=w[1], pre_gamma=w[2])
+        gw = torch.autograd.grad((out, n), w, (y, y))
+        now = [y, h, g, out, n, *gw]
+        if first is None:
+            first = now
+        assert all(torch.equal(a, b) for a, b in zip(first, now))
+
+
+# ----------------------------------------------------------------------------------------------------------------- block norm
+def check_norm(R, C, dtype, act='silu', branch=True, gate=True, post=True, scale=True, pre=True, make=None, train=True, up=('dout', 'dn'), seed=0):
+    make = make or (lambda t: t.cuda())
+    row = lambda i, std=1.: rnd(R, C, seed=seed + i, dtype=dtype, std=std)
+    vec = lambda i: rnd(C, seed=seed + 10 + i, mean=1., std=0.3)
+    t = dict(x=row(0, 2.))
+    if branch:
+        t['branch'] = row(1)
+        if gate:
+            t['gate'] = row(2, 3.)
+        if post:
+            t['post'] = vec(0)
+        if scale:
+            t['scale'] = vec(1)
+    if pre:
+        t['pre'] = vec(2)
+    return run_norm(t, act, make, train, up)
+
+
+def run_norm(t, act, make, train=True, up=('dout', 'dn')):
+    dtype = t['x'].dtype
+    d = {k: (make(v) if v.dim() == 2 else v.cuda()).detach().requires_grad_(train) for k, v in t.items()}
+    out, n = F.block_norm(d['x'], d.get('branch'), gate=d.get('gate'), gate_act=act, post_gamma=d.get('post'), scale=d.get('scale'), pre_gamma=d.get('pre'))
+    ups = {}
+    if 'branch' in t and 'dout' in up:
+        ups['dout'] = rnd(*t['x'].shape, seed=80, dtype=dtype)
+    if 'pre' in t and 'dn' in up:
+        ups['dn'] = rnd(*t['x'].shape, seed=81, dtype=dtype)
+    ref = block_norm_ref(t['x'], t.get('branch'), t.get('gate'), act, t.get('post'), t.get('scale'), t.get('pre'), grads=train, **ups)
+    for name, v in (('out', out), ('normed', n)):
+        if name in ref:
+            assert_within(v, ref[name], dtype, name)
+    if not train:
+        return
+    outs = [v for k, v in (('dout', out), ('dn', n)) if k in ups]
+    names = [k for k in t if not (k == 'pre' and 'dn' not in ups)]
+    grads = torch.autograd.grad(outs, [d[k] for k in names], [v.cuda() for v in ups.values()])
+    for k, g in zip(names, grads):
+        assert_within(g, ref['d' + k], dtype if t[k].dim() == 2 else torch.float32, 'd' + k)
+
+
+# widths around the thread and chunk counts of a row (64, 256, 512, 1024 threads; chunks of 1, 4 and 8), up to the widest
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('C', [1, 2, 7, 8, 16, 63, 64, 72, 127, 255, 256, 257, 500, 512, 520, 1001, 1023, 1032, 2048, 2056, 4096, 4100, 5001, 8192, 8200, 16383, 16384])
+def test_block_norm_widths(C, dtype):
+    check_norm(5, C, dtype)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('R', [1, 2, 3, 31, 33, 257, 5000])
+@pytest.mark.parametrize('C', [24, 130])
+def test_block_norm_rows(R, C, dtype):
+    check_norm(R, C, dtype)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('act', ['silu', 'sigmoid', 'none'])
+@pytest.mark.parametrize('C', [64, 33])
+def test_block_norm_parts(act, C, dtype):
+    for mask in range(16):
+        gate, post, scale, pre = (bool(mask >> i & 1) for i in range(4))
+        check_norm(9, C, dtype, act, True, gate, post, scale, pre)
+    check_norm(9, C, dtype, branch=False)
+    check_norm(9, C, dtype, up=('dout',))
+    check_norm(9, C, dtype, up=('dn',))
+    check_norm(9, C, dtype, train=False)
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_block_norm_strides(dtype):
+    """thirds of a fused projection, rows off a 16-byte boundary, transposed rows, repeated rows, leading axes"""
+    C, R = 40, 12
+
+    def part(t, lo, width):
+        w = torch.zeros(R, width, dtype=dtype, device='cuda')
+        v = w[:, lo:lo + C]
+        v.copy_(t)
+        return v
+    for make in (lambda t: part(t, 16, 160), lambda t: part(t, 3, 47), lambda t: t.t().contiguous().t().cuda(),
+                 lambda t: part(t, 0, 80)):
+        check_norm(R, C, dtype, make=make)
+    x = rnd(2, 6, C, dtype=dtype).cuda()
+    g = torch.ones(C, device='cuda')
+    o1, n1 = F.block_norm(x, x.transpose(0, 1).contiguous().transpose(0, 1), pre_gamma=g)
+    o2, n2 = F.block_norm(x.reshape(12, C), x.reshape(12, C), pre_gamma=g)
+    assert o1.shape == x.shape and torch.equal(o1.reshape(12, C), o2) and torch.equal(n1.reshape(12, C), n2)
+    row = x[0, :1].expand(R, C)
+    o3, _ = F.block_norm(row, row, pre_gamma=g)
+    assert torch.equal(o3, o2[:1].expand(R, C))
+    o4, n4 = F.block_norm(x[0, 0], x[0, 0], pre_gamma=g)
+    assert o4.shape == (C,) and torch.equal(n4, n2[0])
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('C', [48, 37])
+def test_block_norm_rows_of_zeros_and_extremes(C, dtype):
+    """rows of zeros (the floor of the norm: N is linear there), of tiny numbers, and gates at the ends of the type"""
+    R = 6
+    t = dict(x=rnd(R, C, dtype=dtype), branch=rnd(R, C, seed=1, dtype=dtype), gate=rnd(R, C, seed=2, dtype=dtype), post=rnd(C, seed=3, mean=1.),
+             scale=rnd(C, seed=4), pre=rnd(C, seed=5, mean=1.))
+    t['branch'][0] = 0
+    t['x'][1] = 0
+    t['branch'][1] = 0                                    # both norms at their floor
+    t['x'][2] *= 1e-6
+    t['branch'][2] *= 1e-6
+    top = torch.finfo(dtype).max
+    t['gate'][3] = torch.tensor([top, -top, 90., -90.]).repeat(C // 4 + 1)[:C].to(dtype)
+    zeroed = dict(t, x=t['x'].clone(), branch=t['branch'].clone(), gate=t['gate'].clone())
+    for act in ('silu', 'sigmoid'):
+        if act == 'silu':                                 # silu of the largest number overflows the row by design
+            zeroed['gate'][3] = torch.tensor([60., -top, 90., -90.]).repeat(C // 4 + 1)[:C].to(dtype)
+        run_norm(zeroed if act == 'silu' else t, act, lambda v: v.cuda())
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_a_row_of_nan_stays_in_its_row(dtype):
+    R, C = 70, 24
+    x, b = rnd(R, C, dtype=dtype).cuda(), rnd(R, C, seed=1, dtype=dtype).cuda()
+    g = torch.ones(C, device='cuda')
+    o1, n1 = F.block_norm(x, b, post_gamma=g, pre_gamma=g)
+    b2 = b.clone()
+    b2[33] = NAN
+    o2, n2 = F.block_norm(x, b2, post_gamma=g, pre_gamma=g)
+    rest = torch.arange(R, device='cuda') != 33
+    assert o2[33].isnan().all() and n2[33].isnan().all() and torch.equal(o1[rest], o2[rest]) and torch.equal(n1[rest], n2[rest])
+
+
+def test_block_norm_rows_past_32_bit_offsets():
+    C, R = 64, 40
+    step = 1 << 20
+    far = torch.zeros((1 << 31) + 64 + R * C, dtype=torch.bfloat16, device='cuda')
+    x = far[-R * C:].view(R, C)
+    x.copy_(rnd(R, C, dtype=torch.bfloat16))
+    wide = torch.zeros(2100 * step, dtype=torch.bfloat16, device='cuda').view(2100, step)[:, 8:8 + C]      # the last row begins past 2^31 elements
+    val = rnd(2100, C, seed=1, dtype=torch.bfloat16)
+    wide.copy_(val)
+    g = torch.ones(C, device='cuda')
+    o, n = F.block_norm(wide, wide, pre_gamma=g)
+    ref = block_norm_ref(val, val, pre=torch.ones(C))
+    assert_within(o, ref['out'], torch.bfloat16, 'out')
+    assert_within(n, ref['normed'], torch.bfloat16, 'normed')
+    assert_within(F.block_norm(x, pre_gamma=g)[1], block_norm_ref(rnd(R, C, dtype=torch.bfloat16), pre=torch.ones(C))['normed'], torch.bfloat16, 'normed')
+
+
+# ----------------------------------------------------------------------------------------------------------------- as used together
+def two_blocks(x, weights, lengths=None, states=None, gate=F.gate_loop, norm=F.block_norm):
+    """norm, projection, recurrence, norm / gate / scale / residual add and the next norm: two blocks; x (B, T, C)"""
+    C = x.shape[-1]
+    _, n = norm(x, pre_gamma=weights['n0'])
+    new = []
+    for i in range(2):
+        z = n @ weights[f'p{i}'].t()
+        y, s = gate(z[..., :3 * C], state=None if states is None else states[i], lengths=lengths, return_state=True)
+        new.append(s)
+        x, n = norm(x, y, gate=z[..., 3 * C:], post_gamma=weights[f'w{i}'], scale=weights[f's{i}'], pre_gamma=weights[f'n{i + 1}'])
+    return n, new
+
+
+def block_weights(C, dtype=torch.float32):
+    w = {f'p{i}': (rnd(4 * C, C, seed=i) / C ** 0.5).to(dtype) for i in range(2)}
+    w.update({f'{k}{i}': rnd(C, seed=20 + 3 * i + j, mean=1., std=0.2) for j, k in enumerate('nws') for i in range(3)})
+    return {k: v for k, v in w.items() if k not in ('w2', 's2')}
+
+
+def plain_gate(z, state=None, lengths=None, return_state=True):
+    C = z.shape[-1] // 3
+    q, kv, a = z.split(C, -1)
+    h = torch.zeros_like(q[:, 0]) if state is None else state
+    ys = []
+    for t in range(z.shape[1]):
+        on = (torch.full((z.shape[0],), z.shape[1]) if lengths is None else lengths)[:, None] > t
+        h = torch.where(on, torch.sigmoid(a[:, t]) * h + kv[:, t], h)
+        ys.append(torch.where(on, q[:, t] * h, torch.zeros_like(h)))
+    return torch.stack(ys, 1), h
+
+
+def plain_norm(x, branch=None, gate=None, post_gamma=None, scale=None, pre_gamma=None):
+    N = lambda v, w: torch.nn.functional.normalize(v, dim=-1) * v.shape[-1] ** 0.5 * w
+    if branch is not None:
+        x = x + scale * torch.nn.functional.silu(gate) * N(branch, post_gamma)
+    return x, N(x, pre_gamma)
+
+
+def test_two_blocks_train_and_decode():
+    """the operators in a chain, in 32 bits: outputs, states and every gradient against the same chain in 64 bits; then prefill and
+    single tokens against the whole sequence.  Tolerance: the chain multiplies errors of 1e-7 by its condition, of order 100 here (two norms,
+    two recurrences and two projections of unit gain, gradients up to ten times larger): 2e-5 of each result's largest value."""
+    B, T, C = 2, 37, 48
+    w = block_weights(C)
+    x = rnd(B, T, C, seed=50)
+    lengths = torch.tensor([T, 20])
+    w64 = {k: v.double().requires_grad_() for k, v in w.items()}
+    x64 = x.double().requires_grad_()
+    n64, s64 = two_blocks(x64, w64, lengths, gate=plain_gate, norm=plain_norm)
+    up = rnd(B, T, C, seed=51)
+    live = (torch.arange(T)[None] < lengths[:, None])[..., None]
+    want = torch.autograd.grad((n64 * live * up.double()).sum() + s64[0].sum() + s64[1].sum(), [x64, *w64.values()])
+    wg = {k: v.cuda().requires_grad_() for k, v in w.items()}
+    xg = x.cuda().requires_grad_()
+    n, s = two_blocks(xg, wg, lengths.cuda())
+    got = torch.autograd.grad((n * live.cuda() * up.cuda()).sum() + s[0].sum() + s[1].sum(), [xg, *wg.values()])
+    for what, a, b in [('n', n * live.cuda(), n64 * live), ('s0', s[0], s64[0]), ('s1', s[1], s64[1])] + list(zip(['x', *w], got, want)):
+        assert (a.detach().double().cpu() - b.detach()).abs().max() <= 2e-5 * b.detach().abs().max(), what
+    with torch.no_grad():
+        full, last = two_blocks(xg[:1], wg)
+        pre, st = two_blocks(xg[:1, :30], wg)
+        assert (pre - full[:, :30]).abs().max() <= 2e-5 * full.abs().max()
+        for t in range(30, T):
+            tok = xg[:1, t]
+            _, nn = F.block_norm(tok, pre_gamma=wg['n0'])
+            for i in range(2):
+                z = nn @ wg[f'p{i}'].t()
+                y = F.gate_loop_step(z[:, :3 * C], st[i])
+                tok, nn = F.block_norm(tok, y, gate=z[:, 3 * C:], post_gamma=wg[f'w{i}'], scale=wg[f's{i}'], pre_gamma=wg[f'n{i + 1}'])
+            assert (nn - full[:, t]).abs().max() <= 2e-5 * full.abs().max()
+        for a, b in zip(st, last):
+            assert (a - b).abs().max() <= 2e-5 * b.abs().max()
+
+
+@pytest.mark.parametrize('T,C', [(40, 64), (3000, 40)])
+def test_captured_and_replayed(T, C):
+    """forward and backward of both operators in one graph, replayed on new inputs with eager work of the same operators in between"""
+    B, dtype = 2, torch.bfloat16
+    w = [torch.ones(C, device='cuda', requires_grad=True) for _ in range(3)]
+    data = [loop_inputs(B, T, 1, C, dtype, s).squeeze(2).cuda() for s in range(4)]
+    lengths = torch.tensor([T, T // 2], dtype=torch.int32, device='cuda')
+
+    def work(z):
+        y, h = F.gate_loop(z, lengths=lengths, return_state=True)
+        out, n = F.block_norm(z[..., :C], y, gate=z[..., C:2 * C], post_gamma=w[0], scale=w[1], pre_gamma=w[2])
+        g = torch.autograd.grad((out, n, h), [z, *w], (torch.ones_like(out), torch.ones_like(n), torch.ones_like(h)))
+        return [t.detach() for t in (y, h, out, n)] + list(g)
+    eager = [[t.clone() for t in work(z.clone().requires_grad_())] for z in data]
+    static = data[0].clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = work(static)
+    for rep in (0, 1, 2, 3, 1):
+        with torch.no_grad():
+            static.copy_(data[rep])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, eager[rep]):
+            assert torch.equal(a, b)
+        again = work(data[rep].clone().requires_grad_())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(again, eager[rep]))
+
+
+def test_two_graphs_and_two_streams_at_once():
+    """two captured calls replayed on two streams, with eager calls on a third: each has its own workspaces"""
+    C, T = 64, 20000
+    data = [loop_inputs(1, T, 1, C, torch.bfloat16, s).squeeze(2).cuda() for s in range(3)]
+    want = [F.gate_loop(z, return_state=True) for z in data]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(3)]
+    for z in data[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(F.gate_loop(z, return_state=True))
+        graphs.append(g)
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            third = F.gate_loop(data[2], return_state=True)
+        torch.cuda.synchronize()
+        for got, ref in zip(outs + [third], want):
+            assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+def test_second_derivatives_are_refused():
+    z = loop_inputs(1, 4, 1, 8, torch.float32).cuda().requires_grad_()
+    g = torch.autograd.grad(F.gate_loop(z).square().sum(), z, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), z)
+
+
+def test_inputs_changed_before_the_backward_pass_are_refused():
+    z = loop_inputs(1, 4, 1, 8, torch.float32).cuda()
+    s = torch.zeros(1, 1, 8, device='cuda', requires_grad=True)
+    y = F.gate_loop(z, state=s)
+    z.add_(1)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+def test_step_kernels_leave_neighbours_alone():
+    """guard values around every output"""
+    for dtype in DT:
+        for C in (8, 13):
+            B = 3
+            z = loop_inputs(B, 1, 1, C, dtype).view(B, 3 * C).cuda()
+            pool = torch.full((B * C + 64,), 7., device='cuda')
+            state = pool[32:32 + B * C].view(B, C)
+            state.zero_()
+            F.gate_loop_step(z, state)
+            assert (pool[:32] == 7).all() and (pool[32 + B * C:] == 7).all()
+            assert torch.equal(state, z[:, C:2 * C].float())
