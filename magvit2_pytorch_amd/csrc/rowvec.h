@@ -6,12 +6,14 @@
 template <typename E, int V> struct RowVec {
     static_assert(V == E::kVec, "a 16-byte chunk or one element");
     i32x4 v;
+    __device__ __forceinline__ void clear() { v = i32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void load(const void* p, int64_t i) { v = *(const i32x4*)((const typename E::T*)p + i); }
     __device__ __forceinline__ void get(float* f) const { Chunk<E>::unpack(v, f); }
     static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { *(i32x4*)((typename E::T*)p + i) = Chunk<E>::pack(f); }
 };
 template <typename E> struct RowVec<E, 1> {
     typename E::T v;
+    __device__ __forceinline__ void clear() { v = 0; }
     __device__ __forceinline__ void load(const void* p, int64_t i) { v = ((const typename E::T*)p)[i]; }
     __device__ __forceinline__ void get(float* f) const { f[0] = ld_elem<E>(&v, 0); }
     static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { st_elem<E>(p, i, f[0]); }

@@ -228,6 +228,8 @@ def test_abi_refuses_before_any_launch():
     assert lib.mv2_gateloop_forward(None, ptr, ptr, ptr, None, None, None, ptr, None, None, None, 0, None) == EINVAL
     long = L(T=100000)
     assert lib.mv2_gateloop_states(ctypes.byref(long)) > 0 and bwd(long, st=None, ws=1 << 40) == EINVAL          # a backward pass needs the kept states
+    need = lib.mv2_gateloop_workspace_bytes(ctypes.byref(long), 0)
+    assert need > 0 and fwd(long) == EWORKSPACE and bwd(long) == EWORKSPACE                                       # spans meet in a workspace
     N = lambda **kw: ops_hip.BlockNormDesc(**{**dict(dtype=0, C=8, rows=4, x_stride=8, branch_stride=8, gate_stride=8, gate_act=2, reserved=0), **kw})
 
     def nf(d, x=ptr, b=ptr, g=ptr, post=ptr, sc=ptr, pre=ptr, out=ptr, n=ptr):
