@@ -35,7 +35,7 @@ struct LoopArgs {
 };
 
 #define LOOP_STEPS 8               // tokens between two kept states of the walking kernels
-#define SPAN_KEEP 128              // and of the spans
+#define SPAN_KEEP 256              // and of the spans: tokens of a workgroup
 
 __device__ __forceinline__ int live_tokens(const LoopArgs& A, int b) {
     if (!A.lengths) return A.T;
@@ -188,16 +188,16 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
 }
 
 // --------------------------------------------------------------------------- spans of tokens joined along the sequence
-// The walking kernels above leave the chip empty where there are few channels and many tokens.  Here a workgroup of WAVES waves owns
-// WAVES * 32 tokens of CL * V channels of one sequence (a "block"): a lane holds L consecutive tokens of V channels in registers (every
-// element is read once), CL lanes side by side read whole 128-byte pieces of rows, and the 64 / CL lane rows of a wave, the waves, and the
-// blocks of a sequence are joined through the pair (A, H) of a span: it takes the state h in front of it to A h + H, and spans join as
-// (A1, H1) (A2, H2) -> (A1 A2, A2 H1 + H2).
+// The walking kernels above leave the chip empty where there are few channels and many tokens.  Here a workgroup owns WAVES * TW tokens of
+// CL * V channels of one sequence (a "block"): a lane holds L consecutive tokens of V channels in registers (every element is read once),
+// CL lanes side by side read whole 128-byte pieces of rows.  Lane rows and blocks are joined through the pair (A, H) of a span: it takes the
+// state h in front of it to A h + H, and spans join as (A1, H1) (A2, H2) -> (A1 A2, A2 H1 + H2).  Within the workgroup the pairs meet in LDS,
+// where thread (channel, segment) takes a run of lane rows, and come back as the state in front of each lane row.
 // Between workgroups: a block publishes its pair and reads the pairs of the blocks before it in its group of LOOP_GROUP blocks, and the
 // state that the last block of the group before published: always the same pairs in the same order, so results do not depend on timing.
 // Every wait ends: a block's place in the order is the ticket it draws when it starts, blocks wait for lower tickets only - for workgroups
 // that are running - and a pair is published before its block waits for anything.
-#define LOOP_GROUP 32
+#define LOOP_GROUP 16
 #define LOOP_CUT 2.f               // A of a span in which a document starts (products of decays are <= 1 or NaN): nothing passes through it
 typedef unsigned long long u64;
 
@@ -207,44 +207,63 @@ __device__ __forceinline__ bool pair_there(u64 w) { return (w >> 63) != 0; }
 __device__ __forceinline__ float pair_A(u64 w) { return __uint_as_float((unsigned)(w >> 32) & 0x7fffffffu); }
 __device__ __forceinline__ float pair_H(u64 w) { return __uint_as_float((unsigned)w); }
 __device__ __forceinline__ void publish(u64* p, float A, float H) { __hip_atomic_store(p, pair_word(A, H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// state behind a span, from the state in front of it; CUTS: may documents start in it?
+template <bool CUTS> __device__ __forceinline__ float pass(float A, float H, float h) {
+    const float r = fmaf(A, h, H);
+    return CUTS && A == LOOP_CUT ? H : r;
+}
 // (A, H) := (A, H) then (A2, H2)
-__device__ __forceinline__ void join(float& A, float& H, float A2, float H2) {
-    const bool cut2 = A2 == LOOP_CUT;
-    H = cut2 ? H2 : fmaf(A2, H, H2);
-    A = (cut2 || A == LOOP_CUT) ? LOOP_CUT : A * A2;
+template <bool CUTS> __device__ __forceinline__ void join(float& A, float& H, float A2, float H2) {
+    H = pass<CUTS>(A2, H2, H);
+    const float r = A * A2;
+    A = CUTS && (A == LOOP_CUT || A2 == LOOP_CUT) ? LOOP_CUT : r;
 }
 
+// Tiles are dealt to `nq` queues of neighbours, workgroup i draws from queue i % nq: with 8 queues neighbouring tiles, which share cache lines
+// where rows are not whole lines, stay on one XCD (workgroups go to the XCDs in turn; nothing but speed depends on it).
 struct SpanWork {
-    unsigned* ticket;
+    unsigned* ticket;              // one per queue, 64 bytes apart
     u64* pairs;                    // [block][tile][channel of the tile]
     u64* states;                   // [group][tile][channel of the tile]: the state behind a whole group
-    int nblk, ntile, ctiles;
+    int nblk, ntile, ctiles, nq;
 };
 
-// What a workgroup's channels receive from the blocks before this one (in the direction of the recurrence): block `kb` counts in that
-// direction, `first` is what block 0 starts from.  Entered by all threads with (A, H) of the whole block in totA / totH (LDS, published here);
-// on return carry[ch] holds the state in front of the block.
-template <int NCH, int THREADS>
-__device__ __forceinline__ void span_carry(const SpanWork& W, int kb, int tile, bool ok, float first, const float* totA, const float* totH, float* carry,
-                                           float (*partA)[NCH], float (*partH)[NCH]) {
-    constexpr int SLOTS = THREADS / NCH, M = LOOP_GROUP / SLOTS;
-    static_assert(SLOTS * M == LOOP_GROUP, "slots share a group evenly");
-    const int tid = threadIdx.x, ch = tid % NCH, slot = tid / NCH;
-    if (W.nblk == 1) {
-        if (tid < NCH) carry[ch] = first;
+// (block in the direction of the recurrence, tile) of this workgroup; false: its queue is empty, the workgroup ends
+__device__ __forceinline__ bool span_place(const SpanWork& W, int& kb, int& tile) {
+    __shared__ unsigned drawn;
+    if (W.nblk == 1) { kb = 0; tile = blockIdx.x; return true; }
+    const unsigned x = blockIdx.x % (unsigned)W.nq;
+    if (threadIdx.x == 0) drawn = __hip_atomic_fetch_add(W.ticket + 16 * x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const unsigned lo = (unsigned)((u64)x * W.ntile / W.nq), cnt = (unsigned)((u64)(x + 1) * W.ntile / W.nq) - lo;
+    kb = (int)(drawn / cnt); tile = (int)(lo + drawn % cnt);
+    return kb < W.nblk;
+}
+
+// State of the recurrence in front of this workgroup's block for channel ch (thread = (ch, seg), SEGS threads per channel).  kb counts blocks in
+// the direction of the recurrence, (A, H) is the whole block's pair (known to the threads of the last segment, which publish it), `first` what
+// block 0 starts from (the same threads).  All threads enter; everyone gets the state.
+template <int NCH, int SEGS, bool CUTS>
+__device__ __forceinline__ float span_carry(const SpanWork& W, int kb, int tile, int ch, int seg, bool ok, float first, float A, float H,
+                                            float (*partA)[NCH], float (*partH)[NCH]) {
+    constexpr int M = LOOP_GROUP / SEGS;
+    static_assert(SEGS * M == LOOP_GROUP, "the threads of a channel share a group evenly");
+    const bool tail = seg == SEGS - 1;
+    if (kb == 0) {
+        if (tail) {
+            partH[0][ch] = first;
+            // block 0 publishes a state rather than a pair: whoever depends on it does not read `first` again, which may be overwritten by then
+            if (ok && W.nblk > 1) publish(W.pairs + (int64_t)tile * NCH + ch, LOOP_CUT, pass<CUTS>(A, H, first));
+        }
         __syncthreads();
-        return;
+        return partH[0][ch];
     }
-    u64* mine = W.pairs + ((int64_t)kb * W.ntile + tile) * NCH;
-    if (tid < NCH && ok) {
-        // block 0 publishes a state rather than a pair: whoever depends on it does not read `first` again, which may be overwritten by then
-        if (kb == 0) publish(mine + ch, LOOP_CUT, totA[ch] == LOOP_CUT ? totH[ch] : fmaf(totA[ch], first, totH[ch]));
-        else publish(mine + ch, totA[ch], totH[ch]);
-    }
+    if (ok && tail) publish(W.pairs + ((int64_t)kb * W.ntile + tile) * NCH + ch, A, H);
     const int grp = kb / LOOP_GROUP, in = kb % LOOP_GROUP;
-    const int lead = grp > 0 ? 1 : 0, count = lead + in;      // the group before, then the blocks of this group
-    float A = 1.f, H = 0.f;
-    if (ok && kb > 0) {
+    const int lead = grp > 0 ? 1 : 0, count = lead + in;      // the state behind the group before, then the blocks of this group
+    float a = 1.f, h = 0.f;
+    if (ok) {
         u64 w[M];
 #pragma unroll
         for (int j = 0; j < M; ++j) w[j] = 0;
@@ -253,7 +272,7 @@ __device__ __forceinline__ void span_carry(const SpanWork& W, int kb, int tile, 
             all = true;
 #pragma unroll
             for (int j = 0; j < M; ++j) {
-                const int e = slot * M + j;
+                const int e = seg * M + j;
                 if (e < count && !pair_there(w[j])) {
                     const u64* p = e < lead ? W.states + ((int64_t)(grp - 1) * W.ntile + tile) * NCH
                                             : W.pairs + ((int64_t)(grp * LOOP_GROUP + e - lead) * W.ntile + tile) * NCH;
@@ -265,166 +284,123 @@ __device__ __forceinline__ void span_carry(const SpanWork& W, int kb, int tile, 
         } while (!all);
 #pragma unroll
         for (int j = 0; j < M; ++j)
-            if (slot * M + j < count) join(A, H, pair_A(w[j]), pair_H(w[j]));
+            if (seg * M + j < count) join<true>(a, h, pair_A(w[j]), pair_H(w[j]));
     }
-    partA[slot][ch] = A; partH[slot][ch] = H;
+    partA[seg][ch] = a; partH[seg][ch] = h;
     __syncthreads();
-    if (tid < NCH) {
-        float h = first;
-        if (kb > 0) {
-            A = 1.f; H = 0.f;
+    h = partH[0][ch];                                         // the first entry is a state: nothing in front of it counts
 #pragma unroll
-            for (int s = 0; s < SLOTS; ++s) join(A, H, partA[s][ch], partH[s][ch]);
-            h = H;                                            // the first entry is a state: nothing in front of it counts
-        }
-        carry[ch] = h;
-        if (ok && in == LOOP_GROUP - 1 && kb + 1 < W.nblk)
-            publish(W.states + ((int64_t)grp * W.ntile + tile) * NCH + ch, LOOP_CUT, totA[ch] == LOOP_CUT ? totH[ch] : fmaf(totA[ch], h, totH[ch]));
-    }
-    __syncthreads();
+    for (int s = 1; s < SEGS; ++s) h = pass<true>(partA[s][ch], partH[s][ch], h);
+    if (ok && tail && in == LOOP_GROUP - 1 && kb + 1 < W.nblk)
+        publish(W.states + ((int64_t)grp * W.ntile + tile) * NCH + ch, LOOP_CUT, pass<CUTS>(A, H, h));
+    return h;
 }
 
-// pairs of the waves -> what is in front of each wave; totals of the block.  In the direction of the recurrence (REV: last wave first).
-template <int NCH, int WAVES, bool REV>
-__device__ __forceinline__ void wave_prefix(float (*sA)[NCH], float (*sH)[NCH], float* totA, float* totH) {
-    const int ch = threadIdx.x;
-    if (ch < NCH) {
-        float A = 1.f, H = 0.f;
+// Lane rows of a workgroup, ROWS of them, in LDS: row r's pair at rowA[r], rowH[r].  Replaces rowH[r] by the state in front of row r (REV: the
+// recurrence runs from the last row to the first).  partA / partH: SEGS rows of scratch each.  All threads enter, after a barrier; leaves behind one.
+template <int NCH, int SEGS, int ROWS, bool REV, bool CUTS>
+__device__ __forceinline__ void span_join(const SpanWork& W, int kb, int tile, bool ok, float first, const float (*rowA)[NCH], float (*rowH)[NCH],
+                                          float (*partA)[NCH], float (*partH)[NCH], float (*prevA)[NCH], float (*prevH)[NCH]) {
+    constexpr int RPS = ROWS / SEGS;
+    const int ch = threadIdx.x % NCH, seg = threadIdx.x / NCH;
+    float ra[RPS], rh[RPS], A = 1.f, H = 0.f;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            const int w = REV ? WAVES - 1 - i : i;
-            const float a2 = sA[w][ch], h2 = sH[w][ch];
-            sA[w][ch] = A; sH[w][ch] = H;
-            join(A, H, a2, h2);
-        }
-        totA[ch] = A; totH[ch] = H;
+    for (int j = 0; j < RPS; ++j) {
+        const int r = REV ? ROWS - 1 - (seg * RPS + j) : seg * RPS + j;
+        ra[j] = rowA[r][ch]; rh[j] = rowH[r][ch];
+        join<CUTS>(A, H, ra[j], rh[j]);
     }
-}
-
-// joins the lane rows of a wave: on entry a lane's own pair, on return the pair in front of the lane; the wave's whole pair goes to LDS
-template <int V, int CL, bool REV>
-__device__ __forceinline__ void lane_prefix(float* A, float* H, float* waveA, float* waveH) {
-    constexpr int TL = 64 / CL;
-    const int lane = threadIdx.x & 63, r = REV ? TL - 1 - lane / CL : lane / CL, cl = lane % CL;
-#pragma unroll
-    for (int d = 1; d < TL; d *= 2) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            float a0 = REV ? __shfl_down(A[k], d * CL, 64) : __shfl_up(A[k], d * CL, 64);
-            float h0 = REV ? __shfl_down(H[k], d * CL, 64) : __shfl_up(H[k], d * CL, 64);
-            if (r >= d) { join(a0, h0, A[k], H[k]); A[k] = a0; H[k] = h0; }
-        }
-    }
-    if (r == TL - 1)
-#pragma unroll
-        for (int k = 0; k < V; ++k) { waveA[cl * V + k] = A[k]; waveH[cl * V + k] = H[k]; }
-    if (TL > 1) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float a0 = REV ? __shfl_down(A[k], CL, 64) : __shfl_up(A[k], CL, 64);
-            const float h0 = REV ? __shfl_down(H[k], CL, 64) : __shfl_up(H[k], CL, 64);
-            A[k] = r == 0 ? 1.f : a0; H[k] = r == 0 ? 0.f : h0;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) { A[k] = 1.f; H[k] = 0.f; }
-    }
-}
-
-// (block in the direction of the recurrence, tile) of this workgroup
-__device__ __forceinline__ void span_place(const SpanWork& W, int& kb, int& tile) {
-    __shared__ unsigned drawn;
-    if (W.nblk == 1) { kb = 0; tile = blockIdx.x; return; }
-    if (threadIdx.x == 0) drawn = __hip_atomic_fetch_add(W.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    partA[seg][ch] = A; partH[seg][ch] = H;
     __syncthreads();
-    kb = (int)(drawn / (unsigned)W.ntile); tile = (int)(drawn % (unsigned)W.ntile);
+    float fa = 1.f, fh = 0.f;                                 // everything in front of this segment
+    for (int s = 0; s < seg; ++s) join<CUTS>(fa, fh, partA[s][ch], partH[s][ch]);
+    join<CUTS>(A = fa, H = fh, partA[seg][ch], partH[seg][ch]);
+    const float h0 = span_carry<NCH, SEGS, CUTS>(W, kb, tile, ch, seg, ok, first, A, H, prevA, prevH);
+    float h = pass<CUTS>(fa, fh, h0);
+#pragma unroll
+    for (int j = 0; j < RPS; ++j) {
+        const int r = REV ? ROWS - 1 - (seg * RPS + j) : seg * RPS + j;
+        rowH[r][ch] = h;
+        h = pass<CUTS>(ra[j], rh[j], h);
+    }
+    __syncthreads();
 }
 
 __global__ __launch_bounds__(256) void span_clear_kernel(u64* p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
-template <typename E, int V, int CL, int WAVES>
+template <typename E, int V, int CL, int WAVES, int TW, bool CUTS>
 __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* h0, void* __restrict__ y, float* hlast,
                                                                    float* __restrict__ states) {
-    constexpr int TL = 64 / CL, L = 32 / TL, NCH = CL * V, SPAN = WAVES * 32;
-    __shared__ float sA[WAVES][NCH], sH[WAVES][NCH], totA[NCH], totH[NCH], carry[NCH], partA[WAVES * 64 / NCH][NCH], partH[WAVES * 64 / NCH][NCH];
+    constexpr int TL = 64 / CL, L = TW / TL, NCH = CL * V, SPAN = WAVES * TW, ROWS = WAVES * TL, SEGS = WAVES * 64 / NCH;
+    static_assert(SPAN == SPAN_KEEP, "a block begins at a kept state");
+    __shared__ __attribute__((aligned(16))) float rowA[ROWS][NCH], rowH[ROWS][NCH];
+    __shared__ float partA[SEGS][NCH], partH[SEGS][NCH], prevA[SEGS][NCH], prevH[SEGS][NCH];
     int kb, tile;
-    span_place(W, kb, tile);
+    if (!span_place(W, kb, tile)) return;
     const int ct = tile % W.ctiles, seq = tile / W.ctiles, b = seq / A.P, p = seq % A.P;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, cl = lane % CL;
-    const int n = live_tokens(A, b), t0 = kb * SPAN + wave * 32 + (lane / CL) * L;
+    const int row = threadIdx.x / CL, cl = threadIdx.x % CL;
+    const int n = live_tokens(A, b), b0 = kb * SPAN, t0 = b0 + row * L;
     const int c = ct * NCH + cl * V;
-    const bool cok = c < A.C;
+    const bool cok = c < A.C, whole = b0 + SPAN <= n;         // whole: every token of the block exists
     const int cc = cok ? c : 0;
-    const unsigned char* rs = A.resets ? A.resets + (int64_t)b * A.T : nullptr;
 
-    RowVec<E, V> vq[L], vk[L];
-    float g[L][V];
+    RowVec<E, V> vq[L], vk[L], va[L];
     unsigned cuts = 0;
-    {
-        RowVec<E, V> va[L];
+    if (b0 < n) {
         const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
-        if (kb * SPAN < n) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) {                     // rows behind the last token are not read: the last one stands in for them
-                const int64_t at = in0 + (int64_t)min(t0 + i, n - 1) * A.st;
-                va[i].load(a, at); vk[i].load(kv, at); vq[i].load(q, at);
-            }
-            if (rs)
-#pragma unroll
-                for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && rs[min(t0 + i, n - 1)]) ? 1u << i : 0u;
-        } else {
-#pragma unroll
-            for (int i = 0; i < L; ++i) { va[i].clear(); vk[i].clear(); vq[i].clear(); }
+        for (int i = 0; i < L; ++i) {                         // rows behind the last token are not read: the last one stands in for them
+            const int64_t at = in0 + (int64_t)min(t0 + i, n - 1) * A.st;
+            va[i].load(a, at); vk[i].load(kv, at); vq[i].load(q, at);
         }
+        if (CUTS) {
+            const unsigned char* rs = A.resets + (int64_t)b * A.T;
+#pragma unroll
+            for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && rs[min(t0 + i, n - 1)]) ? 1u << i : 0u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < L; ++i) { va[i].clear(); vk[i].clear(); vq[i].clear(); }
+    }
+    if (!whole) {                                             // a token that does not exist lets the state pass: decay 1, nothing added
+#pragma unroll
+        for (int i = 0; i < L; ++i)
+            if (t0 + i >= n) { va[i].infinite(); vk[i].clear(); }
+    }
+    float g[L][V];
+    {
+        float pa[V], ph[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) { pa[k] = 1.f; ph[k] = 0.f; }
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            float fa[V];
-            va[i].get(fa);
+            float fk[V], fa[V];
+            vk[i].get(fk); va[i].get(fa);
 #pragma unroll
-            for (int k = 0; k < V; ++k) g[i][k] = t0 + i < n ? sigm<E>(fa[k]) : 1.f;
+            for (int k = 0; k < V; ++k) {
+                g[i][k] = sigm<E>(fa[k]);
+                const float r = fmaf(g[i][k], ph[k], fk[k]);
+                ph[k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
+                pa[k] *= g[i][k];
+            }
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k) { rowA[row][cl * V + k] = CUTS && cuts ? LOOP_CUT : pa[k]; rowH[row][cl * V + k] = ph[k]; }
     }
-    float pa[V], ph[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) { pa[k] = 1.f; ph[k] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-        float fk[V];
-        vk[i].get(fk);
-        const bool cut = cuts >> i & 1, on = t0 + i < n;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float x = on ? fk[k] : 0.f;
-            ph[k] = cut ? x : fmaf(g[i][k], ph[k], x);
-            pa[k] *= g[i][k];
-        }
-    }
-    if (cuts)
-#pragma unroll
-        for (int k = 0; k < V; ++k) pa[k] = LOOP_CUT;
-    lane_prefix<V, CL, false>(pa, ph, sA[wave], sH[wave]);
     __syncthreads();
-    wave_prefix<NCH, WAVES, false>(sA, sH, totA, totH);
-    __syncthreads();
-    const int chn = threadIdx.x % NCH;
-    const bool chok = ct * NCH + chn < A.C;
-    float first = 0.f;
-    if (kb == 0 && h0 && chok && threadIdx.x < NCH) first = h0[(int64_t)seq * A.C + ct * NCH + chn];
-    span_carry<NCH, WAVES * 64>(W, kb, tile, chok, first, totA, totH, carry, partA, partH);
+    const int chn = threadIdx.x % NCH, chc = ct * NCH + chn;
+    const bool chok = chc < A.C;
+    const float first = kb == 0 && h0 && chok && threadIdx.x >= (SEGS - 1) * NCH ? h0[(int64_t)seq * A.C + chc] : 0.f;
+    span_join<NCH, SEGS, ROWS, false, CUTS>(W, kb, tile, chok, first, rowA, rowH, partA, partH, prevA, prevH);
 
     float h[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int ch = cl * V + k;
-        float wa = sA[wave][ch], wh = sH[wave][ch];
-        join(wa, wh, pa[k], ph[k]);
-        h[k] = wa == LOOP_CUT ? wh : fmaf(wa, carry[ch], wh);
-    }
-    if (states && cok && t0 > 0 && t0 < n && t0 % SPAN_KEEP == 0) {
-        float* o = states + (((int64_t)b * A.nstate + t0 / SPAN_KEEP - 1) * A.P + p) * A.C + c;
+    for (int k = 0; k < V; ++k) h[k] = rowH[row][cl * V + k];
+    if (states && cok && row == 0 && kb > 0 && t0 < n) {
+        float* o = states + (((int64_t)b * A.nstate + kb - 1) * A.P + p) * A.C + c;
 #pragma unroll
         for (int k = 0; k < V; ++k) o[k] = h[k];
     }
@@ -433,163 +409,185 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
     for (int i = 0; i < L; ++i) {
         float fk[V], fq[V];
         vk[i].get(fk); vq[i].get(fq);
-        const bool cut = cuts >> i & 1, on = t0 + i < n;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const float x = on ? fk[k] : 0.f;
-            h[k] = cut ? x : fmaf(g[i][k], h[k], x);
-            fq[k] = on ? fq[k] * h[k] : 0.f;
+            const float r = fmaf(g[i][k], h[k], fk[k]);
+            h[k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
+            fq[k] *= h[k];
         }
+        if (!whole && t0 + i >= n)
+#pragma unroll
+            for (int k = 0; k < V; ++k) fq[k] = 0.f;
         if (cok && t0 + i < A.T) RowVec<E, V>::store(y, y0 + (t0 + i) * yt, fq);
     }
-    if (hlast && cok && kb == W.nblk - 1 && wave == WAVES - 1 && lane / CL == TL - 1) {
+    if (hlast && cok && kb == W.nblk - 1 && row == ROWS - 1) {
 #pragma unroll
         for (int k = 0; k < V; ++k) hlast[(int64_t)seq * A.C + c + k] = h[k];
     }
 }
 
-// The same from the last token to the first for D; the states in front of a block's tokens are formed again from the kept state
-template <typename E, int V, int CL, int WAVES>
+// The same from the last token to the first for D.  The states in front of a block's tokens are formed again from the kept state.  Held per
+// element: m = min(g, 1 - g) with the sign of a, from which g and g (1 - g) follow without a cancellation and without another exponential.
+template <typename E, int V, int CL, int WAVES, int TW, bool CUTS>
 __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* __restrict__ h0, const float* __restrict__ states,
                                                                    const void* __restrict__ dy, const float* __restrict__ dhlast, void* __restrict__ dq,
                                                                    void* __restrict__ dkv, void* __restrict__ da, float* __restrict__ dh0) {
-    constexpr int TL = 64 / CL, L = 32 / TL, NCH = CL * V, SPAN = WAVES * 32;
+    constexpr int TL = 64 / CL, L = TW / TL, NCH = CL * V, SPAN = WAVES * TW, ROWS = WAVES * TL, SEGS = WAVES * 64 / NCH, RPS = ROWS / SEGS;
     static_assert(SPAN == SPAN_KEEP, "a block begins at a kept state");
-    __shared__ float sA[WAVES][NCH], sH[WAVES][NCH], bA[WAVES][NCH], bH[WAVES][NCH], totA[NCH], totH[NCH], carry[NCH];
-    __shared__ float partA[WAVES * 64 / NCH][NCH], partH[WAVES * 64 / NCH][NCH];
+    __shared__ __attribute__((aligned(16))) float rowA[ROWS][NCH], rowH[ROWS][NCH], rowU[ROWS][NCH];
+    __shared__ float partA[SEGS][NCH], partH[SEGS][NCH], prevA[SEGS][NCH], prevH[SEGS][NCH];
     int back_kb, tile;
-    span_place(W, back_kb, tile);
+    if (!span_place(W, back_kb, tile)) return;
     const int kb = W.nblk - 1 - back_kb;
     const int ct = tile % W.ctiles, seq = tile / W.ctiles, b = seq / A.P, p = seq % A.P;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, cl = lane % CL;
-    const int n = live_tokens(A, b), t0 = kb * SPAN + wave * 32 + (lane / CL) * L;
+    const int row = threadIdx.x / CL, cl = threadIdx.x % CL;
+    const int n = live_tokens(A, b), b0 = kb * SPAN, t0 = b0 + row * L;
     const int c = ct * NCH + cl * V;
-    const bool cok = c < A.C;
+    const bool cok = c < A.C, whole = b0 + SPAN <= n;
     const int cc = cok ? c : 0;
-    const unsigned char* rs = A.resets ? A.resets + (int64_t)b * A.T : nullptr;
+    const int chn = threadIdx.x % NCH, seg = threadIdx.x / NCH, chc = ct * NCH + chn;
+    const bool chok = chc < A.C;
     const int64_t yt = (int64_t)A.P * A.C, y0 = ((int64_t)b * A.T * A.P + p) * A.C + cc;
 
-    RowVec<E, V> vq[L], vk[L], va[L], vy[L];
-    float hin[V];                                             // the block's kept state
+    RowVec<E, V> vq[L], vk[L], vy[L];
+    float m[L][V];
     unsigned cuts = 0;
+    float hin = 0.f;                                          // kept state in front of the block, channel chn
+    {
+        RowVec<E, V> va[L];
+        if (b0 < n) {
+            const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
 #pragma unroll
-    for (int k = 0; k < V; ++k) hin[k] = 0.f;
-    if (kb * SPAN < n) {
-        const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
+            for (int i = 0; i < L; ++i) {
+                const int t = min(t0 + i, n - 1);
+                const int64_t at = in0 + (int64_t)t * A.st;
+                va[i].load(a, at); vk[i].load(kv, at); vq[i].load(q, at); vy[i].load(dy, y0 + t * yt);
+            }
+            if (CUTS) {
+                const unsigned char* rs = A.resets + (int64_t)b * A.T;
+#pragma unroll
+                for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && rs[min(t0 + i, n - 1)]) ? 1u << i : 0u;
+            }
+            if (chok) {
+                if (kb > 0) hin = states[(((int64_t)b * A.nstate + kb - 1) * A.P + p) * A.C + chc];
+                else if (h0) hin = h0[(int64_t)seq * A.C + chc];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; ++i) { va[i].clear(); vk[i].clear(); vq[i].clear(); vy[i].clear(); }
+        }
+        if (!whole) {                                         // a token that does not exist: decay 1, nothing added in either direction
+#pragma unroll
+            for (int i = 0; i < L; ++i)
+                if (t0 + i >= n) { va[i].infinite(); vk[i].clear(); vq[i].clear(); vy[i].clear(); }
+        }
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int t = min(t0 + i, n - 1);
-            const int64_t at = in0 + (int64_t)t * A.st;
-            va[i].load(a, at); vk[i].load(kv, at); vq[i].load(q, at); vy[i].load(dy, y0 + t * yt);
+            float fa[V];
+            va[i].get(fa);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float e = Gate<E>::ex(-fabsf(fa[k]));
+                m[i][k] = copysignf(e * Gate<E>::recip(1.f + e), fa[k]);
+            }
         }
-        if (rs)
-#pragma unroll
-            for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && rs[min(t0 + i, n - 1)]) ? 1u << i : 0u;
-        const float* hp = kb > 0 ? states + (((int64_t)b * A.nstate + kb - 1) * A.P + p) * A.C + cc : (h0 ? h0 + (int64_t)seq * A.C + cc : nullptr);
-        if (hp)
-#pragma unroll
-            for (int k = 0; k < V; ++k) hin[k] = hp[k];
-    } else {
-#pragma unroll
-        for (int i = 0; i < L; ++i) { va[i].clear(); vk[i].clear(); vq[i].clear(); vy[i].clear(); }
     }
-    float g[L][V];
+    auto decay = [&](int i, int k) { const float v = m[i][k]; return signbit(v) ? -v : 1.f - v; };
+    {
+        float pa[V], ph[V], pu[V];
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-        float fa[V];
-        va[i].get(fa);
+        for (int k = 0; k < V; ++k) { pa[k] = 1.f; ph[k] = pu[k] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            float fk[V];
+            vk[i].get(fk);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float g = decay(i, k), r = fmaf(g, ph[k], fk[k]);
+                ph[k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
+                pa[k] *= g;
+            }
+        }
+#pragma unroll
+        for (int i = L - 1; i >= 0; --i) {
+            float fq[V], fy[V];
+            vq[i].get(fq); vy[i].get(fy);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float r = decay(i, k) * fmaf(fq[k], fy[k], pu[k]);
+                pu[k] = CUTS && (cuts >> i & 1) ? 0.f : r;
+            }
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            float slope;
-            sigm_slope<E>(fa[k], g[i][k], slope);
-            if (t0 + i >= n) g[i][k] = 1.f;
+            rowA[row][cl * V + k] = CUTS && cuts ? LOOP_CUT : pa[k];
+            rowH[row][cl * V + k] = ph[k]; rowU[row][cl * V + k] = pu[k];
         }
     }
-    float pa[V], ph[V], ba[V], bh[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) { pa[k] = ba[k] = 1.f; ph[k] = bh[k] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-        float fk[V];
-        vk[i].get(fk);
-        const bool cut = cuts >> i & 1, on = t0 + i < n;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float x = on ? fk[k] : 0.f;
-            ph[k] = cut ? x : fmaf(g[i][k], ph[k], x);
-            pa[k] *= g[i][k];
-        }
-    }
-#pragma unroll
-    for (int i = L - 1; i >= 0; --i) {
-        float fq[V], fy[V];
-        vq[i].get(fq); vy[i].get(fy);
-        const bool cut = cuts >> i & 1, on = t0 + i < n;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float d = on ? fmaf(fq[k], fy[k], bh[k]) : bh[k];
-            bh[k] = cut ? 0.f : g[i][k] * d;
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) { if (cuts) pa[k] = LOOP_CUT; ba[k] = pa[k]; }
-    lane_prefix<V, CL, false>(pa, ph, sA[wave], sH[wave]);
-    lane_prefix<V, CL, true>(ba, bh, bA[wave], bH[wave]);
     __syncthreads();
-    wave_prefix<NCH, WAVES, false>(sA, sH, totA, totH);       // the forward totals are not needed
-    wave_prefix<NCH, WAVES, true>(bA, bH, totA, totH);
-    __syncthreads();
-    const int chn = threadIdx.x % NCH;
-    const bool chok = ct * NCH + chn < A.C;
-    float first = 0.f;
-    if (back_kb == 0 && dhlast && chok && threadIdx.x < NCH) first = dhlast[(int64_t)seq * A.C + ct * NCH + chn];
-    span_carry<NCH, WAVES * 64>(W, back_kb, tile, chok, first, totA, totH, carry, partA, partH);
+    {   // states in front of the lane rows: from the kept state
+        float ra[RPS], rh[RPS], pA = 1.f, pH = 0.f;
+#pragma unroll
+        for (int j = 0; j < RPS; ++j) {
+            ra[j] = rowA[seg * RPS + j][chn]; rh[j] = rowH[seg * RPS + j][chn];
+            join<CUTS>(pA, pH, ra[j], rh[j]);
+        }
+        prevA[seg][chn] = pA; prevH[seg][chn] = pH;
+        __syncthreads();
+        float h = hin;
+        for (int s = 0; s < seg; ++s) h = pass<CUTS>(prevA[s][chn], prevH[s][chn], h);
+#pragma unroll
+        for (int j = 0; j < RPS; ++j) {
+            rowH[seg * RPS + j][chn] = h;
+            h = pass<CUTS>(ra[j], rh[j], h);
+        }
+    }
+    const float first = back_kb == 0 && dhlast && chok && seg == SEGS - 1 ? dhlast[(int64_t)seq * A.C + chc] : 0.f;
+    // (the barrier inside, between its use of partA and of prevA, keeps prevA apart from its use above)
+    span_join<NCH, SEGS, ROWS, true, CUTS>(W, back_kb, tile, chok, first, rowA, rowU, partA, partH, prevA, prevH);
 
     float h[L + 1][V], back[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int ch = cl * V + k;
-        float wa = sA[wave][ch], wh = sH[wave][ch];
-        join(wa, wh, pa[k], ph[k]);
-        h[0][k] = wa == LOOP_CUT ? wh : fmaf(wa, hin[k], wh);
-        wa = bA[wave][ch], wh = bH[wave][ch];
-        join(wa, wh, ba[k], bh[k]);
-        back[k] = wa == LOOP_CUT ? wh : fmaf(wa, carry[ch], wh);
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-        float fk[V];
-        vk[i].get(fk);
-        const bool cut = cuts >> i & 1, on = t0 + i < n;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float x = on ? fk[k] : 0.f;
-            h[i + 1][k] = cut ? x : fmaf(g[i][k], h[i][k], x);
-        }
-    }
+    for (int k = 0; k < V; ++k) { h[0][k] = rowH[row][cl * V + k]; back[k] = rowU[row][cl * V + k]; }
     const int64_t g0 = (int64_t)b * A.gb + (int64_t)p * A.gp + c;
 #pragma unroll
-    for (int i = L - 1; i >= 0; --i) {
-        float fq[V], fy[V], fa[V], ok[V], oa[V];
-        vq[i].get(fq); vy[i].get(fy); va[i].get(fa);
-        const bool cut = cuts >> i & 1, on = t0 + i < n;
+    for (int i = 0; i < L; ++i) {
+        float fk[V], fy[V];
+        vk[i].get(fk); vy[i].get(fy);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            float gg, slope;
-            sigm_slope<E>(fa[k], gg, slope);
-            const float d = fmaf(fq[k], fy[k], back[k]);
-            fq[k] = on ? h[i + 1][k] * fy[k] : 0.f;
-            ok[k] = on ? d : 0.f;
-            oa[k] = on && !cut ? d * h[i][k] * slope : 0.f;
-            back[k] = on ? (cut ? 0.f : g[i][k] * d) : back[k];
+            const float r = fmaf(decay(i, k), h[i][k], fk[k]);
+            h[i + 1][k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
+            fy[k] *= h[i + 1][k];
         }
+        if (!whole && t0 + i >= n)
+#pragma unroll
+            for (int k = 0; k < V; ++k) fy[k] = 0.f;
+        if (cok && t0 + i < A.T) RowVec<E, V>::store(dq, g0 + (t0 + i) * A.gt, fy);
+    }
+#pragma unroll
+    for (int i = L - 1; i >= 0; --i) {
+        float fq[V], fy[V], oa[V];
+        vq[i].get(fq); vy[i].get(fy);
+        const bool cut = CUTS && (cuts >> i & 1);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float s = fabsf(m[i][k]), g = decay(i, k);
+            fq[k] = fmaf(fq[k], fy[k], back[k]);
+            const float r = fq[k] * h[i][k] * (s * (1.f - s));
+            oa[k] = cut ? 0.f : r;
+            back[k] = cut ? 0.f : g * fq[k];
+        }
+        if (!whole && t0 + i >= n)
+#pragma unroll
+            for (int k = 0; k < V; ++k) { back[k] = fq[k]; fq[k] = 0.f; oa[k] = 0.f; }
         if (cok && t0 + i < A.T) {
             const int64_t at = g0 + (t0 + i) * A.gt;
-            RowVec<E, V>::store(dq, at, fq); RowVec<E, V>::store(dkv, at, ok); RowVec<E, V>::store(da, at, oa);
+            RowVec<E, V>::store(dkv, at, fq); RowVec<E, V>::store(da, at, oa);
         }
     }
-    if (dh0 && cok && kb == 0 && wave == 0 && lane / CL == 0) {
+    if (dh0 && cok && kb == 0 && row == 0) {
 #pragma unroll
         for (int k = 0; k < V; ++k) dh0[(int64_t)seq * A.C + c + k] = back[k];
     }
@@ -613,12 +611,16 @@ static int loop_check(const mv2_gateloop_desc* d) {
     return MV2_OK;
 }
 
-// Which form runs: one thread per chunk where the tokens are few or the channels many, spans otherwise.  A function of the sizes alone (the
-// backward pass finds the states that the forward pass kept).
+// Which form runs: one thread per chunk where the tokens are few for that many channels, spans otherwise.  A function of the sizes alone (the
+// backward pass finds the states that the forward pass kept).  A walk takes 0.36 us a token (backward 0.65) until the memory is busy,
+// a span of up to 256 tokens some 5 us (8) and as much again for every 4096 (2048) chunks.  Measured, bf16, us forward / backward, walk : span:
+//     512 chunks, 8 tokens 5.7 / 7.5 : 5.2 / 7.8     16 tokens 8.9 / 12.6 : 5.2 / 7.8
+//   16384 chunks, 33 tokens 18 / 33 : 22 / 56        64 tokens 31 / 61 : 24 / 59
+//   65536 chunks, 128 tokens 107 / 236 : 125 / 303   256 tokens 212 / 473 : 228 / 484
 static bool loop_walks(const mv2_gateloop_desc* d) {
     const int kvec = d->dtype == MV2_BF16 ? 8 : 4;
     const double chunks = (double)d->B * d->P * ((d->C + kvec - 1) / kvec);
-    return d->T <= 16 || chunks >= 131072;
+    return d->T <= 8 + chunks / 512;
 }
 
 extern "C" int64_t mv2_gateloop_states(const mv2_gateloop_desc* d) {
@@ -627,25 +629,28 @@ extern "C" int64_t mv2_gateloop_states(const mv2_gateloop_desc* d) {
     return d->T > 0 ? (d->T - 1) / (loop_walks(d) ? LOOP_STEPS : SPAN_KEEP) : 0;
 }
 
-struct SpanShape { int64_t nblk, ctiles, ntile, words; };
-static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, int span) {
+struct SpanShape { int64_t nblk, ctiles, ntile, nq, words; };
+static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, bool backward) {
     SpanShape s;
-    s.nblk = (d->T + span - 1) / span;
+    s.nblk = (d->T + SPAN_KEEP - 1) / SPAN_KEEP;
     s.ctiles = (d->C + nch - 1) / nch;
     s.ntile = s.ctiles * d->B * d->P;
-    s.words = s.nblk > 1 ? 2 + (s.nblk + (s.nblk + LOOP_GROUP - 1) / LOOP_GROUP) * s.ntile * nch : 0;
+    // queues per XCD, forward: 4 x 8192 x 768 bf16 48 us against 50 from one queue, rows that are not whole lines 6 x 4095 x 1000 52 against 59;
+    // backward only for those (104 us against 109; whole lines 91 against 87).  Few tiles would leave XCDs idle.
+    const int64_t es = d->dtype == MV2_BF16 ? 2 : 4;
+    s.nq = s.ntile >= 32 && (!backward || d->in_t * es % 128 != 0) ? 8 : 1;
+    s.words = s.nblk > 1 ? 64 + (s.nblk + (s.nblk + LOOP_GROUP - 1) / LOOP_GROUP) * s.ntile * nch : 0;
     return s;
 }
-#define SPAN_FWD_WAVES 8
-#define SPAN_BWD_WAVES 4
+#define SPAN_WAVES 8               // waves of a workgroup and tokens of a wave
+#define SPAN_TW 32
 // channels of a workgroup: 128-byte pieces of rows (64 bf16 or 32 fp32), 64 single elements where rows are not whole 16-byte chunks
 static int span_channels(const mv2_gateloop_desc* d, bool wide) { return wide && d->dtype == MV2_F32 ? 32 : 64; }
 
 extern "C" size_t mv2_gateloop_workspace_bytes(const mv2_gateloop_desc* d, int backward) {
     if (loop_check(d) != MV2_OK || loop_walks(d)) return 0;
-    const int span = 32 * (backward ? SPAN_BWD_WAVES : SPAN_FWD_WAVES);
     int64_t words = 0;
-    for (int wide = 0; wide < 2; ++wide) words = std::max(words, span_shape(d, span_channels(d, wide), span).words);      // whichever the addresses allow
+    for (int wide = 0; wide < 2; ++wide) words = std::max(words, span_shape(d, span_channels(d, wide), backward != 0).words);      // whichever the addresses allow
     return (size_t)words * sizeof(u64);
 }
 
@@ -659,17 +664,18 @@ static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, co
 }
 
 // the pairs' words, cleared by a kernel (a captured memset would not do: the launch may be recorded into a graph)
-static int span_work(const mv2_gateloop_desc* d, bool wide, int waves, void* workspace, size_t workspace_bytes, hipStream_t st, SpanWork& W, unsigned& grid) {
+static int span_work(const mv2_gateloop_desc* d, bool wide, bool backward, void* workspace, size_t workspace_bytes, hipStream_t st, SpanWork& W, unsigned& grid) {
     const int nch = span_channels(d, wide);
-    const SpanShape s = span_shape(d, nch, waves * 32);
-    if ((double)s.nblk * s.ntile > 2147483647.0) return MV2_ETOOLARGE;
+    const SpanShape s = span_shape(d, nch, backward);
+    if ((double)s.nblk * (s.ntile + 8) > 2147483647.0) return MV2_ETOOLARGE;
     W.nblk = (int)s.nblk; W.ntile = (int)s.ntile; W.ctiles = (int)s.ctiles;
-    grid = (unsigned)(s.nblk * s.ntile);
+    W.nq = (int)s.nq;
+    grid = (unsigned)(s.nblk > 1 ? s.nblk * s.nq * ((s.ntile + s.nq - 1) / s.nq) : s.ntile);
     W.ticket = nullptr; W.pairs = W.states = nullptr;
     if (s.words == 0) return MV2_OK;
     if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < s.words * sizeof(u64)) return MV2_EWORKSPACE;
     W.ticket = (unsigned*)workspace;
-    W.pairs = (u64*)workspace + 2;
+    W.pairs = (u64*)workspace + 64;
     W.states = W.pairs + s.nblk * s.ntile * nch;
     hipLaunchKernelGGL(span_clear_kernel, dim3((unsigned)std::min<int64_t>((s.words + 255) / 256, 2048)), dim3(256), 0, st, (u64*)workspace, s.words);
     MV2_LAUNCH_CHECK();
@@ -695,11 +701,13 @@ extern "C" int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, c
     } else {
         SpanWork W;
         unsigned grid;
-        rc = span_work(d, wide, SPAN_FWD_WAVES, workspace, workspace_bytes, st, W, grid);
+        rc = span_work(d, wide, false, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, CL) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, CL, SPAN_FWD_WAVES>), dim3(grid), dim3(64 * SPAN_FWD_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
-        if (d->dtype == MV2_BF16) { if (wide) GO(BF16, 8, 8); else GO(BF16, 1, 64); }
-        else { if (wide) GO(F32, 4, 8); else GO(F32, 1, 64); }
+#define GO(E, V, CL, CUTS) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
+#define GO2(E, V, CL) do { if (resets) GO(E, V, CL, true); else GO(E, V, CL, false); } while (0)
+        if (d->dtype == MV2_BF16) { if (wide) GO2(BF16, 8, 8); else GO2(BF16, 1, 64); }
+        else { if (wide) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
+#undef GO2
 #undef GO
     }
     MV2_LAUNCH_CHECK();
@@ -719,21 +727,23 @@ extern "C" int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, 
                       d->grad_t % kvec == 0 && d->grad_p % kvec == 0 && rows_aligned16({q, kv, a, dy, dq, dkv, da});
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
-        const int64_t n = (int64_t)d->B * d->P * (d->C / (wide ? kvec : 1));
+        const int64_t n = (int64_t)d->B * d->P * (d->C / (wide ? kvec / 2 : 1));
         const dim3 grid((unsigned)((n + 255) / 256));
 #define GO(E, V) hipLaunchKernelGGL((loop_walk_bwd_kernel<E, V>), grid, dim3(256), 0, st, A, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-        if (d->dtype == MV2_BF16) { if (wide) GO(BF16, 8); else GO(BF16, 1); }
-        else { if (wide) GO(F32, 4); else GO(F32, 1); }
+        if (d->dtype == MV2_BF16) { if (wide) GO(BF16, 4); else GO(BF16, 1); }
+        else { if (wide) GO(F32, 2); else GO(F32, 1); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
-        rc = span_work(d, wide, SPAN_BWD_WAVES, workspace, workspace_bytes, st, W, grid);
+        rc = span_work(d, wide, true, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, CL)                                                                                                                                    \
-    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, CL, SPAN_BWD_WAVES>), dim3(grid), dim3(64 * SPAN_BWD_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-        if (d->dtype == MV2_BF16) { if (wide) GO(BF16, 8, 8); else GO(BF16, 1, 64); }
-        else { if (wide) GO(F32, 4, 8); else GO(F32, 1, 64); }
+#define GO(E, V, CL, CUTS)                                                                                                                                    \
+    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
+#define GO2(E, V, CL) do { if (resets) GO(E, V, CL, true); else GO(E, V, CL, false); } while (0)
+        if (d->dtype == MV2_BF16) { if (wide) GO2(BF16, 8, 8); else GO2(BF16, 1, 64); }
+        else { if (wide) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
+#undef GO2
 #undef GO
     }
     MV2_LAUNCH_CHECK();
