@@ -305,6 +305,49 @@ class HipOps:
         return _mk(self.lib.mv2_gateloop_backward, args, 'mv2_gateloop_backward',
                    (d, q, kv, a, h0, lengths, resets, states, dy, dh_last, dq, dkv, da, dh0, ws), (dq, dkv, da, dh0))
 
+    # the same at once on the current stream (functional.py), from a call's plan: (qkva,) or (q, kv, a), workspaces allocated here
+    def _now(self, fn, what, *args):
+        """on the current stream of this launcher's device, which need not be the current device"""
+        idx = self.device.index
+        stream = torch._C._cuda_getCurrentRawStream(idx)
+        if torch._C._cuda_getDevice() == idx:
+            rc = fn(*args, stream)
+        else:
+            with torch.cuda.device(idx):
+                rc = fn(*args, stream)
+        if rc != 0:
+            raise Mv2Error(f'{what} failed with code {rc}')
+
+    @staticmethod
+    def _loop_ptrs(plan, parts):
+        if plan.fused:
+            p = parts[0].data_ptr()
+            part = plan.C * parts[0].element_size()
+            return p, p + part, p + 2 * part
+        return tuple(t.data_ptr() for t in parts)
+
+    def gateloop_forward_now(self, plan, qkva, h0, lengths, resets, y, h_last, states):
+        n = plan.ws_forward
+        ws = self.empty((n,), torch.uint8) if n else None
+        self._now(self.lib.mv2_gateloop_forward, 'mv2_gateloop_forward', plan.desc, *self._loop_ptrs(plan, qkva), _ptr(h0), _ptr(lengths), _ptr(resets),
+                  y.data_ptr(), _ptr(h_last), _ptr(states), _ptr(ws), n)
+
+    def gateloop_backward_now(self, plan, qkva, h0, lengths, resets, states, dy, dh_last, grads, dh0):
+        n = plan.ws_backward
+        ws = self.empty((n,), torch.uint8) if n else None
+        self._now(self.lib.mv2_gateloop_backward, 'mv2_gateloop_backward', plan.desc, *self._loop_ptrs(plan, qkva), _ptr(h0), _ptr(lengths), _ptr(resets),
+                  _ptr(states), dy.data_ptr(), _ptr(dh_last), *self._loop_ptrs(plan, grads), _ptr(dh0), _ptr(ws), n)
+
+    def block_norm_forward_now(self, plan, x, branch, gate, post, scale, pre, out, normed, rstd):
+        self._now(self.lib.mv2_block_norm_forward, 'mv2_block_norm_forward', plan.desc, x.data_ptr(), _ptr(branch), _ptr(gate), _ptr(post), _ptr(scale),
+                  _ptr(pre), _ptr(out), _ptr(normed), _ptr(rstd))
+
+    def block_norm_backward_now(self, plan, saved, dout, dn, rows, cols):
+        n = plan.ws_backward if any(c is not None for c in cols) else 0
+        ws = self.empty((n,), torch.uint8) if n else None
+        self._now(self.lib.mv2_block_norm_backward, 'mv2_block_norm_backward', plan.desc, *map(_ptr, saved), _ptr(dout), _ptr(dn), *map(_ptr, rows),
+                  *map(_ptr, cols), _ptr(ws), n)
+
     def block_norm_workspace_bytes(self, d: BlockNormDesc) -> int:
         return int(self.lib.mv2_block_norm_workspace_bytes(C.byref(d)))
 

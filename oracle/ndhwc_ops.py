@@ -580,6 +580,23 @@ class CpuOps:
         step.what = 'gateloop_backward'
         return step
 
+    # at once, from a call's plan (functional.py)
+    @staticmethod
+    def _loop_parts(plan, parts):
+        return parts[0].split(plan.C, -1) if plan.fused else parts
+
+    def gateloop_forward_now(self, plan, qkva, h0, lengths, resets, y, h_last, states):
+        self.gateloop_forward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, y, h_last, states, None)(0)
+
+    def gateloop_backward_now(self, plan, qkva, h0, lengths, resets, states, dy, dh_last, grads, dh0):
+        self.gateloop_backward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, states, dy, dh_last, *self._loop_parts(plan, grads), dh0, None)(0)
+
+    def block_norm_forward_now(self, plan, *args):
+        self.block_norm_forward(plan.desc, *args)(0)
+
+    def block_norm_backward_now(self, plan, saved, dout, dn, rows, cols):
+        self.block_norm_backward(plan.desc, *saved, dout, dn, *rows, *cols, None)(0)
+
     def block_norm_workspace_bytes(self, d):
         return 4
 

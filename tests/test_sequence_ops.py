@@ -17,7 +17,7 @@ EINVAL, ETOOLARGE, EWORKSPACE = -1, -2, -3
 @pytest.fixture
 def emulated(monkeypatch):
     monkeypatch.setattr(F, '_backends', {torch.device('cpu'): CpuOps()})
-    monkeypatch.setattr(F, '_geometries', {})
+    monkeypatch.setattr(F, '_plans', {})
 
 
 def rnd(*shape, seed=0, dtype=torch.float32):
@@ -201,7 +201,8 @@ def test_refusals(emulated):
             call()
 
 
-def test_no_cpu_path():
+def test_no_cpu_path(monkeypatch):
+    monkeypatch.setattr(F, '_plans', {})
     with pytest.raises(Mv2Error):
         F.gate_loop(rnd(1, 2, 6))
     with pytest.raises(Mv2Error):

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from magvit2_pytorch_amd import functional as F
+from magvit2_pytorch_amd.ops_hip import GateLoopDesc, HipOps
 from tests._sequence_ref import assert_within, block_norm_ref, gate_loop_ref
 
 pytestmark = pytest.mark.gpu
@@ -225,12 +226,13 @@ def test_last_state_written_over_the_first(dtype):
     """the C ABI lets h_last be h0 itself, for any length"""
     for B, T, C in ((2, 1, 64), (2, 600, 40), (1, 5000, 64), (1, 5000, 9)):
         z = loop_inputs(B, T, 1, C, dtype).cuda()
-        ops = F._ops(z.device)
-        s0 = rnd(B, C, seed=2).cuda()
-        y, h = F.gate_loop(z, state=s0[:, None], return_state=True)
-        geo = F._loop_geometry(ops, {torch.bfloat16: 0, torch.float32: 1}[dtype], (B, T, 1, C), (z.stride(0) if B > 1 else 0, z.stride(1) if T > 1 else 0, 0), True)
+        y, h = F.gate_loop(z, state=(s0 := rnd(B, C, seed=2).cuda())[:, None], return_state=True)
+        ops = HipOps(z.device)
+        d = GateLoopDesc(dtype=0 if dtype == torch.bfloat16 else 1, B=B, T=T, P=1, C=C, in_b=z.stride(0), in_t=z.stride(1), in_p=z.stride(2),
+                         grad_b=0, grad_t=0, grad_p=0)
+        ws = torch.empty(max(1, ops.gateloop_sizes(d)[1]), dtype=torch.uint8, device='cuda')
         s, y2 = s0.clone(), torch.empty_like(y)
-        ops.gateloop_forward(geo.desc, *z.split(C, -1), s, None, None, y2, s, None, F._bytes(ops, geo.ws_forward))(ops.current_stream())
+        ops.gateloop_forward(d, *z.split(C, -1), s, None, None, y2, s, None, ws)(ops.current_stream())
         assert torch.equal(s, h[:, 0]) and torch.equal(y2, y)
 
 
