@@ -5,7 +5,8 @@
 //     dbranch = r1 (d' - b (b . d')),  d' = sqrt(C) w1 D s act(gate),  b = branch r1          (likewise),
 //     dw1 = sqrt(C) sum_rows D s act(gate) b,   dw2 = sqrt(C) sum_rows dn o.
 // A group of G threads (a power of two) owns a row and keeps it in registers: every tensor is read once and written once.  out is not saved:
-// the backward pass forms it again from x, branch and gate, unrounded, as the forward pass had it.
+// the backward pass forms it again from x, branch and gate, unrounded, as the forward pass had it.  Memory-bound: a workgroup walks many
+// rows with the parameters in registers, R rows at a time so that their loads and their sums' latencies overlap.
 #include <algorithm>
 #include <initializer_list>
 #include "rowvec.h"
@@ -17,271 +18,373 @@ struct NormArgs {
     float root;                    // sqrt(C)
 };
 
-// sum over the G threads of a row's group; every thread of the workgroup takes part (groups of more than a wave meet in LDS)
-template <int BLOCK> __device__ __forceinline__ float group_sum(float v, int G, float* red) {
-    const int w = G < 64 ? G : 64;
-    for (int o = w >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    if (G <= 64) return v;
-    __syncthreads();                                   // the previous sum has been read
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    const int nw = G / 64, first = (threadIdx.x >> 6) / nw * nw;
-    float s = 0.f;
-    for (int i = 0; i < nw; ++i) s += red[first + i];
-    return s;
-}
+// Sums over the G threads of a row's group of N values at a time, in every thread.  Groups of more than a wave meet in LDS: `red` has two buffers
+// that calls use in turn, so one barrier a call is enough (a buffer is written again behind the barrier of the call in between).
+template <int BLOCK, int N> struct GroupSum {
+    float (*red)[N][BLOCK / 64];
+    int turn;
+    __device__ __forceinline__ void operator()(float (&v)[N], int G) {
+        lanes_sum(v, G);
+        if (G <= 64) return;
+        const int wave = threadIdx.x >> 6, nw = G / 64, first = wave / nw * nw;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) red[turn][i][wave] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = 0.f;
+            for (int j = 0; j < nw; ++j) s += red[turn][i][first + j];
+            v[i] = s;
+        }
+        turn ^= 1;
+    }
+};
 
-__device__ __forceinline__ float sigmoid_f(float g) { return 1.f / (1.f + expf(-g)); }
-__device__ __forceinline__ float gate_act(int act, float g) {
+// the gate's activation and its derivative
+template <typename E> __device__ __forceinline__ float gate_act(int act, float g) {
     if (act == MV2_ACT_NONE) return g;
-    const float s = sigmoid_f(g);
+    const float s = sigm<E>(g);
     return act == MV2_ACT_SILU ? g * s : s;
 }
-// act and its derivative; s (1 - s) as e / (1 + e)^2 with e = exp(-|g|): no cancellation
-__device__ __forceinline__ void gate_act_slope(int act, float g, float& v, float& d) {
+// exp(-|g|) down to the smallest numbers: the hardware's exp2 flushes results below 2^-126, but silu's slope multiplies them by |g|
+template <typename E> __device__ __forceinline__ float exp_tail(float g);
+template <> __device__ __forceinline__ float exp_tail<BF16>(float g) {
+    const float t = -fabsf(g) * 1.44269504088896340736f;
+    const bool small = t < -126.f;
+    return ldexpf(__builtin_amdgcn_exp2f(small ? t + 64.f : t), small ? -64 : 0);
+}
+template <> __device__ __forceinline__ float exp_tail<F32>(float g) { return expf(-fabsf(g)); }
+template <typename E> __device__ __forceinline__ void gate_act_slope(int act, float g, float& v, float& d) {
     if (act == MV2_ACT_NONE) { v = g; d = 1.f; return; }
-    const float e = expf(-fabsf(g)), r = 1.f / (1.f + e), er = e * r;
+    const float e = exp_tail<E>(g), r = Gate<E>::recip(1.f + e), er = e * r;
     const float s = g < 0.f ? er : r, ds = er * r;
     if (act == MV2_ACT_SIGMOID) { v = s; d = ds; }
     else { v = g * s; d = fmaf(g, ds, s); }
 }
+// 1 / max(|v|, 1e-12) from the sum of squares
+__device__ __forceinline__ float inv_norm(float ss) { return 1.f / fmaxf(sqrtf(ss), 1e-12f); }
 
-template <typename E, int V, int NC, int BLOCK>
+// a thread's parameters: f times w, or d where there is none; kept in registers for up to 16 elements, read again (from the caches) beyond
+// (7000 x 4096 bf16, 16 a thread: 60 us forward kept, 136 read again)
+template <int NC, int V> struct Params {
+    static constexpr bool KEPT = NC * V <= 16;
+    float r[KEPT ? NC : 1][KEPT ? V : 1];
+    const float* w;
+    float f, d;
+    int l, G, nch;
+    __device__ __forceinline__ Params(const float* w_, float f_, float d_, int l_, int G_, int nch_) : w(w_), f(f_), d(d_), l(l_), G(G_), nch(nch_) {
+        if (KEPT)
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+#pragma unroll
+                for (int k = 0; k < V; ++k) r[KEPT ? j : 0][KEPT ? k : 0] = w && l + j * G < nch ? f * w[(l + j * G) * V + k] : d;
+    }
+    __device__ __forceinline__ void get(int j, float* o) const {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = KEPT ? r[KEPT ? j : 0][KEPT ? k : 0] : (w ? f * w[(l + j * G) * V + k] : d);
+    }
+};
+
+template <typename E, int V, int NC, int R, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G, const void* x, const void* __restrict__ branch, const void* __restrict__ gate,
                                                                const float* __restrict__ w1, const float* __restrict__ sc, const float* __restrict__ w2,
                                                                void* out, void* __restrict__ normed, float* __restrict__ rstd) {
-    __shared__ float red[BLOCK / 64];
+    __shared__ float red[2][R][BLOCK / 64];
+    GroupSum<BLOCK, R> sum{red, 0};
     const int l = threadIdx.x & (G - 1), per = BLOCK / G;
     const int nch = A.C / V;
-    const int64_t groups = (A.rows + per - 1) / per;
-    for (int64_t blk = blockIdx.x; blk < groups; blk += gridDim.x) {
-        const int64_t row = blk * per + threadIdx.x / G;
-        const bool on = row < A.rows;
-        RowVec<E, V> vx[NC], vb[NC], vg[NC];
+    const Params<NC, V> p1(w1, A.root, 1.f, l, G, nch), ps(sc, 1.f, 1.f, l, G, nch), p2(w2, A.root, 1.f, l, G, nch);
+    const int64_t step = (int64_t)per * R;
+    for (int64_t base = blockIdx.x * step; base < A.rows; base += gridDim.x * step) {
+        int64_t row[R];
+        bool on[R];
+        RowVec<E, V> vx[R][NC], vb[R][NC], vg[R][NC];
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const int ch = l + j * G;
-            if (on && ch < nch) {
-                vx[j].load(x, row * A.xs + (int64_t)ch * V);
-                if (branch) vb[j].load(branch, row * A.bs + (int64_t)ch * V);
-                if (gate) vg[j].load(gate, row * A.gs + (int64_t)ch * V);
+        for (int i = 0; i < R; ++i) {
+            row[i] = base + i * per + threadIdx.x / G;
+            on[i] = row[i] < A.rows;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                const int ch = l + j * G;
+                if (on[i] && ch < nch) {
+                    vx[i][j].load(x, row[i] * A.xs + ch * V);
+                    if (branch) vb[i][j].load(branch, row[i] * A.bs + ch * V);
+                    if (gate) vg[i][j].load(gate, row[i] * A.gs + ch * V);
+                } else { vx[i][j].clear(); vb[i][j].clear(); vg[i][j].clear(); }
             }
         }
-        float r1 = 1.f;
+        float r1[R], r2[R];
         if (branch && (w1 || rstd)) {
-            float ss = 0.f;
 #pragma unroll
-            for (int j = 0; j < NC; ++j)
-                if (on && l + j * G < nch) {
-                    float f[V]; vb[j].get(f);
+            for (int i = 0; i < R; ++i) {
+                r1[i] = 0.f;
 #pragma unroll
-                    for (int k = 0; k < V; ++k) ss = fmaf(f[k], f[k], ss);
+                for (int j = 0; j < NC; ++j) {
+                    float f[V]; vb[i][j].get(f);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) r1[i] = fmaf(f[k], f[k], r1[i]);
                 }
-            r1 = 1.f / fmaxf(sqrtf(group_sum<BLOCK>(ss, G, red)), 1e-12f);
-            if (rstd && on && l == 0) rstd[row] = r1;
+            }
+            sum(r1, G);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                r1[i] = inv_norm(r1[i]);
+                if (rstd && on[i] && l == 0) rstd[row[i]] = r1[i];
+            }
         }
-        float o[NC][V], ss = 0.f;
+        float o[R][NC][V];
+#pragma unroll
+        for (int i = 0; i < R; ++i) r2[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const int ch = l + j * G;
-            if (on && ch < nch) {
-                vx[j].get(o[j]);
+            float f1[V], fs[V];
+            p1.get(j, f1); ps.get(j, fs);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int ch = l + j * G;
+                vx[i][j].get(o[i][j]);
                 if (branch) {
                     float fb[V], fg[V];
-                    vb[j].get(fb);
-                    if (gate) vg[j].get(fg);
+                    vb[i][j].get(fb); vg[i][j].get(fg);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const int c = ch * V + k;
                         float u = fb[k];
-                        if (w1) u *= r1 * (A.root * w1[c]);
-                        if (gate) u *= gate_act(A.act, fg[k]);
-                        o[j][k] = sc ? fmaf(sc[c], u, o[j][k]) : o[j][k] + u;
+                        if (w1) u *= r1[i] * f1[k];
+                        if (gate) u *= gate_act<E>(A.act, fg[k]);
+                        o[i][j][k] = fmaf(fs[k], u, o[i][j][k]);
                     }
-                    RowVec<E, V>::store(out, row * A.C + (int64_t)ch * V, o[j]);
+                    if (on[i] && ch < nch) RowVec<E, V>::store(out, row[i] * A.C + ch * V, o[i][j]);
                 }
+                if (on[i] && ch < nch)
 #pragma unroll
-                for (int k = 0; k < V; ++k) ss = fmaf(o[j][k], o[j][k], ss);
+                    for (int k = 0; k < V; ++k) r2[i] = fmaf(o[i][j][k], o[i][j][k], r2[i]);
             }
         }
         if (!w2) continue;
-        const float r2 = 1.f / fmaxf(sqrtf(group_sum<BLOCK>(ss, G, red)), 1e-12f);
-        if (rstd && on && l == 0) rstd[A.rows + row] = r2;
+        sum(r2, G);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            r2[i] = inv_norm(r2[i]);
+            if (rstd && on[i] && l == 0) rstd[A.rows + row[i]] = r2[i];
+        }
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const int ch = l + j * G;
-            if (on && ch < nch) {
+            float f2[V];
+            p2.get(j, f2);
 #pragma unroll
-                for (int k = 0; k < V; ++k) o[j][k] *= r2 * (A.root * w2[ch * V + k]);
-                RowVec<E, V>::store(normed, row * A.C + (int64_t)ch * V, o[j]);
+            for (int i = 0; i < R; ++i) {
+                const int ch = l + j * G;
+#pragma unroll
+                for (int k = 0; k < V; ++k) o[i][j][k] *= r2[i] * f2[k];
+                if (on[i] && ch < nch) RowVec<E, V>::store(normed, row[i] * A.C + ch * V, o[i][j]);
             }
         }
     }
 }
 
 // parts: [gridDim.x][3][C] column sums of a workgroup's rows (dw1, ds, dw2), summed in workgroup order by block_norm_cols_kernel
-template <typename E, int V, int NC, int BLOCK>
+template <typename E, int V, int NC, int R, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G, const void* __restrict__ x, const void* __restrict__ branch,
                                                                const void* __restrict__ gate, const float* __restrict__ w1, const float* __restrict__ sc,
                                                                const float* __restrict__ w2, const float* __restrict__ rstd, const void* __restrict__ dout,
                                                                const void* __restrict__ dn, void* __restrict__ dx, void* __restrict__ dbranch,
                                                                void* __restrict__ dgate, float* __restrict__ parts) {
-    __shared__ float red[BLOCK / 64];
+    __shared__ float red[2][R][BLOCK / 64];
+    GroupSum<BLOCK, R> sum{red, 0};
     const int l = threadIdx.x & (G - 1), per = BLOCK / G;
     const int nch = A.C / V;
-    const int64_t groups = (A.rows + per - 1) / per;
+    const Params<NC, V> p1(w1, A.root, 1.f, l, G, nch), ps(sc, 1.f, 1.f, l, G, nch), p2(w2, A.root, 1.f, l, G, nch);
+    const int64_t step = (int64_t)per * R;
     float s1[NC][V], s2[NC][V], s3[NC][V];
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int k = 0; k < V; ++k) s1[j][k] = s2[j][k] = s3[j][k] = 0.f;
-    for (int64_t blk = blockIdx.x; blk < groups; blk += gridDim.x) {
-        const int64_t row = blk * per + threadIdx.x / G;
-        const bool on = row < A.rows;
-        RowVec<E, V> vx[NC], vb[NC], vg[NC], vo[NC], vn[NC];
+    for (int64_t base = blockIdx.x * step; base < A.rows; base += gridDim.x * step) {
+        int64_t row[R];
+        bool on[R];
+        RowVec<E, V> vx[R][NC], vb[R][NC], vg[R][NC], vo[R][NC], vn[R][NC];
+        float r1[R], r2[R];
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const int ch = l + j * G;
-            if (on && ch < nch) {
-                if (w2) vx[j].load(x, row * A.xs + (int64_t)ch * V);
-                if (branch) vb[j].load(branch, row * A.bs + (int64_t)ch * V);
-                if (gate) vg[j].load(gate, row * A.gs + (int64_t)ch * V);
-                if (dout) vo[j].load(dout, row * A.C + (int64_t)ch * V);
-                if (w2 && dn) vn[j].load(dn, row * A.C + (int64_t)ch * V);
-            }
-        }
-        const float r1 = (on && branch && w1) ? rstd[row] : 0.f, r2 = (on && w2) ? rstd[A.rows + row] : 0.f;
-        float D[NC][V];                                // gradient that arrives at out
-        float dot = 0.f;
-        float o[NC][V];                                // out r2
-        if (w2 && dn) {
+        for (int i = 0; i < R; ++i) {
+            row[i] = base + i * per + threadIdx.x / G;
+            on[i] = row[i] < A.rows;
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
                 const int ch = l + j * G;
-                if (on && ch < nch) {
+                vx[i][j].clear(); vb[i][j].clear(); vg[i][j].clear(); vo[i][j].clear(); vn[i][j].clear();
+                if (on[i] && ch < nch) {
+                    if (w2 && dn) { vx[i][j].load(x, row[i] * A.xs + ch * V); vn[i][j].load(dn, row[i] * A.C + ch * V); }
+                    if (branch) vb[i][j].load(branch, row[i] * A.bs + ch * V);
+                    if (gate) vg[i][j].load(gate, row[i] * A.gs + ch * V);
+                    if (dout) vo[i][j].load(dout, row[i] * A.C + ch * V);
+                }
+            }
+            r1[i] = on[i] && branch && w1 ? rstd[row[i]] : 0.f;
+            r2[i] = on[i] && w2 ? rstd[A.rows + row[i]] : 0.f;
+        }
+        float D[R][NC][V];                             // gradient that arrives at out
+        float dot[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) dot[i] = 0.f;
+        if (w2 && dn) {
+            float o[R][NC][V];                         // out r2
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                float f1[V], fs[V], f2[V];
+                p1.get(j, f1); ps.get(j, fs); p2.get(j, f2);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
                     float fb[V], fg[V], fn[V];
-                    vx[j].get(o[j]); vn[j].get(fn);
-                    if (branch) { vb[j].get(fb); if (gate) vg[j].get(fg); }
+                    vx[i][j].get(o[i][j]); vn[i][j].get(fn); vb[i][j].get(fb); vg[i][j].get(fg);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const int c = ch * V + k;
                         if (branch) {
                             float u = fb[k];
-                            if (w1) u *= r1 * (A.root * w1[c]);
-                            if (gate) u *= gate_act(A.act, fg[k]);
-                            o[j][k] = sc ? fmaf(sc[c], u, o[j][k]) : o[j][k] + u;
+                            if (w1) u *= r1[i] * f1[k];
+                            if (gate) u *= gate_act<E>(A.act, fg[k]);
+                            o[i][j][k] = fmaf(fs[k], u, o[i][j][k]);
                         }
-                        o[j][k] *= r2;
-                        s3[j][k] = fmaf(fn[k], o[j][k], s3[j][k]);
-                        D[j][k] = fn[k] * (A.root * w2[c]);
-                        dot = fmaf(o[j][k], D[j][k], dot);
+                        o[i][j][k] *= r2[i];
+                        s3[j][k] = fmaf(fn[k], o[i][j][k], s3[j][k]);
+                        D[i][j][k] = fn[k] * f2[k];
+                        dot[i] = fmaf(o[i][j][k], D[i][j][k], dot[i]);
                     }
                 }
             }
-            dot = group_sum<BLOCK>(dot, G, red);
-            if (r2 >= 1e12f) dot = 0.f;                // |out| below the floor: N is linear there
+            sum(dot, G);
 #pragma unroll
-            for (int j = 0; j < NC; ++j)
-                if (on && l + j * G < nch)
+            for (int i = 0; i < R; ++i) {
+                if (r2[i] >= 1e12f) dot[i] = 0.f;      // |out| below the floor: N is linear there
 #pragma unroll
-                    for (int k = 0; k < V; ++k) D[j][k] = r2 * (D[j][k] - o[j][k] * dot);
+                for (int j = 0; j < NC; ++j)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) D[i][j][k] = r2[i] * (D[i][j][k] - o[i][j][k] * dot[i]);
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < NC; ++j)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int k = 0; k < V; ++k) D[j][k] = 0.f;
+                for (int j = 0; j < NC; ++j)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) D[i][j][k] = 0.f;
         }
-        float dot1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) dot[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const int ch = l + j * G;
-            if (on && ch < nch) {
-                if (dout) {
-                    float fo[V]; vo[j].get(fo);
+            float f1[V], fs[V];
+            p1.get(j, f1); ps.get(j, fs);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) D[j][k] += fo[k];
-                }
-                if (dx) RowVec<E, V>::store(dx, row * A.C + (int64_t)ch * V, D[j]);
+            for (int i = 0; i < R; ++i) {
+                const int ch = l + j * G;
+                const bool in = on[i] && ch < nch;
+                float fo[V];
+                vo[i][j].get(fo);
+#pragma unroll
+                for (int k = 0; k < V; ++k) D[i][j][k] += fo[k];
+                if (dx && in) RowVec<E, V>::store(dx, row[i] * A.C + ch * V, D[i][j]);
                 if (branch) {
                     float fb[V], fg[V], og[V];
-                    vb[j].get(fb);
-                    if (gate) vg[j].get(fg);
+                    vb[i][j].get(fb); vg[i][j].get(fg);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const int c = ch * V + k;
-                        const float b = w1 ? fb[k] * r1 : fb[k];
-                        const float rw = w1 ? A.root * w1[c] : 1.f;
-                        const float u = b * rw, s = sc ? sc[c] : 1.f;
+                        const float b = w1 ? fb[k] * r1[i] : fb[k];
+                        const float u = b * f1[k], d = D[i][j][k];
                         float act = 1.f, slope = 0.f;
-                        if (gate) gate_act_slope(A.act, fg[k], act, slope);
-                        const float d = D[j][k];
-                        og[k] = d * s * u * slope;
+                        if (gate) gate_act_slope<E>(A.act, fg[k], act, slope);
+                        og[k] = d * fs[k] * u * slope;
                         s2[j][k] = fmaf(d * act, u, s2[j][k]);
-                        const float db = d * s * act;
+                        const float db = d * fs[k] * act;
                         s1[j][k] = fmaf(db, b, s1[j][k]);
-                        D[j][k] = db * rw;
-                        dot1 = fmaf(D[j][k], b, dot1);
+                        D[i][j][k] = db * f1[k];
+                        dot[i] = fmaf(D[i][j][k], b, dot[i]);
                     }
-                    if (dgate) RowVec<E, V>::store(dgate, row * A.C + (int64_t)ch * V, og);
+                    if (dgate && in) RowVec<E, V>::store(dgate, row[i] * A.C + ch * V, og);
                 }
             }
         }
         if (!branch || !dbranch) continue;
-        if (w1) {
-            dot1 = group_sum<BLOCK>(dot1, G, red);
-            if (r1 >= 1e12f) dot1 = 0.f;
-        }
+        if (w1) sum(dot, G);
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const int ch = l + j * G;
-            if (on && ch < nch) {
+        for (int i = 0; i < R; ++i) {
+            if (r1[i] >= 1e12f) dot[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                const int ch = l + j * G;
                 if (w1) {
-                    float fb[V]; vb[j].get(fb);
+                    float fb[V]; vb[i][j].get(fb);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) D[j][k] = r1 * (D[j][k] - fb[k] * r1 * dot1);
+                    for (int k = 0; k < V; ++k) D[i][j][k] = r1[i] * (D[i][j][k] - fb[k] * r1[i] * dot[i]);
                 }
-                RowVec<E, V>::store(dbranch, row * A.C + (int64_t)ch * V, D[j]);
+                if (on[i] && ch < nch) RowVec<E, V>::store(dbranch, row[i] * A.C + ch * V, D[i][j]);
             }
         }
     }
     if (!parts) return;
-    // one group of the workgroup after the other adds its rows' sums
     float* o = parts + (int64_t)blockIdx.x * 3 * A.C;
-    for (int g = 0; g < per; ++g) {
-        if ((int)threadIdx.x / G == g) {
+    if (per == 1) {
 #pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                const int ch = l + j * G;
-                if (ch < nch)
+        for (int j = 0; j < NC; ++j) {
+            const int ch = l + j * G;
+            if (ch < nch)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        const int c = ch * V + k;
-                        const float a = s1[j][k] * A.root, b = s2[j][k], e = s3[j][k] * A.root;
-                        o[c] = g ? o[c] + a : a;
-                        o[A.C + c] = g ? o[A.C + c] + b : b;
-                        o[2 * A.C + c] = g ? o[2 * A.C + c] + e : e;
-                    }
-            }
+                for (int k = 0; k < V; ++k) {
+                    o[ch * V + k] = s1[j][k] * A.root; o[A.C + ch * V + k] = s2[j][k]; o[2 * A.C + ch * V + k] = s3[j][k] * A.root;
+                }
+        }
+    } else if (NC == 1) {                              // several groups per workgroup (then NC is 1): their sums meet in LDS, group after group
+        __shared__ float meet[NC == 1 ? 3 * V : 1][NC == 1 ? BLOCK : 1];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            meet[k][threadIdx.x] = s1[0][k] * A.root; meet[V + k][threadIdx.x] = s2[0][k]; meet[2 * V + k][threadIdx.x] = s3[0][k] * A.root;
         }
         __syncthreads();
+        for (int e = threadIdx.x; e < 3 * V * G; e += BLOCK) {
+            const int w = e / (V * G), c = e % (V * G), kk = w * V + c % V, ll = c / V;      // column c = ll * V + k of sum w
+            float s = 0.f;
+            for (int g = 0; g < per; ++g) s += meet[kk][g * G + ll];
+            if (c < A.C) o[w * A.C + c] = s;
+        }
     }
 }
 
-// column sums of `n` parts, 64 columns x 4 interleaved quarters per workgroup
-__global__ __launch_bounds__(256) void block_norm_cols_kernel(const float* __restrict__ parts, int n, int C, float* __restrict__ dw1, float* __restrict__ ds,
+// column sums of `n` parts: 32 columns per workgroup, 16 interleaved shares of the parts, eight loads in flight a thread
+__global__ __launch_bounds__(512) void block_norm_cols_kernel(const float* __restrict__ parts, int n, int C, float* __restrict__ dw1, float* __restrict__ ds,
                                                               float* __restrict__ dw2) {
-    __shared__ float red[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), quarter = threadIdx.x >> 6, which = blockIdx.y;
+    __shared__ float red[16][33];
+    const int cl = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + cl, which = blockIdx.y;
     float* out = which == 0 ? dw1 : which == 1 ? ds : dw2;
+    if (!out) return;
     float s = 0.f;
-    if (out && c < C)
-        for (int i = quarter; i < n; i += 4) s += parts[((int64_t)i * 3 + which) * C + c];
-    red[quarter][threadIdx.x & 63] = s;
+    if (c < C) {
+        const float* p = parts + (int64_t)which * C + c;
+        const int64_t pitch = (int64_t)3 * C;
+        int i = share;
+        for (; i + 7 * 16 < n; i += 8 * 16) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = p[(i + 16 * k) * pitch];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        for (; i < n; i += 16) s += p[i * pitch];
+    }
+    red[share][cl] = s;
     __syncthreads();
-    if (quarter == 0 && out && c < C) out[c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    if (share == 0 && c < C) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += red[i][cl];
+        out[c] = s;
+    }
 }
 
 // --------------------------------------------------------------------------- host side
+#define NORM_R 2                   // rows at a time, one chunk per thread: 16384 x 2048 bf16 73 us forward and 126 backward, one row 75 and 147, four 91 and 188
+#define NORM_GROUPS 1024           // workgroups from which on rows are taken NORM_R at a time
+#define NORM_BWD_MOST 1024         // workgroups of a backward pass at most
 static int norm_check(const mv2_block_norm_desc* d) {
     if (!d || d->reserved != 0) return MV2_EINVAL;
     if (d->dtype != MV2_BF16 && d->dtype != MV2_F32) return MV2_EINVAL;
@@ -293,29 +396,43 @@ static int norm_check(const mv2_block_norm_desc* d) {
     return MV2_OK;
 }
 
-// threads per row G and chunks per thread NC: the row's chunks spread over up to 256 threads first, then over registers
-struct NormShape { int V, NC, block, G; };
-static NormShape norm_shape(int C, int V) {
-    const int nch = C / V;
-    NormShape s{V, 1, 256, 1};
+// threads per row G, chunks per thread NC, rows at a time R: the row's chunks spread over up to 256 threads first, then over registers, then over
+// 1024 threads; R > 1 once every workgroup of a full chip has that many rows
+struct NormShape { int V, NC, R, block, G; };
+static NormShape norm_shape(const mv2_block_norm_desc* d, int V) {
+    const int nch = d->C / V;
+    NormShape s{V, 1, 1, 256, 1};
     while (s.G < nch && s.G < 256) s.G *= 2;
     if (nch > 256) {
-        if (V > 1) s.NC = nch <= 512 ? 2 : 4;
-        else s.NC = nch <= 1024 ? 4 : 16;
-        if (nch > 256 * s.NC) s.block = s.G = 1024;
+        s.NC = nch <= 512 ? 2 : V > 2 ? (nch <= 2048 ? 2 : 4) : (nch <= 4096 ? 4 : 16 / V);
+        while (s.G * s.NC < nch || (s.NC > 4 && s.G < 1024)) s.block = s.G *= 2;
     }
+    if (s.NC == 1 && d->rows / (s.block / s.G) >= (int64_t)NORM_R * NORM_GROUPS) s.R = NORM_R;
     return s;
 }
 
+// elements of one access: a 16-byte chunk, a pair of bf16, or one
+static int norm_access(const mv2_block_norm_desc* d, const void* branch, const void* gate, std::initializer_list<const void*> ps) {
+    const int es = d->dtype == MV2_BF16 ? 2 : 4;
+    return std::max(1, rows_access(ps, {(int64_t)d->C * es, d->x_stride * es, branch ? d->branch_stride * es : 0, gate ? d->gate_stride * es : 0}) / es);
+}
+
 static unsigned norm_grid(const mv2_block_norm_desc* d, const NormShape& s, int64_t most) {
-    const int64_t per = s.block / s.G, groups = (d->rows + per - 1) / per;
+    const int64_t per = (int64_t)s.block / s.G * s.R, groups = (d->rows + per - 1) / per;
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, most));
 }
-#define NORM_BWD_GRID 512          // workgroups of the backward pass at most: each leaves 3 C partial column sums
+
+// Workgroups of the backward pass: each leaves 3 C partial column sums, so three turns of the loop at least (1000 x 2048 bf16: 24 us from 256
+// to 512 workgroups, 28 from 768), and no more than the chip holds at once by the registers of the shapes (162 with two rows of one 16-byte
+// chunk, 195 with one row of two; 16384 x 2048: 126 us with 768, 140 with 512).
+static int64_t norm_bwd_grid(const mv2_block_norm_desc* d, const NormShape& s) {
+    const int64_t most = s.block > 256 ? 256 : s.V <= 2 ? NORM_BWD_MOST : s.NC == 1 ? 768 : 512;
+    return std::min(most, std::max<int64_t>(256, d->rows / ((int64_t)s.block / s.G * s.R) / 3));
+}
 
 extern "C" size_t mv2_block_norm_workspace_bytes(const mv2_block_norm_desc* d) {
     if (norm_check(d) != MV2_OK) return 0;
-    return (size_t)NORM_BWD_GRID * 3 * d->C * sizeof(float);
+    return (size_t)NORM_BWD_MOST * 3 * d->C * sizeof(float);
 }
 
 static NormArgs norm_args(const mv2_block_norm_desc* d) {
@@ -325,36 +442,38 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
     return A;
 }
 
-// one launch of KERNEL<E, V, NC, BLOCK> for the shape
+// one launch of KERNEL<E, V, NC, R, BLOCK> for the shape
 #define NORM_CASES(KERNEL, ...)                                                                                   \
     do {                                                                                                          \
         if (d->dtype == MV2_BF16) {                                                                               \
-            if (s.V == 8) {                                                                                       \
-                if (s.block == 1024) NORM_GO(KERNEL, BF16, 8, 4, 1024, __VA_ARGS__);                              \
-                else if (s.NC == 1) NORM_GO(KERNEL, BF16, 8, 1, 256, __VA_ARGS__);                                \
-                else if (s.NC == 2) NORM_GO(KERNEL, BF16, 8, 2, 256, __VA_ARGS__);                                \
-                else NORM_GO(KERNEL, BF16, 8, 4, 256, __VA_ARGS__);                                               \
-            } else {                                                                                              \
-                if (s.block == 1024) NORM_GO(KERNEL, BF16, 1, 16, 1024, __VA_ARGS__);                             \
-                else if (s.NC == 1) NORM_GO(KERNEL, BF16, 1, 1, 256, __VA_ARGS__);                                \
-                else if (s.NC == 4) NORM_GO(KERNEL, BF16, 1, 4, 256, __VA_ARGS__);                                \
-                else NORM_GO(KERNEL, BF16, 1, 16, 256, __VA_ARGS__);                                              \
-            }                                                                                                     \
+            if (s.V == 8) NORM_WIDE(KERNEL, BF16, 8, __VA_ARGS__)                                                 \
+            else if (s.V == 2) NORM_ODD(KERNEL, BF16, 2, __VA_ARGS__)                                             \
+            else NORM_ODD(KERNEL, BF16, 1, __VA_ARGS__)                                                           \
         } else {                                                                                                  \
-            if (s.V == 4) {                                                                                       \
-                if (s.block == 1024) NORM_GO(KERNEL, F32, 4, 4, 1024, __VA_ARGS__);                               \
-                else if (s.NC == 1) NORM_GO(KERNEL, F32, 4, 1, 256, __VA_ARGS__);                                 \
-                else if (s.NC == 2) NORM_GO(KERNEL, F32, 4, 2, 256, __VA_ARGS__);                                 \
-                else NORM_GO(KERNEL, F32, 4, 4, 256, __VA_ARGS__);                                                \
-            } else {                                                                                              \
-                if (s.block == 1024) NORM_GO(KERNEL, F32, 1, 16, 1024, __VA_ARGS__);                              \
-                else if (s.NC == 1) NORM_GO(KERNEL, F32, 1, 1, 256, __VA_ARGS__);                                 \
-                else if (s.NC == 4) NORM_GO(KERNEL, F32, 1, 4, 256, __VA_ARGS__);                                 \
-                else NORM_GO(KERNEL, F32, 1, 16, 256, __VA_ARGS__);                                               \
-            }                                                                                                     \
+            if (s.V == 4) NORM_WIDE(KERNEL, F32, 4, __VA_ARGS__)                                                  \
+            else NORM_ODD(KERNEL, F32, 1, __VA_ARGS__)                                                            \
         }                                                                                                         \
     } while (0)
-#define NORM_GO(KERNEL, E, V, NC, BLOCK, ...) hipLaunchKernelGGL((KERNEL<E, V, NC, BLOCK>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
+#define NORM_SHORT(KERNEL, E, V, ...)                                                                             \
+        if (s.NC == 1 && s.R == 1) NORM_GO(KERNEL, E, V, 1, 1, 256, __VA_ARGS__);                                 \
+        else if (s.NC == 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, __VA_ARGS__);                                   \
+        else if (s.block == 256 && s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 256, __VA_ARGS__);
+#define NORM_WIDE(KERNEL, E, V, ...)                                                                              \
+    {                                                                                                             \
+        NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \
+        else if (s.block == 512) NORM_GO(KERNEL, E, V, 2, 1, 512, __VA_ARGS__);                                   \
+        else if (s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 1024, __VA_ARGS__);                                       \
+        else NORM_GO(KERNEL, E, V, 4, 1, 1024, __VA_ARGS__);                                                      \
+    }
+#define NORM_ODD(KERNEL, E, V, ...)                                                                               \
+    {                                                                                                             \
+        NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \
+        else if (s.block == 256) NORM_GO(KERNEL, E, V, 4, 1, 256, __VA_ARGS__);                                   \
+        else if (s.block == 512) NORM_GO(KERNEL, E, V, 4, 1, 512, __VA_ARGS__);                                   \
+        else if (s.NC == 4) NORM_GO(KERNEL, E, V, 4, 1, 1024, __VA_ARGS__);                                       \
+        else NORM_GO(KERNEL, E, V, 16 / V, 1, 1024, __VA_ARGS__);                                                 \
+    }
+#define NORM_GO(KERNEL, E, V, NC, R, BLOCK, ...) hipLaunchKernelGGL((KERNEL<E, V, NC, R, BLOCK>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
 
 extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post_gamma,
                                       const float* scale, const float* pre_gamma, void* out, void* normed, float* rstd, void* stream) {
@@ -363,12 +482,11 @@ extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* 
     if (!branch && (gate || post_gamma || scale || !pre_gamma)) return MV2_EINVAL;
     if (d->rows == 0) return MV2_OK;
     if (!x || (branch && !out) || (pre_gamma && !normed)) return MV2_EINVAL;
-    const int kvec = d->dtype == MV2_BF16 ? 8 : 4;
-    const bool wide = d->C % kvec == 0 && d->x_stride % kvec == 0 && (!branch || d->branch_stride % kvec == 0) && (!gate || d->gate_stride % kvec == 0) &&
-                      rows_aligned16({x, branch, gate, out, normed});
-    const NormShape s = norm_shape(d->C, wide ? kvec : 1);
+    const int V = norm_access(d, branch, gate, {x, branch, gate, out, normed});
+    const NormShape s = norm_shape(d, V);
     const NormArgs A = norm_args(d);
-    const unsigned grid = norm_grid(d, s, 8192);
+    // workgroups at most: 16384 x 2048 71 us with 1024, 73 with 2048; narrow accesses want more in flight: 16384 x 1001 76 us with 4096, 85 with 1024
+    const unsigned grid = norm_grid(d, s, V <= 2 ? 4096 : 1024);
     hipStream_t st = (hipStream_t)stream;
     NORM_CASES(block_norm_fwd_kernel, x, branch, gate, post_gamma, scale, pre_gamma, out, normed, rstd);
     MV2_LAUNCH_CHECK();
@@ -386,18 +504,16 @@ extern "C" int mv2_block_norm_backward(const mv2_block_norm_desc* d, const void*
     if (d->rows > 0 && (!x || ((pre_gamma || post_gamma) && !rstd))) return MV2_EINVAL;
     const bool cols = dpost || dscale || dpre;
     if (cols && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < mv2_block_norm_workspace_bytes(d))) return MV2_EWORKSPACE;
-    const int kvec = d->dtype == MV2_BF16 ? 8 : 4;
-    const bool wide = d->C % kvec == 0 && d->x_stride % kvec == 0 && (!branch || d->branch_stride % kvec == 0) && (!gate || d->gate_stride % kvec == 0) &&
-                      rows_aligned16({x, branch, gate, dout, dn, dx, dbranch, dgate});
-    const NormShape s = norm_shape(d->C, wide ? kvec : 1);
+    const int V = norm_access(d, branch, gate, {x, branch, gate, dout, dn, dx, dbranch, dgate});
+    const NormShape s = norm_shape(d, V);
     const NormArgs A = norm_args(d);
-    const unsigned grid = norm_grid(d, s, NORM_BWD_GRID);
+    const unsigned grid = norm_grid(d, s, norm_bwd_grid(d, s));
     float* parts = cols ? (float*)workspace : nullptr;
     hipStream_t st = (hipStream_t)stream;
     NORM_CASES(block_norm_bwd_kernel, x, branch, gate, post_gamma, scale, pre_gamma, rstd, dout, dn, dx, dbranch, dgate, parts);
     MV2_LAUNCH_CHECK();
     if (cols) {
-        hipLaunchKernelGGL(block_norm_cols_kernel, dim3((unsigned)((d->C + 63) / 64), 3), dim3(256), 0, st, (const float*)parts, (int)grid, (int)d->C, dpost,
+        hipLaunchKernelGGL(block_norm_cols_kernel, dim3((unsigned)((d->C + 31) / 32), 3), dim3(512), 0, st, (const float*)parts, (int)grid, (int)d->C, dpost,
                            dscale, dpre);
         MV2_LAUNCH_CHECK();
     }

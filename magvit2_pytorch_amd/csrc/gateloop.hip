@@ -7,24 +7,6 @@
 #include <initializer_list>
 #include "rowvec.h"
 
-// sigmoid(a) and its slope g (1 - g) = e / (1 + e)^2 with e = exp(-|a|): no cancellation for either sign, no overflow, NaN stays NaN.
-// bf16 storage: hardware exp / rcp (1 ulp each, far below the stores' 2^-9); fp32: the library's exp and an exact division.
-template <typename E> struct Gate;
-template <> struct Gate<BF16> {
-    static __device__ __forceinline__ float recip(float v) { return __builtin_amdgcn_rcpf(v); }
-    static __device__ __forceinline__ float ex(float v) { return __expf(v); }
-};
-template <> struct Gate<F32> {
-    static __device__ __forceinline__ float recip(float v) { return 1.f / v; }
-    static __device__ __forceinline__ float ex(float v) { return expf(v); }
-};
-template <typename E> __device__ __forceinline__ float sigm(float a) { return Gate<E>::recip(1.f + Gate<E>::ex(-a)); }
-template <typename E> __device__ __forceinline__ void sigm_slope(float a, float& g, float& slope) {
-    const float e = Gate<E>::ex(-fabsf(a)), r = Gate<E>::recip(1.f + e), er = e * r;
-    g = a < 0.f ? er : r;
-    slope = er * r;
-}
-
 struct LoopArgs {
     int B, T, P, C;
     int64_t sb, st, sp;            // q, kv, a
@@ -644,14 +626,20 @@ static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, bool backward) 
 }
 #define SPAN_WAVES 8               // waves of a workgroup and tokens of a wave
 #define SPAN_TW 32
-// channels of a workgroup: 128-byte pieces of rows (64 bf16 or 32 fp32), 64 single elements where rows are not whole 16-byte chunks
-static int span_channels(const mv2_gateloop_desc* d, bool wide) { return wide && d->dtype == MV2_F32 ? 32 : 64; }
+// channels of a workgroup: 128-byte pieces of rows (64 bf16 or, in chunks of four, 32 fp32), 64 single elements of rows that are not whole chunks
+static int span_channels(bool fours) { return fours ? 32 : 64; }
 
 extern "C" size_t mv2_gateloop_workspace_bytes(const mv2_gateloop_desc* d, int backward) {
     if (loop_check(d) != MV2_OK || loop_walks(d)) return 0;
     int64_t words = 0;
-    for (int wide = 0; wide < 2; ++wide) words = std::max(words, span_shape(d, span_channels(d, wide), backward != 0).words);      // whichever the addresses allow
+    for (int fours = 0; fours < 2; ++fours) words = std::max(words, span_shape(d, span_channels(fours), backward != 0).words);      // whichever the addresses allow
     return (size_t)words * sizeof(u64);
+}
+
+// elements of one access: a 16-byte chunk, a pair of bf16, or one
+static int loop_access(const mv2_gateloop_desc* d, bool backward, std::initializer_list<const void*> ps) {
+    const int64_t es = d->dtype == MV2_BF16 ? 2 : 4, g = backward ? es : 0;
+    return (int)std::max<int64_t>(1, rows_access(ps, {d->C * es, d->in_b * es, d->in_t * es, d->in_p * es, d->grad_b * g, d->grad_t * g, d->grad_p * g}) / es);
 }
 
 static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, const unsigned char* resets) {
@@ -664,8 +652,8 @@ static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, co
 }
 
 // the pairs' words, cleared by a kernel (a captured memset would not do: the launch may be recorded into a graph)
-static int span_work(const mv2_gateloop_desc* d, bool wide, bool backward, void* workspace, size_t workspace_bytes, hipStream_t st, SpanWork& W, unsigned& grid) {
-    const int nch = span_channels(d, wide);
+static int span_work(const mv2_gateloop_desc* d, bool fours, bool backward, void* workspace, size_t workspace_bytes, hipStream_t st, SpanWork& W, unsigned& grid) {
+    const int nch = span_channels(fours);
     const SpanShape s = span_shape(d, nch, backward);
     if ((double)s.nblk * (s.ntile + 8) > 2147483647.0) return MV2_ETOOLARGE;
     W.nblk = (int)s.nblk; W.ntile = (int)s.ntile; W.ctiles = (int)s.ctiles;
@@ -688,25 +676,24 @@ extern "C" int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, c
     if (rc != MV2_OK) return rc;
     if (d->T > 0 && (!q || !kv || !a || !y)) return MV2_EINVAL;
     const LoopArgs A = loop_args(d, lengths, resets);
-    const int kvec = d->dtype == MV2_BF16 ? 8 : 4;
-    const bool wide = d->C % kvec == 0 && d->in_b % kvec == 0 && d->in_t % kvec == 0 && d->in_p % kvec == 0 && rows_aligned16({q, kv, a, y});
+    const int V = loop_access(d, false, {q, kv, a, y});
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
-        const int64_t n = (int64_t)d->B * d->P * (d->C / (wide ? kvec : 1));
+        const int64_t n = (int64_t)d->B * d->P * (d->C / V);
         const dim3 grid((unsigned)((n + 255) / 256));
 #define GO(E, V) hipLaunchKernelGGL((loop_walk_fwd_kernel<E, V>), grid, dim3(256), 0, st, A, q, kv, a, h0, y, h_last, states)
-        if (d->dtype == MV2_BF16) { if (wide) GO(BF16, 8); else GO(BF16, 1); }
-        else { if (wide) GO(F32, 4); else GO(F32, 1); }
+        if (d->dtype == MV2_BF16) { if (V == 8) GO(BF16, 8); else if (V == 2) GO(BF16, 2); else GO(BF16, 1); }
+        else { if (V == 4) GO(F32, 4); else GO(F32, 1); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
-        rc = span_work(d, wide, false, workspace, workspace_bytes, st, W, grid);
+        rc = span_work(d, V == 4, false, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
 #define GO(E, V, CL, CUTS) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
 #define GO2(E, V, CL) do { if (resets) GO(E, V, CL, true); else GO(E, V, CL, false); } while (0)
-        if (d->dtype == MV2_BF16) { if (wide) GO2(BF16, 8, 8); else GO2(BF16, 1, 64); }
-        else { if (wide) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
+        if (d->dtype == MV2_BF16) { if (V == 8) GO2(BF16, 8, 8); else if (V == 2) GO2(BF16, 2, 32); else GO2(BF16, 1, 64); }
+        else { if (V == 4) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
 #undef GO2
 #undef GO
     }
@@ -722,27 +709,25 @@ extern "C" int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, 
     if (d->T > 0 && (!q || !kv || !a || !dy || !dq || !dkv || !da)) return MV2_EINVAL;
     const LoopArgs A = loop_args(d, lengths, resets);
     if (A.nstate > 0 && !states) return MV2_EINVAL;
-    const int kvec = d->dtype == MV2_BF16 ? 8 : 4;
-    const bool wide = d->C % kvec == 0 && d->in_b % kvec == 0 && d->in_t % kvec == 0 && d->in_p % kvec == 0 && d->grad_b % kvec == 0 &&
-                      d->grad_t % kvec == 0 && d->grad_p % kvec == 0 && rows_aligned16({q, kv, a, dy, dq, dkv, da});
+    const int V = loop_access(d, true, {q, kv, a, dy, dq, dkv, da});
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
-        const int64_t n = (int64_t)d->B * d->P * (d->C / (wide ? kvec / 2 : 1));
+        const int64_t n = (int64_t)d->B * d->P * (d->C / (V > 2 ? V / 2 : V));
         const dim3 grid((unsigned)((n + 255) / 256));
 #define GO(E, V) hipLaunchKernelGGL((loop_walk_bwd_kernel<E, V>), grid, dim3(256), 0, st, A, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-        if (d->dtype == MV2_BF16) { if (wide) GO(BF16, 4); else GO(BF16, 1); }
-        else { if (wide) GO(F32, 2); else GO(F32, 1); }
+        if (d->dtype == MV2_BF16) { if (V == 8) GO(BF16, 4); else if (V == 2) GO(BF16, 2); else GO(BF16, 1); }
+        else { if (V == 4) GO(F32, 2); else GO(F32, 1); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
-        rc = span_work(d, wide, true, workspace, workspace_bytes, st, W, grid);
+        rc = span_work(d, V == 4, true, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
 #define GO(E, V, CL, CUTS)                                                                                                                                    \
     hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
 #define GO2(E, V, CL) do { if (resets) GO(E, V, CL, true); else GO(E, V, CL, false); } while (0)
-        if (d->dtype == MV2_BF16) { if (wide) GO2(BF16, 8, 8); else GO2(BF16, 1, 64); }
-        else { if (wide) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
+        if (d->dtype == MV2_BF16) { if (V == 8) GO2(BF16, 8, 8); else if (V == 2) GO2(BF16, 2, 32); else GO2(BF16, 1, 64); }
+        else { if (V == 4) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
 #undef GO2
 #undef GO
     }
