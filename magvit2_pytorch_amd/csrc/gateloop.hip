@@ -26,6 +26,20 @@ __device__ __forceinline__ int live_tokens(const LoopArgs& A, int b) {
 }
 
 // --------------------------------------------------------------------------- one thread per chunk of channels walks its tokens
+// chunk i -> sequence, chunk of its row, sample, pixel (divisions in 32 bits where they do: a quarter of a single token's kernel otherwise)
+__device__ __forceinline__ void walk_place(const LoopArgs& A, int64_t i, int64_t total, int cpr, int64_t& seq, int& chunk, int& b, int& p) {
+    if (total <= 0x7fffffff) {
+        const unsigned s = (unsigned)i / (unsigned)cpr;
+        chunk = (int)((unsigned)i - s * (unsigned)cpr);
+        b = (int)(s / (unsigned)A.P); p = (int)(s - (unsigned)b * (unsigned)A.P);
+        seq = s;
+    } else {
+        seq = i / cpr;
+        chunk = (int)(i - seq * cpr);
+        b = (int)(seq / A.P); p = (int)(seq - (int64_t)b * A.P);
+    }
+}
+
 template <typename E, int V>
 __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const void* __restrict__ q, const void* __restrict__ kv, const void* __restrict__ a,
                                                             const float* h0, void* __restrict__ y, float* hlast, float* __restrict__ states) {
@@ -33,9 +47,10 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
     const int64_t total = (int64_t)A.B * A.P * cpr;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
-    const int64_t seq = i / cpr;
-    const int c = (int)(i - seq * cpr) * V;
-    const int b = (int)(seq / A.P), p = (int)(seq - (int64_t)b * A.P);
+    int64_t seq;
+    int c, b, p;
+    walk_place(A, i, total, cpr, seq, c, b, p);
+    c *= V;
     const int n = live_tokens(A, b);
     const int64_t in0 = b * A.sb + p * A.sp + c;
     const int64_t yt = (int64_t)A.P * A.C, y0 = (int64_t)b * A.T * yt + (int64_t)p * A.C + c;
@@ -107,9 +122,10 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
     const int64_t total = (int64_t)A.B * A.P * cpr;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
-    const int64_t seq = i / cpr;
-    const int c = (int)(i - seq * cpr) * V;
-    const int b = (int)(seq / A.P), p = (int)(seq - (int64_t)b * A.P);
+    int64_t seq;
+    int c, b, p;
+    walk_place(A, i, total, cpr, seq, c, b, p);
+    c *= V;
     const int n = live_tokens(A, b);
     const int64_t in0 = b * A.sb + p * A.sp + c, g0 = b * A.gb + p * A.gp + c;
     const int64_t yt = (int64_t)A.P * A.C, y0 = (int64_t)b * A.T * yt + (int64_t)p * A.C + c;
@@ -364,10 +380,13 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 g[i][k] = sigm<E>(fa[k]);
-                const float r = fmaf(g[i][k], ph[k], fk[k]);
-                ph[k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
                 pa[k] *= g[i][k];
             }
+#pragma unroll
+            for (int k = 0; k < V; ++k) ph[k] = fmaf(g[i][k], ph[k], fk[k]);
+            if (CUTS && __any(cuts >> i & 1))                 // documents start in few waves: the others do without the choice
+#pragma unroll
+                for (int k = 0; k < V; ++k) ph[k] = cuts >> i & 1 ? fk[k] : ph[k];
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) { rowA[row][cl * V + k] = CUTS && cuts ? LOOP_CUT : pa[k]; rowH[row][cl * V + k] = ph[k]; }
@@ -392,11 +411,12 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
         float fk[V], fq[V];
         vk[i].get(fk); vq[i].get(fq);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float r = fmaf(g[i][k], h[k], fk[k]);
-            h[k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
-            fq[k] *= h[k];
-        }
+        for (int k = 0; k < V; ++k) h[k] = fmaf(g[i][k], h[k], fk[k]);
+        if (CUTS && __any(cuts >> i & 1))
+#pragma unroll
+            for (int k = 0; k < V; ++k) h[k] = cuts >> i & 1 ? fk[k] : h[k];
+#pragma unroll
+        for (int k = 0; k < V; ++k) fq[k] *= h[k];
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) fq[k] = 0.f;
@@ -486,20 +506,23 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
             vk[i].get(fk);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const float g = decay(i, k), r = fmaf(g, ph[k], fk[k]);
-                ph[k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
+                const float g = decay(i, k);
+                ph[k] = fmaf(g, ph[k], fk[k]);
                 pa[k] *= g;
             }
+            if (CUTS && __any(cuts >> i & 1))                 // documents start in few waves: the others do without the choice
+#pragma unroll
+                for (int k = 0; k < V; ++k) ph[k] = cuts >> i & 1 ? fk[k] : ph[k];
         }
 #pragma unroll
         for (int i = L - 1; i >= 0; --i) {
             float fq[V], fy[V];
             vq[i].get(fq); vy[i].get(fy);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float r = decay(i, k) * fmaf(fq[k], fy[k], pu[k]);
-                pu[k] = CUTS && (cuts >> i & 1) ? 0.f : r;
-            }
+            for (int k = 0; k < V; ++k) pu[k] = decay(i, k) * fmaf(fq[k], fy[k], pu[k]);
+            if (CUTS && __any(cuts >> i & 1))
+#pragma unroll
+                for (int k = 0; k < V; ++k) pu[k] = cuts >> i & 1 ? 0.f : pu[k];
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -538,11 +561,12 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
         float fk[V], fy[V];
         vk[i].get(fk); vy[i].get(fy);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float r = fmaf(decay(i, k), h[i][k], fk[k]);
-            h[i + 1][k] = CUTS && (cuts >> i & 1) ? fk[k] : r;
-            fy[k] *= h[i + 1][k];
-        }
+        for (int k = 0; k < V; ++k) h[i + 1][k] = fmaf(decay(i, k), h[i][k], fk[k]);
+        if (CUTS && __any(cuts >> i & 1))
+#pragma unroll
+            for (int k = 0; k < V; ++k) h[i + 1][k] = cuts >> i & 1 ? fk[k] : h[i + 1][k];
+#pragma unroll
+        for (int k = 0; k < V; ++k) fy[k] *= h[i + 1][k];
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) fy[k] = 0.f;
@@ -552,15 +576,19 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
     for (int i = L - 1; i >= 0; --i) {
         float fq[V], fy[V], oa[V];
         vq[i].get(fq); vy[i].get(fy);
-        const bool cut = CUTS && (cuts >> i & 1);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const float s = fabsf(m[i][k]), g = decay(i, k);
+            const float s = fabsf(m[i][k]);
             fq[k] = fmaf(fq[k], fy[k], back[k]);
-            const float r = fq[k] * h[i][k] * (s * (1.f - s));
-            oa[k] = cut ? 0.f : r;
-            back[k] = cut ? 0.f : g * fq[k];
+            oa[k] = fq[k] * h[i][k] * (s * (1.f - s));
+            back[k] = decay(i, k) * fq[k];
         }
+        if (CUTS && __any(cuts >> i & 1))
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                oa[k] = cuts >> i & 1 ? 0.f : oa[k];
+                back[k] = cuts >> i & 1 ? 0.f : back[k];
+            }
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) { back[k] = fq[k]; fq[k] = 0.f; oa[k] = 0.f; }
