@@ -62,27 +62,21 @@ template <typename E> __device__ __forceinline__ void gate_act_slope(int act, fl
     if (act == MV2_ACT_SIGMOID) { v = s; d = ds; }
     else { v = g * s; d = fmaf(g, ds, s); }
 }
-// 1 / max(|v|, 1e-12) from the sum of squares
-__device__ __forceinline__ float inv_norm(float ss) { return 1.f / fmaxf(sqrtf(ss), 1e-12f); }
+// 1 / max(|v|, 1e-12) from the sum of squares; NaN stays NaN (fmaxf would drop it, and the row's other elements would come out finite)
+__device__ __forceinline__ float inv_norm(float ss) {
+    const float n = sqrtf(ss);
+    return 1.f / (n < 1e-12f ? 1e-12f : n);
+}
 
-// a thread's parameters: f times w, or d where there is none; kept in registers for up to 16 elements, read again (from the caches) beyond
-// (7000 x 4096 bf16, 16 a thread: 60 us forward kept, 136 read again)
+// a thread's parameters, f times w, or ones where there are none: in registers for all the rows (7000 x 4096 bf16, 16 a thread: 60 us forward;
+// read again with every row 136)
 template <int NC, int V> struct Params {
-    static constexpr bool KEPT = NC * V <= 16;
-    float r[KEPT ? NC : 1][KEPT ? V : 1];
-    const float* w;
-    float f, d;
-    int l, G, nch;
-    __device__ __forceinline__ Params(const float* w_, float f_, float d_, int l_, int G_, int nch_) : w(w_), f(f_), d(d_), l(l_), G(G_), nch(nch_) {
-        if (KEPT)
+    float r[NC][V];
+    __device__ __forceinline__ Params(const float* w, float f, int l, int G, int nch) {
 #pragma unroll
-            for (int j = 0; j < NC; ++j)
+        for (int j = 0; j < NC; ++j)
 #pragma unroll
-                for (int k = 0; k < V; ++k) r[KEPT ? j : 0][KEPT ? k : 0] = w && l + j * G < nch ? f * w[(l + j * G) * V + k] : d;
-    }
-    __device__ __forceinline__ void get(int j, float* o) const {
-#pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = KEPT ? r[KEPT ? j : 0][KEPT ? k : 0] : (w ? f * w[(l + j * G) * V + k] : d);
+            for (int k = 0; k < V; ++k) r[j][k] = w && l + j * G < nch ? f * w[(l + j * G) * V + k] : 1.f;
     }
 };
 
@@ -94,7 +88,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
     GroupSum<BLOCK, R> sum{red, 0};
     const int l = threadIdx.x & (G - 1), per = BLOCK / G;
     const int nch = A.C / V;
-    const Params<NC, V> p1(w1, A.root, 1.f, l, G, nch), ps(sc, 1.f, 1.f, l, G, nch), p2(w2, A.root, 1.f, l, G, nch);
+    const Params<NC, V> p1(w1, A.root, l, G, nch), ps(sc, 1.f, l, G, nch), p2(w2, A.root, l, G, nch);
     const int64_t step = (int64_t)per * R;
     for (int64_t base = blockIdx.x * step; base < A.rows; base += gridDim.x * step) {
         int64_t row[R];
@@ -115,7 +109,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
             }
         }
         float r1[R], r2[R];
-        if (branch && (w1 || rstd)) {
+        if (w1) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 r1[i] = 0.f;
@@ -138,8 +132,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
         for (int i = 0; i < R; ++i) r2[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            float f1[V], fs[V];
-            p1.get(j, f1); ps.get(j, fs);
+            const float (&f1)[V] = p1.r[j], (&fs)[V] = ps.r[j];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int ch = l + j * G;
@@ -170,8 +163,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
         }
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            float f2[V];
-            p2.get(j, f2);
+            const float (&f2)[V] = p2.r[j];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int ch = l + j * G;
@@ -194,7 +186,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
     GroupSum<BLOCK, R> sum{red, 0};
     const int l = threadIdx.x & (G - 1), per = BLOCK / G;
     const int nch = A.C / V;
-    const Params<NC, V> p1(w1, A.root, 1.f, l, G, nch), ps(sc, 1.f, 1.f, l, G, nch), p2(w2, A.root, 1.f, l, G, nch);
+    const Params<NC, V> p1(w1, A.root, l, G, nch), ps(sc, 1.f, l, G, nch), p2(w2, A.root, l, G, nch);
     const int64_t step = (int64_t)per * R;
     float s1[NC][V], s2[NC][V], s3[NC][V];
 #pragma unroll
@@ -232,8 +224,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
             float o[R][NC][V];                         // out r2
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                float f1[V], fs[V], f2[V];
-                p1.get(j, f1); ps.get(j, fs); p2.get(j, f2);
+                const float (&f1)[V] = p1.r[j], (&fs)[V] = ps.r[j], (&f2)[V] = p2.r[j];
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
                     float fb[V], fg[V], fn[V];
@@ -274,8 +265,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
         for (int i = 0; i < R; ++i) dot[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            float f1[V], fs[V];
-            p1.get(j, f1); ps.get(j, fs);
+            const float (&f1)[V] = p1.r[j], (&fs)[V] = ps.r[j];
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const int ch = l + j * G;
@@ -446,11 +436,11 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
 #define NORM_CASES(KERNEL, ...)                                                                                   \
     do {                                                                                                          \
         if (d->dtype == MV2_BF16) {                                                                               \
-            if (s.V == 8) NORM_WIDE(KERNEL, BF16, 8, __VA_ARGS__)                                                 \
+            if (s.V == 8) { NORM_WIDE(KERNEL, BF16, 8, __VA_ARGS__) }                                             \
             else if (s.V == 2) NORM_ODD(KERNEL, BF16, 2, __VA_ARGS__)                                             \
             else NORM_ODD(KERNEL, BF16, 1, __VA_ARGS__)                                                           \
         } else {                                                                                                  \
-            if (s.V == 4) NORM_WIDE(KERNEL, F32, 4, __VA_ARGS__)                                                  \
+            if (s.V == 4) { NORM_WIDE(KERNEL, F32, 4, __VA_ARGS__) else NORM_GO(KERNEL, F32, 4, 4, 1, 1024, __VA_ARGS__); } \
             else NORM_ODD(KERNEL, F32, 1, __VA_ARGS__)                                                            \
         }                                                                                                         \
     } while (0)
@@ -459,12 +449,9 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
         else if (s.NC == 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, __VA_ARGS__);                                   \
         else if (s.block == 256 && s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 256, __VA_ARGS__);
 #define NORM_WIDE(KERNEL, E, V, ...)                                                                              \
-    {                                                                                                             \
         NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \
         else if (s.block == 512) NORM_GO(KERNEL, E, V, 2, 1, 512, __VA_ARGS__);                                   \
-        else if (s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 1024, __VA_ARGS__);                                       \
-        else NORM_GO(KERNEL, E, V, 4, 1, 1024, __VA_ARGS__);                                                      \
-    }
+        else if (s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 1024, __VA_ARGS__);
 #define NORM_ODD(KERNEL, E, V, ...)                                                                               \
     {                                                                                                             \
         NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \

@@ -617,7 +617,7 @@ static int loop_check(const mv2_gateloop_desc* d) {
     if ((double)d->B * d->T * d->P * d->C > far) return MV2_ETOOLARGE;
     if ((double)d->B * d->in_b + (double)d->T * d->in_t + (double)d->P * d->in_p > far) return MV2_ETOOLARGE;
     if ((double)d->B * d->grad_b + (double)d->T * d->grad_t + (double)d->P * d->grad_p > far) return MV2_ETOOLARGE;
-    if (((double)d->B * d->P * d->C + 255) / 256 > 2147483647.0) return MV2_ETOOLARGE;
+    if ((double)d->B * d->P * d->C > 4294967040.0) return MV2_ETOOLARGE;      // threads of a launch: 32 bits
     return MV2_OK;
 }
 
@@ -683,7 +683,7 @@ static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, co
 static int span_work(const mv2_gateloop_desc* d, bool fours, bool backward, void* workspace, size_t workspace_bytes, hipStream_t st, SpanWork& W, unsigned& grid) {
     const int nch = span_channels(fours);
     const SpanShape s = span_shape(d, nch, backward);
-    if ((double)s.nblk * (s.ntile + 8) > 2147483647.0) return MV2_ETOOLARGE;
+    if ((double)s.nblk * (s.ntile + 8) * 64 * SPAN_WAVES > 4294967040.0) return MV2_ETOOLARGE;
     W.nblk = (int)s.nblk; W.ntile = (int)s.ntile; W.ctiles = (int)s.ctiles;
     W.nq = (int)s.nq;
     grid = (unsigned)(s.nblk > 1 ? s.nblk * s.nq * ((s.ntile + s.nq - 1) / s.nq) : s.ntile);

@@ -372,7 +372,7 @@ def test_a_row_of_nan_stays_in_its_row(dtype):
     g = torch.ones(C, device='cuda')
     o1, n1 = F.block_norm(x, b, post_gamma=g, pre_gamma=g)
     b2 = b.clone()
-    b2[33] = NAN
+    b2[33, 5] = NAN                                       # one element: the row's norm is NaN, and so is all of the row
     o2, n2 = F.block_norm(x, b2, post_gamma=g, pre_gamma=g)
     rest = torch.arange(R, device='cuda') != 33
     assert o2[33].isnan().all() and n2[33].isnan().all() and torch.equal(o1[rest], o2[rest]) and torch.equal(n1[rest], n2[rest])
