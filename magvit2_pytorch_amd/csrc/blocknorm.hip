@@ -80,7 +80,7 @@ template <int NC, int V> struct Params {
     }
 };
 
-template <typename E, int V, int NC, int R, int BLOCK>
+template <typename E, int V, int NC, int R, int BLOCK, bool S>
 __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G, const void* x, const void* __restrict__ branch, const void* __restrict__ gate,
                                                                const float* __restrict__ w1, const float* __restrict__ sc, const float* __restrict__ w2,
                                                                void* out, void* __restrict__ normed, float* __restrict__ rstd) {
@@ -102,9 +102,9 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
             for (int j = 0; j < NC; ++j) {
                 const int ch = l + j * G;
                 if (on[i] && ch < nch) {
-                    vx[i][j].load(x, row[i] * A.xs + ch * V);
-                    if (branch) vb[i][j].load(branch, row[i] * A.bs + ch * V);
-                    if (gate) vg[i][j].load(gate, row[i] * A.gs + ch * V);
+                    vx[i][j].template load<S>(x, row[i] * A.xs + ch * V);
+                    if (branch) vb[i][j].template load<S>(branch, row[i] * A.bs + ch * V);
+                    if (gate) vg[i][j].template load<S>(gate, row[i] * A.gs + ch * V);
                 } else { vx[i][j].clear(); vb[i][j].clear(); vg[i][j].clear(); }
             }
         }
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
                         if (gate) u *= gate_act<E>(A.act, fg[k]);
                         o[i][j][k] = fmaf(fs[k], u, o[i][j][k]);
                     }
-                    if (on[i] && ch < nch) RowVec<E, V>::store(out, row[i] * A.C + ch * V, o[i][j]);
+                    if (on[i] && ch < nch) RowVec<E, V>::template store<S>(out, row[i] * A.C + ch * V, o[i][j]);
                 }
                 if (on[i] && ch < nch)
 #pragma unroll
@@ -169,14 +169,14 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
                 const int ch = l + j * G;
 #pragma unroll
                 for (int k = 0; k < V; ++k) o[i][j][k] *= r2[i] * f2[k];
-                if (on[i] && ch < nch) RowVec<E, V>::store(normed, row[i] * A.C + ch * V, o[i][j]);
+                if (on[i] && ch < nch) RowVec<E, V>::template store<S>(normed, row[i] * A.C + ch * V, o[i][j]);
             }
         }
     }
 }
 
 // parts: [gridDim.x][3][C] column sums of a workgroup's rows (dw1, ds, dw2), summed in workgroup order by block_norm_cols_kernel
-template <typename E, int V, int NC, int R, int BLOCK>
+template <typename E, int V, int NC, int R, int BLOCK, bool S>
 __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G, const void* __restrict__ x, const void* __restrict__ branch,
                                                                const void* __restrict__ gate, const float* __restrict__ w1, const float* __restrict__ sc,
                                                                const float* __restrict__ w2, const float* __restrict__ rstd, const void* __restrict__ dout,
@@ -207,10 +207,10 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
                 const int ch = l + j * G;
                 vx[i][j].clear(); vb[i][j].clear(); vg[i][j].clear(); vo[i][j].clear(); vn[i][j].clear();
                 if (on[i] && ch < nch) {
-                    if (w2 && dn) { vx[i][j].load(x, row[i] * A.xs + ch * V); vn[i][j].load(dn, row[i] * A.C + ch * V); }
-                    if (branch) vb[i][j].load(branch, row[i] * A.bs + ch * V);
-                    if (gate) vg[i][j].load(gate, row[i] * A.gs + ch * V);
-                    if (dout) vo[i][j].load(dout, row[i] * A.C + ch * V);
+                    if (w2 && dn) { vx[i][j].template load<S>(x, row[i] * A.xs + ch * V); vn[i][j].template load<S>(dn, row[i] * A.C + ch * V); }
+                    if (branch) vb[i][j].template load<S>(branch, row[i] * A.bs + ch * V);
+                    if (gate) vg[i][j].template load<S>(gate, row[i] * A.gs + ch * V);
+                    if (dout) vo[i][j].template load<S>(dout, row[i] * A.C + ch * V);
                 }
             }
             r1[i] = on[i] && branch && w1 ? rstd[row[i]] : 0.f;
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
                 vo[i][j].get(fo);
 #pragma unroll
                 for (int k = 0; k < V; ++k) D[i][j][k] += fo[k];
-                if (dx && in) RowVec<E, V>::store(dx, row[i] * A.C + ch * V, D[i][j]);
+                if (dx && in) RowVec<E, V>::template store<S>(dx, row[i] * A.C + ch * V, D[i][j]);
                 if (branch) {
                     float fb[V], fg[V], og[V];
                     vb[i][j].get(fb); vg[i][j].get(fg);
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
                         D[i][j][k] = db * f1[k];
                         dot[i] = fmaf(D[i][j][k], b, dot[i]);
                     }
-                    if (dgate && in) RowVec<E, V>::store(dgate, row[i] * A.C + ch * V, og);
+                    if (dgate && in) RowVec<E, V>::template store<S>(dgate, row[i] * A.C + ch * V, og);
                 }
             }
         }
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
 #pragma unroll
                     for (int k = 0; k < V; ++k) D[i][j][k] = r1[i] * (D[i][j][k] - fb[k] * r1[i] * dot[i]);
                 }
-                if (on[i] && ch < nch) RowVec<E, V>::store(dbranch, row[i] * A.C + ch * V, D[i][j]);
+                if (on[i] && ch < nch) RowVec<E, V>::template store<S>(dbranch, row[i] * A.C + ch * V, D[i][j]);
             }
         }
     }
@@ -388,10 +388,10 @@ static int norm_check(const mv2_block_norm_desc* d) {
 
 // threads per row G, chunks per thread NC, rows at a time R: the row's chunks spread over up to 256 threads first, then over registers, then over
 // 1024 threads; R > 1 once every workgroup of a full chip has that many rows
-struct NormShape { int V, NC, R, block, G; };
-static NormShape norm_shape(const mv2_block_norm_desc* d, int V) {
+struct NormShape { int V, NC, R, block, G; bool stream; };
+static NormShape norm_shape(const mv2_block_norm_desc* d, int V, int tensors) {
     const int nch = d->C / V;
-    NormShape s{V, 1, 1, 256, 1};
+    NormShape s{V, 1, 1, 256, 1, V > 2 && calls_stream((double)d->rows * d->C * tensors * (d->dtype == MV2_BF16 ? 2 : 4))};
     while (s.G < nch && s.G < 256) s.G *= 2;
     if (nch > 256) {
         s.NC = nch <= 512 ? 2 : V > 2 ? (nch <= 2048 ? 2 : 4) : (nch <= 4096 ? 4 : 16 / V);
@@ -432,7 +432,8 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
     return A;
 }
 
-// one launch of KERNEL<E, V, NC, R, BLOCK> for the shape
+// one launch of KERNEL<E, V, NC, R, BLOCK, S> for the shape; S, past the caches: where the call is large, and always at widths beyond 512 chunks (a row of
+// a thousand and more threads: 2000 x 16384 81 us forward, 95 through the caches)
 #define NORM_CASES(KERNEL, ...)                                                                                   \
     do {                                                                                                          \
         if (d->dtype == MV2_BF16) {                                                                               \
@@ -440,27 +441,29 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
             else if (s.V == 2) NORM_ODD(KERNEL, BF16, 2, __VA_ARGS__)                                             \
             else NORM_ODD(KERNEL, BF16, 1, __VA_ARGS__)                                                           \
         } else {                                                                                                  \
-            if (s.V == 4) { NORM_WIDE(KERNEL, F32, 4, __VA_ARGS__) else NORM_GO(KERNEL, F32, 4, 4, 1, 1024, __VA_ARGS__); } \
+            if (s.V == 4) { NORM_WIDE(KERNEL, F32, 4, __VA_ARGS__) else NORM_GO(KERNEL, F32, 4, 4, 1, 1024, true, __VA_ARGS__); } \
             else NORM_ODD(KERNEL, F32, 1, __VA_ARGS__)                                                            \
         }                                                                                                         \
     } while (0)
 #define NORM_SHORT(KERNEL, E, V, ...)                                                                             \
-        if (s.NC == 1 && s.R == 1) NORM_GO(KERNEL, E, V, 1, 1, 256, __VA_ARGS__);                                 \
-        else if (s.NC == 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, __VA_ARGS__);                                   \
-        else if (s.block == 256 && s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 256, __VA_ARGS__);
+        if (s.NC == 1 && s.R == 1) NORM_GO(KERNEL, E, V, 1, 1, 256, false, __VA_ARGS__);                          \
+        else if (s.NC == 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, false, __VA_ARGS__);                            \
+        else if (s.block == 256 && s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 256, false, __VA_ARGS__);
 #define NORM_WIDE(KERNEL, E, V, ...)                                                                              \
-        NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \
-        else if (s.block == 512) NORM_GO(KERNEL, E, V, 2, 1, 512, __VA_ARGS__);                                   \
-        else if (s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 1024, __VA_ARGS__);
+        if (s.stream && s.NC == 1 && s.R > 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, true, __VA_ARGS__);           \
+        else if (s.stream && s.NC == 2 && s.block == 256) NORM_GO(KERNEL, E, V, 2, 1, 256, true, __VA_ARGS__);    \
+        else NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                \
+        else if (s.block == 512) NORM_GO(KERNEL, E, V, 2, 1, 512, true, __VA_ARGS__);                             \
+        else if (s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 1024, true, __VA_ARGS__);
 #define NORM_ODD(KERNEL, E, V, ...)                                                                               \
     {                                                                                                             \
         NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \
-        else if (s.block == 256) NORM_GO(KERNEL, E, V, 4, 1, 256, __VA_ARGS__);                                   \
-        else if (s.block == 512) NORM_GO(KERNEL, E, V, 4, 1, 512, __VA_ARGS__);                                   \
-        else if (s.NC == 4) NORM_GO(KERNEL, E, V, 4, 1, 1024, __VA_ARGS__);                                       \
-        else NORM_GO(KERNEL, E, V, 16 / V, 1, 1024, __VA_ARGS__);                                                 \
+        else if (s.block == 256) NORM_GO(KERNEL, E, V, 4, 1, 256, false, __VA_ARGS__);                                   \
+        else if (s.block == 512) NORM_GO(KERNEL, E, V, 4, 1, 512, false, __VA_ARGS__);                                   \
+        else if (s.NC == 4) NORM_GO(KERNEL, E, V, 4, 1, 1024, false, __VA_ARGS__);                                       \
+        else NORM_GO(KERNEL, E, V, 16 / V, 1, 1024, false, __VA_ARGS__);                                                 \
     }
-#define NORM_GO(KERNEL, E, V, NC, R, BLOCK, ...) hipLaunchKernelGGL((KERNEL<E, V, NC, R, BLOCK>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
+#define NORM_GO(KERNEL, E, V, NC, R, BLOCK, S, ...) hipLaunchKernelGGL((KERNEL<E, V, NC, R, BLOCK, S>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
 
 extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post_gamma,
                                       const float* scale, const float* pre_gamma, void* out, void* normed, float* rstd, void* stream) {
@@ -470,7 +473,7 @@ extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* 
     if (d->rows == 0) return MV2_OK;
     if (!x || (branch && !out) || (pre_gamma && !normed)) return MV2_EINVAL;
     const int V = norm_access(d, branch, gate, {x, branch, gate, out, normed});
-    const NormShape s = norm_shape(d, V);
+    const NormShape s = norm_shape(d, V, 1 + !!branch * 2 + !!gate + !!pre_gamma);
     const NormArgs A = norm_args(d);
     // workgroups at most: 16384 x 2048 71 us with 1024, 73 with 2048; narrow accesses want more in flight: 16384 x 1001 76 us with 4096, 85 with 1024
     const unsigned grid = norm_grid(d, s, V <= 2 ? 4096 : 1024);
@@ -492,7 +495,7 @@ extern "C" int mv2_block_norm_backward(const mv2_block_norm_desc* d, const void*
     const bool cols = dpost || dscale || dpre;
     if (cols && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < mv2_block_norm_workspace_bytes(d))) return MV2_EWORKSPACE;
     const int V = norm_access(d, branch, gate, {x, branch, gate, dout, dn, dx, dbranch, dgate});
-    const NormShape s = norm_shape(d, V);
+    const NormShape s = norm_shape(d, V, !!dout + !!dn * 2 + !!branch + !!gate + !!dx + !!dbranch + !!dgate);
     const NormArgs A = norm_args(d);
     const unsigned grid = norm_grid(d, s, norm_bwd_grid(d, s));
     float* parts = cols ? (float*)workspace : nullptr;

@@ -40,7 +40,7 @@ __device__ __forceinline__ void walk_place(const LoopArgs& A, int64_t i, int64_t
     }
 }
 
-template <typename E, int V>
+template <typename E, int V, bool S>
 __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const void* __restrict__ q, const void* __restrict__ kv, const void* __restrict__ a,
                                                             const float* h0, void* __restrict__ y, float* hlast, float* __restrict__ states) {
     const int cpr = A.C / V;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
 #pragma unroll
         for (int s = 0; s < LOOP_STEPS; ++s) {
             const int64_t at = in0 + (t + s) * A.st;
-            vk[s].load(kv, at); va[s].load(a, at); vq[s].load(q, at);
+            vk[s].template load<S>(kv, at); va[s].template load<S>(a, at); vq[s].template load<S>(q, at);
         }
         if (states && t > 0) {
             float* o = states + (((int64_t)b * A.nstate + t / LOOP_STEPS - 1) * A.P + p) * A.C + c;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
                 h[k] = cut ? fk[k] : fmaf(sigm<E>(fa[k]), h[k], fk[k]);
                 fq[k] *= h[k];
             }
-            RowVec<E, V>::store(y, y0 + (t + s) * yt, fq);
+            RowVec<E, V>::template store<S>(y, y0 + (t + s) * yt, fq);
         }
     }
     if (states && t > 0 && t < n) {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
     for (; t < n; ++t) {
         RowVec<E, V> vq, vk, va;
         const int64_t at = in0 + t * A.st;
-        vk.load(kv, at); va.load(a, at); vq.load(q, at);
+        vk.template load<S>(kv, at); va.template load<S>(a, at); vq.template load<S>(q, at);
         float fq[V], fk[V], fa[V];
         vq.get(fq); vk.get(fk); va.get(fa);
         const bool cut = rs && rs[t];
@@ -101,19 +101,19 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
             h[k] = cut ? fk[k] : fmaf(sigm<E>(fa[k]), h[k], fk[k]);
             fq[k] *= h[k];
         }
-        RowVec<E, V>::store(y, y0 + t * yt, fq);
+        RowVec<E, V>::template store<S>(y, y0 + t * yt, fq);
     }
     float zero[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) zero[k] = 0.f;
-    for (; t < A.T; ++t) RowVec<E, V>::store(y, y0 + t * yt, zero);
+    for (; t < A.T; ++t) RowVec<E, V>::template store<S>(y, y0 + t * yt, zero);
     if (hlast) {
 #pragma unroll
         for (int k = 0; k < V; ++k) hlast[seq * A.C + c + k] = h[k];
     }
 }
 
-template <typename E, int V>
+template <typename E, int V, bool S>
 __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const void* __restrict__ q, const void* __restrict__ kv, const void* __restrict__ a,
                                                             const float* __restrict__ h0, const float* __restrict__ states, const void* __restrict__ dy,
                                                             const float* __restrict__ dhlast, void* __restrict__ dq, void* __restrict__ dkv,
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
     for (int k = 0; k < V; ++k) { back[k] = dhlast ? dhlast[seq * A.C + c + k] : 0.f; zero[k] = 0.f; }
     for (int t = n; t < A.T; ++t) {
         const int64_t at = g0 + t * A.gt;
-        RowVec<E, V>::store(dq, at, zero); RowVec<E, V>::store(dkv, at, zero); RowVec<E, V>::store(da, at, zero);
+        RowVec<E, V>::template store<S>(dq, at, zero); RowVec<E, V>::template store<S>(dkv, at, zero); RowVec<E, V>::template store<S>(da, at, zero);
     }
     for (int blk = (n + LOOP_STEPS - 1) / LOOP_STEPS - 1; blk >= 0; --blk) {
         const int t0 = blk * LOOP_STEPS;
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
         for (int s = 0; s < LOOP_STEPS; ++s)
             if (t0 + s < n) {
                 const int64_t at = in0 + (t0 + s) * A.st;
-                vk[s].load(kv, at); va[s].load(a, at); vq[s].load(q, at); vy[s].load(dy, y0 + (t0 + s) * yt);
+                vk[s].template load<S>(kv, at); va[s].template load<S>(a, at); vq[s].template load<S>(q, at); vy[s].template load<S>(dy, y0 + (t0 + s) * yt);
             }
         float h[LOOP_STEPS + 1][V];                 // h[s] = state before token t0 + s
         const float* hin = blk > 0 ? states + (((int64_t)b * A.nstate + blk - 1) * A.P + p) * A.C + c : (h0 ? h0 + seq * A.C + c : nullptr);
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
                     back[k] = cut ? 0.f : g * d;
                 }
                 const int64_t at = g0 + (t0 + s) * A.gt;
-                RowVec<E, V>::store(dq, at, oq); RowVec<E, V>::store(dkv, at, ok); RowVec<E, V>::store(da, at, oa);
+                RowVec<E, V>::template store<S>(dq, at, oq); RowVec<E, V>::template store<S>(dkv, at, ok); RowVec<E, V>::template store<S>(da, at, oa);
             }
     }
     if (dh0) {
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) void span_clear_kernel(u64* p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
-template <typename E, int V, int CL, int WAVES, int TW, bool CUTS>
+template <typename E, int V, int CL, int WAVES, int TW, bool CUTS, bool S>
 __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* h0, void* __restrict__ y, float* hlast,
                                                                    float* __restrict__ states) {
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
 #pragma unroll
         for (int i = 0; i < L; ++i) {                         // rows behind the last token are not read: the last one stands in for them
             const int64_t at = in0 + (int64_t)min(t0 + i, n - 1) * A.st;
-            va[i].load(a, at); vk[i].load(kv, at); vq[i].load(q, at);
+            va[i].template load<S>(a, at); vk[i].template load<S>(kv, at); vq[i].template load<S>(q, at);
         }
         if (CUTS) {
             const unsigned char* rs = A.resets + (int64_t)b * A.T;
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) fq[k] = 0.f;
-        if (cok && t0 + i < A.T) RowVec<E, V>::store(y, y0 + (t0 + i) * yt, fq);
+        if (cok && t0 + i < A.T) RowVec<E, V>::template store<S>(y, y0 + (t0 + i) * yt, fq);
     }
     if (hlast && cok && kb == W.nblk - 1 && row == ROWS - 1) {
 #pragma unroll
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
 
 // The same from the last token to the first for D.  The states in front of a block's tokens are formed again from the kept state.  Held per
 // element: m = min(g, 1 - g) with the sign of a, from which g and g (1 - g) follow without a cancellation and without another exponential.
-template <typename E, int V, int CL, int WAVES, int TW, bool CUTS>
+template <typename E, int V, int CL, int WAVES, int TW, bool CUTS, bool S>
 __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* __restrict__ h0, const float* __restrict__ states,
                                                                    const void* __restrict__ dy, const float* __restrict__ dhlast, void* __restrict__ dq,
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
             for (int i = 0; i < L; ++i) {
                 const int t = min(t0 + i, n - 1);
                 const int64_t at = in0 + (int64_t)t * A.st;
-                va[i].load(a, at); vk[i].load(kv, at); vq[i].load(q, at); vy[i].load(dy, y0 + t * yt);
+                va[i].template load<S>(a, at); vk[i].template load<S>(kv, at); vq[i].template load<S>(q, at); vy[i].template load<S>(dy, y0 + t * yt);
             }
             if (CUTS) {
                 const unsigned char* rs = A.resets + (int64_t)b * A.T;
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) fy[k] = 0.f;
-        if (cok && t0 + i < A.T) RowVec<E, V>::store(dq, g0 + (t0 + i) * A.gt, fy);
+        if (cok && t0 + i < A.T) RowVec<E, V>::template store<S>(dq, g0 + (t0 + i) * A.gt, fy);
     }
 #pragma unroll
     for (int i = L - 1; i >= 0; --i) {
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
             for (int k = 0; k < V; ++k) { back[k] = fq[k]; fq[k] = 0.f; oa[k] = 0.f; }
         if (cok && t0 + i < A.T) {
             const int64_t at = g0 + (t0 + i) * A.gt;
-            RowVec<E, V>::store(dkv, at, fq); RowVec<E, V>::store(da, at, oa);
+            RowVec<E, V>::template store<S>(dkv, at, fq); RowVec<E, V>::template store<S>(da, at, oa);
         }
     }
     if (dh0 && cok && kb == 0 && row == 0) {
@@ -670,6 +670,13 @@ static int loop_access(const mv2_gateloop_desc* d, bool backward, std::initializ
     return (int)std::max<int64_t>(1, rows_access(ps, {d->C * es, d->in_b * es, d->in_t * es, d->in_p * es, d->grad_b * g, d->grad_t * g, d->grad_p * g}) / es);
 }
 
+// past the caches: large calls whose rows are whole lines (where lines are shared by tiles, the caches bring the second half: 6 x 4095 x 1000 bf16
+// 52 us forward through them, 65 past)
+static bool loop_streams(const mv2_gateloop_desc* d, int tensors) {
+    const int64_t es = d->dtype == MV2_BF16 ? 2 : 4;
+    return d->C * es % 128 == 0 && d->in_t * es % 128 == 0 && calls_stream((double)d->B * d->T * d->P * d->C * es * tensors);
+}
+
 static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, const unsigned char* resets) {
     LoopArgs A;
     A.B = d->B; A.T = d->T; A.P = d->P; A.C = d->C;
@@ -705,23 +712,24 @@ extern "C" int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, c
     if (d->T > 0 && (!q || !kv || !a || !y)) return MV2_EINVAL;
     const LoopArgs A = loop_args(d, lengths, resets);
     const int V = loop_access(d, false, {q, kv, a, y});
+    const bool stream_past = loop_streams(d, 4);
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
         const int64_t n = (int64_t)d->B * d->P * (d->C / V);
         const dim3 grid((unsigned)((n + 255) / 256));
-#define GO(E, V) hipLaunchKernelGGL((loop_walk_fwd_kernel<E, V>), grid, dim3(256), 0, st, A, q, kv, a, h0, y, h_last, states)
-        if (d->dtype == MV2_BF16) { if (V == 8) GO(BF16, 8); else if (V == 2) GO(BF16, 2); else GO(BF16, 1); }
-        else { if (V == 4) GO(F32, 4); else GO(F32, 1); }
+#define GO(E, V, S) hipLaunchKernelGGL((loop_walk_fwd_kernel<E, V, S>), grid, dim3(256), 0, st, A, q, kv, a, h0, y, h_last, states)
+        if (d->dtype == MV2_BF16) { if (V == 8 && stream_past) GO(BF16, 8, true); else if (V == 8) GO(BF16, 8, false); else if (V == 2) GO(BF16, 2, false); else GO(BF16, 1, false); }
+        else { if (V == 4 && stream_past) GO(F32, 4, true); else if (V == 4) GO(F32, 4, false); else GO(F32, 1, false); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
         rc = span_work(d, V == 4, false, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, CL, CUTS) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
-#define GO2(E, V, CL) do { if (resets) GO(E, V, CL, true); else GO(E, V, CL, false); } while (0)
-        if (d->dtype == MV2_BF16) { if (V == 8) GO2(BF16, 8, 8); else if (V == 2) GO2(BF16, 2, 32); else GO2(BF16, 1, 64); }
-        else { if (V == 4) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
+#define GO(E, V, CL, CUTS, S) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
+#define GO2(E, V, CL, S) do { if (resets) GO(E, V, CL, true, S); else GO(E, V, CL, false, S); } while (0)
+        if (d->dtype == MV2_BF16) { if (V == 8 && stream_past) GO2(BF16, 8, 8, true); else if (V == 8) GO2(BF16, 8, 8, false); else if (V == 2) GO2(BF16, 2, 32, false); else GO2(BF16, 1, 64, false); }
+        else { if (V == 4 && stream_past) GO2(F32, 4, 8, true); else if (V == 4) GO2(F32, 4, 8, false); else GO2(F32, 1, 64, false); }
 #undef GO2
 #undef GO
     }
@@ -738,24 +746,25 @@ extern "C" int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, 
     const LoopArgs A = loop_args(d, lengths, resets);
     if (A.nstate > 0 && !states) return MV2_EINVAL;
     const int V = loop_access(d, true, {q, kv, a, dy, dq, dkv, da});
+    const bool stream_past = loop_streams(d, 7);
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
         const int64_t n = (int64_t)d->B * d->P * (d->C / (V > 2 ? V / 2 : V));
         const dim3 grid((unsigned)((n + 255) / 256));
-#define GO(E, V) hipLaunchKernelGGL((loop_walk_bwd_kernel<E, V>), grid, dim3(256), 0, st, A, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-        if (d->dtype == MV2_BF16) { if (V == 8) GO(BF16, 4); else if (V == 2) GO(BF16, 2); else GO(BF16, 1); }
-        else { if (V == 4) GO(F32, 2); else GO(F32, 1); }
+#define GO(E, V, S) hipLaunchKernelGGL((loop_walk_bwd_kernel<E, V, S>), grid, dim3(256), 0, st, A, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
+        if (d->dtype == MV2_BF16) { if (V == 8) GO(BF16, 4, false); else if (V == 2) GO(BF16, 2, false); else GO(BF16, 1, false); }
+        else { if (V == 4) GO(F32, 2, false); else GO(F32, 1, false); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
         rc = span_work(d, V == 4, true, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, CL, CUTS)                                                                                                                                    \
-    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-#define GO2(E, V, CL) do { if (resets) GO(E, V, CL, true); else GO(E, V, CL, false); } while (0)
-        if (d->dtype == MV2_BF16) { if (V == 8) GO2(BF16, 8, 8); else if (V == 2) GO2(BF16, 2, 32); else GO2(BF16, 1, 64); }
-        else { if (V == 4) GO2(F32, 4, 8); else GO2(F32, 1, 64); }
+#define GO(E, V, CL, CUTS, S)                                                                                                                                 \
+    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
+#define GO2(E, V, CL, S) do { if (resets) GO(E, V, CL, true, S); else GO(E, V, CL, false, S); } while (0)
+        if (d->dtype == MV2_BF16) { if (V == 8 && stream_past) GO2(BF16, 8, 8, true); else if (V == 8) GO2(BF16, 8, 8, false); else if (V == 2) GO2(BF16, 2, 32, false); else GO2(BF16, 1, 64, false); }
+        else { if (V == 4 && stream_past) GO2(F32, 4, 8, true); else if (V == 4) GO2(F32, 4, 8, false); else GO2(F32, 1, 64, false); }
 #undef GO2
 #undef GO
     }

@@ -71,6 +71,15 @@ def _dense(t):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _once(backward):
+    """first-order gradients: torch's guard where a graph of the gradients is asked for, without its cost where it is not"""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 # ----------------------------------------------------------------------------------------------------------------- gated recurrence
 class _LoopPlan:
     """what follows from the arguments' shapes, strides and types"""
@@ -141,7 +150,7 @@ class _GateLoop(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dh):
         state, lengths, resets, states, *qkva = ctx.saved_tensors
         if dy is None and dh is None:
@@ -232,7 +241,7 @@ def _plan_step(qkva, state, state_out):
 
 # ----------------------------------------------------------------------------------------------------------------- norms around a block
 class _NormPlan:
-    __slots__ = ('ops', 'desc', 'copy', 'cast', 'shape', 'rows', 'branch', 'normed', 'keeps', 'ws_backward')
+    __slots__ = ('ops', 'desc', 'copy', 'cast', 'shape', 'rows', 'branch', 'normed', 'keeps', 'cols', 'ws_backward')
 
 
 def _row_stride(shape, stride):
@@ -271,7 +280,7 @@ def _plan_norm(x, branch, gate, gate_act, *params):
     plan.copy = any(t is not None and s is None for t, s in zip((x, branch, gate), steps))
     if plan.copy:
         steps = [C, C, C]
-    plan.shape, plan.rows = tuple(x.shape), x.numel() // C
+    plan.shape, plan.rows, plan.cols = tuple(x.shape), x.numel() // C, (C,)
     plan.branch, plan.normed, plan.keeps = branch is not None, pre is not None, post is not None or pre is not None
     plan.desc = BlockNormDesc(dtype=dtype, C=C, rows=plan.rows, x_stride=steps[0] or 0, branch_stride=steps[1] or 0, gate_stride=steps[2] or 0,
                               gate_act=_ACTS[gate_act] if gate is not None else 0, reserved=0)
@@ -289,7 +298,7 @@ class _BlockNorm(torch.autograd.Function):
         return out, normed
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout, dn):
         saved = ctx.saved_tensors
         if dout is None and dn is None:
@@ -300,7 +309,7 @@ class _BlockNorm(torch.autograd.Function):
         dout = None if dout is None else _dense(dout)
         dn = None if dn is None else _dense(dn)
         rows = [ops.empty(plan.shape, dtype) if n else None for n in need[1:4]]
-        cols = [ops.empty((plan.desc.C,), torch.float32) if n else None for n in need[4:7]]
+        cols = [ops.empty(plan.cols, torch.float32) if n else None for n in need[4:7]]
         ops.block_norm_backward_now(plan, saved, dout, dn, rows, cols)
         return None, *rows, *cols
 

@@ -343,10 +343,12 @@ class HipOps:
                   _ptr(pre), _ptr(out), _ptr(normed), _ptr(rstd))
 
     def block_norm_backward_now(self, plan, saved, dout, dn, rows, cols):
-        n = plan.ws_backward if any(c is not None for c in cols) else 0
+        n = 0 if cols[0] is cols[1] is cols[2] is None else plan.ws_backward
         ws = self.empty((n,), torch.uint8) if n else None
-        self._now(self.lib.mv2_block_norm_backward, 'mv2_block_norm_backward', plan.desc, *map(_ptr, saved), _ptr(dout), _ptr(dn), *map(_ptr, rows),
-                  *map(_ptr, cols), _ptr(ws), n)
+        x, branch, gate, post, scale, pre, rstd = saved
+        self._now(self.lib.mv2_block_norm_backward, 'mv2_block_norm_backward', plan.desc, x.data_ptr(), _ptr(branch), _ptr(gate), _ptr(post), _ptr(scale),
+                  _ptr(pre), _ptr(rstd), _ptr(dout), _ptr(dn), _ptr(rows[0]), _ptr(rows[1]), _ptr(rows[2]), _ptr(cols[0]), _ptr(cols[1]), _ptr(cols[2]),
+                  _ptr(ws), n)
 
     def block_norm_workspace_bytes(self, d: BlockNormDesc) -> int:
         return int(self.lib.mv2_block_norm_workspace_bytes(C.byref(d)))

@@ -529,6 +529,54 @@ def test_two_graphs_and_two_streams_at_once():
             assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
 
 
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T,P,C', [(2048, 1, 1024 + 512), (17, 2048, 256)])
+def test_gate_loop_calls_larger_than_the_caches(T, P, C, dtype):
+    """calls that move 256 MB and more go past the caches: the same numbers as sample by sample, which do not"""
+    B = 12
+    z = torch.randn(B, T, P, 3 * C, device='cuda', generator=torch.Generator('cuda').manual_seed(1)).to(dtype)
+    dy, dh = torch.randn(B, T, P, C, device='cuda').to(dtype), torch.randn(B, P, C, device='cuda')
+    one = T * P * C * z.element_size()
+    assert 4 * B * one >= 256 << 20 > 7 * one
+    resets = torch.rand(B, T, device='cuda') < 0.01
+
+    def both(i, r):
+        leaf = z[i].clone().requires_grad_()
+        y, h = F.gate_loop(leaf, resets=None if r is None else r[i], return_state=True)
+        return y.detach(), h.detach(), torch.autograd.grad((y, h), leaf, (dy[i], dh[i]))[0]
+    for r in (None, resets):
+        whole = both(slice(0, B), r)
+        for b in range(B):
+            assert all(torch.equal(w[b:b + 1], t) for w, t in zip(whole, both(slice(b, b + 1), r)))
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('R,C', [(60000, 768), (20000, 2048), (12000, 4096)])
+def test_block_norm_calls_larger_than_the_caches(R, C, dtype):
+    """rows of a large call are those of small ones; the column sums agree within the bound of their longer sums"""
+    gen = torch.Generator('cuda').manual_seed(2)
+    row = lambda: torch.randn(R, C, device='cuda', generator=gen).to(dtype)
+    x, b, g, dout, dn = (row() for _ in range(5))
+    assert x.numel() * x.element_size() * 4 >= 256 << 20
+    w = [torch.rand(C, device='cuda', generator=gen) + 0.5 for _ in range(3)]
+
+    def both(i):
+        leaves = [t[i].clone().requires_grad_() for t in (x, b, g)] + [t.clone().requires_grad_() for t in w]
+        out, n = F.block_norm(leaves[0], leaves[1], gate=leaves[2], post_gamma=leaves[3], scale=leaves[4], pre_gamma=leaves[5])
+        return [out.detach(), n.detach(), *torch.autograd.grad((out, n), leaves, (dout[i], dn[i]))]
+    whole = both(slice(0, R))
+    step = R // 8
+    parts = [both(slice(i, i + step)) for i in range(0, R, step)]
+    for k in range(5):
+        assert torch.equal(whole[k], torch.cat([p[k] for p in parts]))
+    for k in range(5, 8):
+        # each of the two sums is off by at most (additions on a value's way: R / 1000 + 800) 2^-24 of the sum of absolute values, which for terms
+        # of one size and random sign is about sqrt(R) times the sum's own size
+        got, want = whole[k].double(), sum(p[k].double() for p in parts)
+        size = want.square().mean().sqrt() * R ** 0.5
+        assert (got - want).abs().max() <= 2 * (R / 1000 + 800) * 2.0 ** -24 * size * 4
+
+
 def test_second_derivatives_are_refused():
     z = loop_inputs(1, 4, 1, 8, torch.float32).cuda().requires_grad_()
     g = torch.autograd.grad(F.gate_loop(z).square().sum(), z, create_graph=True)[0]
