@@ -577,6 +577,40 @@ def test_block_norm_calls_larger_than_the_caches(R, C, dtype):
         assert (got - want).abs().max() <= 2 * (R / 1000 + 800) * 2.0 ** -24 * size * 4
 
 
+def test_outputs_past_32_bit_offsets():
+    """more than 2^31 outputs of one call: the second half of a sequence and its gradients are those of a call that begins there"""
+    half, C, dtype = 1 << 21, 520, torch.bfloat16
+    gen = torch.Generator('cuda').manual_seed(3)
+    z = torch.empty(1, 2 * half, 3 * C, device='cuda', dtype=dtype)
+    for i in range(0, 2 * half, 1 << 18):
+        z[:, i:i + (1 << 18)].copy_(torch.randn(1, 1 << 18, 3 * C, device='cuda', generator=gen))
+    dy = torch.randn(1, half, C, device='cuda', generator=gen).to(dtype).repeat(1, 2, 1)
+    assert dy.numel() > 1 << 31
+
+    def both(z, dy, s):
+        leaf = z.requires_grad_()
+        y, h = F.gate_loop(leaf, state=s, return_state=True)
+        return y.detach(), h.detach(), torch.autograd.grad((y, h), leaf, (dy, torch.ones_like(h)))[0]
+    _, mid = F.gate_loop(z[:, :half], return_state=True)
+    y, h, g = both(z, dy, None)
+    y2, h2, g2 = both(z.detach()[:, half:], dy[:, half:], mid)
+    # the spans of the two calls are joined in other groups: some units of 2^-24 apart, at most one step of the type after the store
+    near = lambda a, b: bool(((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-4).all())
+    assert near(h, h2)
+    for i in range(0, half, 1 << 18):
+        s = slice(i, i + (1 << 18))
+        assert near(y[:, half:][:, s], y2[:, s]) and near(g[:, half:][:, s], g2[:, s])
+    del y, y2, g, g2, z
+    R, C = (1 << 21) + 5, 1032
+    x = torch.empty(R, C, device='cuda', dtype=dtype)
+    for i in range(0, R, 1 << 18):
+        x[i:i + (1 << 18)].copy_(torch.randn(min(1 << 18, R - i), C, device='cuda', generator=gen))
+    w = torch.ones(C, device='cuda')
+    out, n = F.block_norm(x, x, gate=x, post_gamma=w, pre_gamma=w)
+    o2, n2 = F.block_norm(x[-100:], x[-100:], gate=x[-100:], post_gamma=w, pre_gamma=w)
+    assert torch.equal(out[-100:], o2) and torch.equal(n[-100:], n2)
+
+
 def test_second_derivatives_are_refused():
     z = loop_inputs(1, 4, 1, 8, torch.float32).cuda().requires_grad_()
     g = torch.autograd.grad(F.gate_loop(z).square().sum(), z, create_graph=True)[0]
