@@ -72,28 +72,37 @@ __device__ __forceinline__ float inv_norm(float ss) {
 // read again with every row 136)
 template <int NC, int V> struct Params {
     float r[NC][V];
-    __device__ __forceinline__ Params(const float* w, float f, int l, int G, int nch) {
+    __device__ __forceinline__ Params(const float* w, float f, int l, int G, int C) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j)
+        for (int j = 0; j < NC; ++j) {
+            const int c = (l + j * G) * V;
 #pragma unroll
-            for (int k = 0; k < V; ++k) r[j][k] = w && l + j * G < nch ? f * w[(l + j * G) * V + k] : 1.f;
+            for (int k = 0; k < V; ++k) r[j][k] = 1.f;
+            if (w && c + V <= C) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) r[j][k] = f * w[c + k];
+            } else if (w) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) if (c + k < C) r[j][k] = f * w[c + k];
+            }
+        }
     }
 };
 
-template <typename E, int V, int NC, int R, int BLOCK, bool S>
+template <typename E, int V, bool RAG, int NC, int R, int BLOCK, bool S>
 __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G, const void* x, const void* __restrict__ branch, const void* __restrict__ gate,
                                                                const float* __restrict__ w1, const float* __restrict__ sc, const float* __restrict__ w2,
                                                                void* out, void* __restrict__ normed, float* __restrict__ rstd) {
     __shared__ float red[2][R][BLOCK / 64];
     GroupSum<BLOCK, R> sum{red, 0};
     const int l = threadIdx.x & (G - 1), per = BLOCK / G;
-    const int nch = A.C / V;
-    const Params<NC, V> p1(w1, A.root, l, G, nch), ps(sc, 1.f, l, G, nch), p2(w2, A.root, l, G, nch);
+    const int nch = (A.C + V - 1) / V;
+    const Params<NC, V> p1(w1, A.root, l, G, A.C), ps(sc, 1.f, l, G, A.C), p2(w2, A.root, l, G, A.C);
     const int64_t step = (int64_t)per * R;
     for (int64_t base = blockIdx.x * step; base < A.rows; base += gridDim.x * step) {
         int64_t row[R];
         bool on[R];
-        RowVec<E, V> vx[R][NC], vb[R][NC], vg[R][NC];
+        RowVec<E, V, RAG> vx[R][NC], vb[R][NC], vg[R][NC];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             row[i] = base + i * per + threadIdx.x / G;
@@ -102,12 +111,19 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
             for (int j = 0; j < NC; ++j) {
                 const int ch = l + j * G;
                 if (on[i] && ch < nch) {
-                    vx[i][j].template load<S>(x, row[i] * A.xs + ch * V);
-                    if (branch) vb[i][j].template load<S>(branch, row[i] * A.bs + ch * V);
-                    if (gate) vg[i][j].template load<S>(gate, row[i] * A.gs + ch * V);
+                    vx[i][j].template load<S>(x, row[i] * A.xs + ch * V, min(V, A.C - ch * V));
+                    if (branch) vb[i][j].template load<S>(branch, row[i] * A.bs + ch * V, min(V, A.C - ch * V));
+                    if (gate) vg[i][j].template load<S>(gate, row[i] * A.gs + ch * V, min(V, A.C - ch * V));
                 } else { vx[i][j].clear(); vb[i][j].clear(); vg[i][j].clear(); }
             }
         }
+        if (RAG)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                const int ch = l + j * G, nv = ch < nch ? min(V, A.C - ch * V) : V;
+#pragma unroll
+                for (int i = 0; i < R; ++i) { vx[i][j].settle(nv); vb[i][j].settle(nv); vg[i][j].settle(nv); }
+            }
         float r1[R], r2[R];
         if (w1) {
 #pragma unroll
@@ -147,7 +163,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
                         if (gate) u *= gate_act<E>(A.act, fg[k]);
                         o[i][j][k] = fmaf(fs[k], u, o[i][j][k]);
                     }
-                    if (on[i] && ch < nch) RowVec<E, V>::template store<S>(out, row[i] * A.C + ch * V, o[i][j]);
+                    if (on[i] && ch < nch) RowVec<E, V, RAG>::template store<S>(out, row[i] * A.C + ch * V, o[i][j], min(V, A.C - ch * V));
                 }
                 if (on[i] && ch < nch)
 #pragma unroll
@@ -169,15 +185,15 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
                 const int ch = l + j * G;
 #pragma unroll
                 for (int k = 0; k < V; ++k) o[i][j][k] *= r2[i] * f2[k];
-                if (on[i] && ch < nch) RowVec<E, V>::template store<S>(normed, row[i] * A.C + ch * V, o[i][j]);
+                if (on[i] && ch < nch) RowVec<E, V, RAG>::template store<S>(normed, row[i] * A.C + ch * V, o[i][j], min(V, A.C - ch * V));
             }
         }
     }
 }
 
 // parts: [gridDim.x][3][C] column sums of a workgroup's rows (dw1, ds, dw2), summed in workgroup order by block_norm_cols_kernel
-template <typename E, int V, int NC, int R, int BLOCK, bool S>
-__global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G, const void* __restrict__ x, const void* __restrict__ branch,
+template <typename E, int V, bool RAG, int NC, int R, int BLOCK, bool S>
+__global__ __launch_bounds__(BLOCK, NC == 1 ? 3 : 1) void block_norm_bwd_kernel(NormArgs A, int G, const void* __restrict__ x, const void* __restrict__ branch,
                                                                const void* __restrict__ gate, const float* __restrict__ w1, const float* __restrict__ sc,
                                                                const float* __restrict__ w2, const float* __restrict__ rstd, const void* __restrict__ dout,
                                                                const void* __restrict__ dn, void* __restrict__ dx, void* __restrict__ dbranch,
@@ -185,8 +201,8 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
     __shared__ float red[2][R][BLOCK / 64];
     GroupSum<BLOCK, R> sum{red, 0};
     const int l = threadIdx.x & (G - 1), per = BLOCK / G;
-    const int nch = A.C / V;
-    const Params<NC, V> p1(w1, A.root, l, G, nch), ps(sc, 1.f, l, G, nch), p2(w2, A.root, l, G, nch);
+    const int nch = (A.C + V - 1) / V;
+    const Params<NC, V> p1(w1, A.root, l, G, A.C), ps(sc, 1.f, l, G, A.C), p2(w2, A.root, l, G, A.C);
     const int64_t step = (int64_t)per * R;
     float s1[NC][V], s2[NC][V], s3[NC][V];
 #pragma unroll
@@ -196,7 +212,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
     for (int64_t base = blockIdx.x * step; base < A.rows; base += gridDim.x * step) {
         int64_t row[R];
         bool on[R];
-        RowVec<E, V> vx[R][NC], vb[R][NC], vg[R][NC], vo[R][NC], vn[R][NC];
+        RowVec<E, V, RAG> vx[R][NC], vb[R][NC], vg[R][NC], vo[R][NC], vn[R][NC];
         float r1[R], r2[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -207,15 +223,24 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
                 const int ch = l + j * G;
                 vx[i][j].clear(); vb[i][j].clear(); vg[i][j].clear(); vo[i][j].clear(); vn[i][j].clear();
                 if (on[i] && ch < nch) {
-                    if (w2 && dn) { vx[i][j].template load<S>(x, row[i] * A.xs + ch * V); vn[i][j].template load<S>(dn, row[i] * A.C + ch * V); }
-                    if (branch) vb[i][j].template load<S>(branch, row[i] * A.bs + ch * V);
-                    if (gate) vg[i][j].template load<S>(gate, row[i] * A.gs + ch * V);
-                    if (dout) vo[i][j].template load<S>(dout, row[i] * A.C + ch * V);
+                    if (w2 && dn) { vx[i][j].template load<S>(x, row[i] * A.xs + ch * V, min(V, A.C - ch * V)); vn[i][j].template load<S>(dn, row[i] * A.C + ch * V, min(V, A.C - ch * V)); }
+                    if (branch) vb[i][j].template load<S>(branch, row[i] * A.bs + ch * V, min(V, A.C - ch * V));
+                    if (gate) vg[i][j].template load<S>(gate, row[i] * A.gs + ch * V, min(V, A.C - ch * V));
+                    if (dout) vo[i][j].template load<S>(dout, row[i] * A.C + ch * V, min(V, A.C - ch * V));
                 }
             }
             r1[i] = on[i] && branch && w1 ? rstd[row[i]] : 0.f;
             r2[i] = on[i] && w2 ? rstd[A.rows + row[i]] : 0.f;
         }
+        if (RAG)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                const int ch = l + j * G, nv = ch < nch ? min(V, A.C - ch * V) : V;
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    vx[i][j].settle(nv); vb[i][j].settle(nv); vg[i][j].settle(nv); vo[i][j].settle(nv); vn[i][j].settle(nv);
+                }
+            }
         float D[R][NC][V];                             // gradient that arrives at out
         float dot[R];
 #pragma unroll
@@ -274,7 +299,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
                 vo[i][j].get(fo);
 #pragma unroll
                 for (int k = 0; k < V; ++k) D[i][j][k] += fo[k];
-                if (dx && in) RowVec<E, V>::template store<S>(dx, row[i] * A.C + ch * V, D[i][j]);
+                if (dx && in) RowVec<E, V, RAG>::template store<S>(dx, row[i] * A.C + ch * V, D[i][j], min(V, A.C - ch * V));
                 if (branch) {
                     float fb[V], fg[V], og[V];
                     vb[i][j].get(fb); vg[i][j].get(fg);
@@ -291,7 +316,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
                         D[i][j][k] = db * f1[k];
                         dot[i] = fmaf(D[i][j][k], b, dot[i]);
                     }
-                    if (dgate && in) RowVec<E, V>::template store<S>(dgate, row[i] * A.C + ch * V, og);
+                    if (dgate && in) RowVec<E, V, RAG>::template store<S>(dgate, row[i] * A.C + ch * V, og, min(V, A.C - ch * V));
                 }
             }
         }
@@ -308,7 +333,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
 #pragma unroll
                     for (int k = 0; k < V; ++k) D[i][j][k] = r1[i] * (D[i][j][k] - fb[k] * r1[i] * dot[i]);
                 }
-                if (on[i] && ch < nch) RowVec<E, V>::template store<S>(dbranch, row[i] * A.C + ch * V, D[i][j]);
+                if (on[i] && ch < nch) RowVec<E, V, RAG>::template store<S>(dbranch, row[i] * A.C + ch * V, D[i][j], min(V, A.C - ch * V));
             }
         }
     }
@@ -320,9 +345,10 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs A, int G
             const int ch = l + j * G;
             if (ch < nch)
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    o[ch * V + k] = s1[j][k] * A.root; o[A.C + ch * V + k] = s2[j][k]; o[2 * A.C + ch * V + k] = s3[j][k] * A.root;
-                }
+                for (int k = 0; k < V; ++k)
+                    if (!RAG || ch * V + k < A.C) {
+                        o[ch * V + k] = s1[j][k] * A.root; o[A.C + ch * V + k] = s2[j][k]; o[2 * A.C + ch * V + k] = s3[j][k] * A.root;
+                    }
         }
     } else if (NC == 1) {                              // several groups per workgroup (then NC is 1): their sums meet in LDS, group after group
         __shared__ float meet[NC == 1 ? 3 * V : 1][NC == 1 ? BLOCK : 1];
@@ -374,7 +400,7 @@ __global__ __launch_bounds__(512) void block_norm_cols_kernel(const float* __res
 // --------------------------------------------------------------------------- host side
 #define NORM_R 2                   // rows at a time, one chunk per thread: 16384 x 2048 bf16 73 us forward and 126 backward, one row 75 and 147, four 91 and 188
 #define NORM_GROUPS 1024           // workgroups from which on rows are taken NORM_R at a time
-#define NORM_BWD_MOST 1024         // workgroups of a backward pass at most
+#define NORM_BWD_MOST 768          // workgroups of a backward pass at most
 static int norm_check(const mv2_block_norm_desc* d) {
     if (!d || d->reserved != 0) return MV2_EINVAL;
     if (d->dtype != MV2_BF16 && d->dtype != MV2_F32) return MV2_EINVAL;
@@ -386,25 +412,24 @@ static int norm_check(const mv2_block_norm_desc* d) {
     return MV2_OK;
 }
 
-// threads per row G, chunks per thread NC, rows at a time R: the row's chunks spread over up to 256 threads first, then over registers, then over
-// 1024 threads; R > 1 once every workgroup of a full chip has that many rows
-struct NormShape { int V, NC, R, block, G; bool stream; };
-static NormShape norm_shape(const mv2_block_norm_desc* d, int V, int tensors) {
-    const int nch = d->C / V;
-    NormShape s{V, 1, 1, 256, 1, V > 2 && calls_stream((double)d->rows * d->C * tensors * (d->dtype == MV2_BF16 ? 2 : 4))};
+// threads per row G, chunks per thread NC, rows at a time R: the row's chunks spread over up to 256 threads first, then over two registers, then over
+// up to 1024 threads (and four registers); R > 1 once every workgroup of a full chip has that many rows
+struct NormShape { int access, NC, R, block, G; bool stream; };
+static NormShape norm_shape(const mv2_block_norm_desc* d, int access, int tensors) {
+    const int es = d->dtype == MV2_BF16 ? 2 : 4, V = access ? 16 / es : 1, nch = (d->C + V - 1) / V;
+    NormShape s{access, 1, 1, 256, 1, access == 2 && calls_stream((double)d->rows * d->C * tensors * es)};
     while (s.G < nch && s.G < 256) s.G *= 2;
     if (nch > 256) {
-        s.NC = nch <= 512 ? 2 : V > 2 ? (nch <= 2048 ? 2 : 4) : (nch <= 4096 ? 4 : 16 / V);
-        while (s.G * s.NC < nch || (s.NC > 4 && s.G < 1024)) s.block = s.G *= 2;
+        s.NC = nch <= 2048 ? 2 : 4;
+        while (s.G * s.NC < nch) s.block = s.G *= 2;
     }
     if (s.NC == 1 && d->rows / (s.block / s.G) >= (int64_t)NORM_R * NORM_GROUPS) s.R = NORM_R;
     return s;
 }
 
-// elements of one access: a 16-byte chunk, a pair of bf16, or one
 static int norm_access(const mv2_block_norm_desc* d, const void* branch, const void* gate, std::initializer_list<const void*> ps) {
     const int es = d->dtype == MV2_BF16 ? 2 : 4;
-    return std::max(1, rows_access(ps, {(int64_t)d->C * es, d->x_stride * es, branch ? d->branch_stride * es : 0, gate ? d->gate_stride * es : 0}) / es);
+    return rows_access(d->dtype, d->C, ps, {d->x_stride * es, branch ? d->branch_stride * es : 0, gate ? d->gate_stride * es : 0});
 }
 
 static unsigned norm_grid(const mv2_block_norm_desc* d, const NormShape& s, int64_t most) {
@@ -412,12 +437,12 @@ static unsigned norm_grid(const mv2_block_norm_desc* d, const NormShape& s, int6
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, most));
 }
 
-// Workgroups of the backward pass: each leaves 3 C partial column sums, so three turns of the loop at least (1000 x 2048 bf16: 24 us from 256
-// to 512 workgroups, 28 from 768), and no more than the chip holds at once by the registers of the shapes (162 with two rows of one 16-byte
-// chunk, 195 with one row of two; 16384 x 2048: 126 us with 768, 140 with 512).
+// Workgroups of the backward pass: each leaves 3 C partial column sums, so two turns of the loop at least (1000 x 2048 bf16 25 us, one turn 28;
+// 4097 x 501 fp32 26 us, three turns 32), and no more than the chip holds at once by the registers of the shapes (up to 168 with two rows of
+// one 16-byte chunk, 200 with one row of two; 16384 x 2048 bf16 126 us with 768, 140 with 512; 8000 x 2048 70 with 768, 77 with 1280).
 static int64_t norm_bwd_grid(const mv2_block_norm_desc* d, const NormShape& s) {
-    const int64_t most = s.block > 256 ? 256 : s.V <= 2 ? NORM_BWD_MOST : s.NC == 1 ? 768 : 512;
-    return std::min(most, std::max<int64_t>(256, d->rows / ((int64_t)s.block / s.G * s.R) / 3));
+    const int64_t most = s.block > 256 ? 256 : s.NC == 1 ? NORM_BWD_MOST : 512;
+    return std::min(most, std::max<int64_t>(256, d->rows / ((int64_t)s.block / s.G * s.R) / 2));
 }
 
 extern "C" size_t mv2_block_norm_workspace_bytes(const mv2_block_norm_desc* d) {
@@ -432,38 +457,28 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
     return A;
 }
 
-// one launch of KERNEL<E, V, NC, R, BLOCK, S> for the shape; S, past the caches: where the call is large, and always at widths beyond 512 chunks (a row of
-// a thousand and more threads: 2000 x 16384 81 us forward, 95 through the caches)
+// one launch of KERNEL<E, V, RAGGED, NC, R, BLOCK, S> for the shape; S, past the caches: where the call is large, and always at widths beyond 512 chunks
+// (a row of a thousand and more threads: 2000 x 16384 81 us forward, 95 through the caches)
 #define NORM_CASES(KERNEL, ...)                                                                                   \
     do {                                                                                                          \
-        if (d->dtype == MV2_BF16) {                                                                               \
-            if (s.V == 8) { NORM_WIDE(KERNEL, BF16, 8, __VA_ARGS__) }                                             \
-            else if (s.V == 2) NORM_ODD(KERNEL, BF16, 2, __VA_ARGS__)                                             \
-            else NORM_ODD(KERNEL, BF16, 1, __VA_ARGS__)                                                           \
-        } else {                                                                                                  \
-            if (s.V == 4) { NORM_WIDE(KERNEL, F32, 4, __VA_ARGS__) else NORM_GO(KERNEL, F32, 4, 4, 1, 1024, true, __VA_ARGS__); } \
-            else NORM_ODD(KERNEL, F32, 1, __VA_ARGS__)                                                            \
-        }                                                                                                         \
+        if (d->dtype == MV2_BF16) { NORM_ACCESS(KERNEL, BF16, 8, __VA_ARGS__) }                                   \
+        else { NORM_ACCESS(KERNEL, F32, 4, __VA_ARGS__) }                                                         \
     } while (0)
-#define NORM_SHORT(KERNEL, E, V, ...)                                                                             \
-        if (s.NC == 1 && s.R == 1) NORM_GO(KERNEL, E, V, 1, 1, 256, false, __VA_ARGS__);                          \
-        else if (s.NC == 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, false, __VA_ARGS__);                            \
-        else if (s.block == 256 && s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 256, false, __VA_ARGS__);
-#define NORM_WIDE(KERNEL, E, V, ...)                                                                              \
-        if (s.stream && s.NC == 1 && s.R > 1) NORM_GO(KERNEL, E, V, 1, NORM_R, 256, true, __VA_ARGS__);           \
-        else if (s.stream && s.NC == 2 && s.block == 256) NORM_GO(KERNEL, E, V, 2, 1, 256, true, __VA_ARGS__);    \
-        else NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                \
-        else if (s.block == 512) NORM_GO(KERNEL, E, V, 2, 1, 512, true, __VA_ARGS__);                             \
-        else if (s.NC == 2) NORM_GO(KERNEL, E, V, 2, 1, 1024, true, __VA_ARGS__);
-#define NORM_ODD(KERNEL, E, V, ...)                                                                               \
-    {                                                                                                             \
-        NORM_SHORT(KERNEL, E, V, __VA_ARGS__)                                                                     \
-        else if (s.block == 256) NORM_GO(KERNEL, E, V, 4, 1, 256, false, __VA_ARGS__);                                   \
-        else if (s.block == 512) NORM_GO(KERNEL, E, V, 4, 1, 512, false, __VA_ARGS__);                                   \
-        else if (s.NC == 4) NORM_GO(KERNEL, E, V, 4, 1, 1024, false, __VA_ARGS__);                                       \
-        else NORM_GO(KERNEL, E, V, 16 / V, 1, 1024, false, __VA_ARGS__);                                                 \
-    }
-#define NORM_GO(KERNEL, E, V, NC, R, BLOCK, S, ...) hipLaunchKernelGGL((KERNEL<E, V, NC, R, BLOCK, S>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
+#define NORM_ACCESS(KERNEL, E, V, ...)                                                                            \
+        if (s.access == 2 && s.stream && s.NC == 1 && s.R > 1) NORM_GO(KERNEL, E, V, false, 1, NORM_R, 256, true, __VA_ARGS__);         \
+        else if (s.access == 2 && s.stream && s.NC == 2 && s.block == 256) NORM_GO(KERNEL, E, V, false, 2, 1, 256, true, __VA_ARGS__);  \
+        else if (s.access == 2) { NORM_SHAPES(KERNEL, E, V, false, true, __VA_ARGS__) }                           \
+        else if (s.access == 1) { NORM_SHAPES(KERNEL, E, V, true, false, __VA_ARGS__) }                           \
+        else if (s.R == 1) NORM_GO(KERNEL, E, 1, false, 1, 1, 256, false, __VA_ARGS__);                           \
+        else NORM_GO(KERNEL, E, 1, false, 1, NORM_R, 256, false, __VA_ARGS__);
+#define NORM_SHAPES(KERNEL, E, V, RAG, S, ...)                                                                    \
+        if (s.NC == 1 && s.R == 1) NORM_GO(KERNEL, E, V, RAG, 1, 1, 256, false, __VA_ARGS__);                     \
+        else if (s.NC == 1) NORM_GO(KERNEL, E, V, RAG, 1, NORM_R, 256, false, __VA_ARGS__);                       \
+        else if (s.block == 256) NORM_GO(KERNEL, E, V, RAG, 2, 1, 256, false, __VA_ARGS__);                       \
+        else if (s.block == 512) NORM_GO(KERNEL, E, V, RAG, 2, 1, 512, S, __VA_ARGS__);                           \
+        else if (s.NC == 2) NORM_GO(KERNEL, E, V, RAG, 2, 1, 1024, S, __VA_ARGS__);                               \
+        else NORM_GO(KERNEL, E, V, RAG, V == 4 ? 4 : 2, 1, 1024, S, __VA_ARGS__);
+#define NORM_GO(KERNEL, E, V, RAG, NC, R, BLOCK, S, ...) hipLaunchKernelGGL((KERNEL<E, V, RAG, NC, R, BLOCK, S>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
 
 extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post_gamma,
                                       const float* scale, const float* pre_gamma, void* out, void* normed, float* rstd, void* stream) {
@@ -472,11 +487,10 @@ extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* 
     if (!branch && (gate || post_gamma || scale || !pre_gamma)) return MV2_EINVAL;
     if (d->rows == 0) return MV2_OK;
     if (!x || (branch && !out) || (pre_gamma && !normed)) return MV2_EINVAL;
-    const int V = norm_access(d, branch, gate, {x, branch, gate, out, normed});
-    const NormShape s = norm_shape(d, V, 1 + !!branch * 2 + !!gate + !!pre_gamma);
+    const int access = norm_access(d, branch, gate, {x, branch, gate, out, normed});
+    const NormShape s = norm_shape(d, access, 1 + !!branch * 2 + !!gate + !!pre_gamma);
     const NormArgs A = norm_args(d);
-    // workgroups at most: 16384 x 2048 71 us with 1024, 73 with 2048; narrow accesses want more in flight: 16384 x 1001 76 us with 4096, 85 with 1024
-    const unsigned grid = norm_grid(d, s, V <= 2 ? 4096 : 1024);
+        const unsigned grid = norm_grid(d, s, 1024);       // 16384 x 2048: 71 us, 73 with 2048
     hipStream_t st = (hipStream_t)stream;
     NORM_CASES(block_norm_fwd_kernel, x, branch, gate, post_gamma, scale, pre_gamma, out, normed, rstd);
     MV2_LAUNCH_CHECK();
@@ -494,8 +508,8 @@ extern "C" int mv2_block_norm_backward(const mv2_block_norm_desc* d, const void*
     if (d->rows > 0 && (!x || ((pre_gamma || post_gamma) && !rstd))) return MV2_EINVAL;
     const bool cols = dpost || dscale || dpre;
     if (cols && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < mv2_block_norm_workspace_bytes(d))) return MV2_EWORKSPACE;
-    const int V = norm_access(d, branch, gate, {x, branch, gate, dout, dn, dx, dbranch, dgate});
-    const NormShape s = norm_shape(d, V, !!dout + !!dn * 2 + !!branch + !!gate + !!dx + !!dbranch + !!dgate);
+    const int access = norm_access(d, branch, gate, {x, branch, gate, dout, dn, dx, dbranch, dgate});
+    const NormShape s = norm_shape(d, access, !!dout + !!dn * 2 + !!branch + !!gate + !!dx + !!dbranch + !!dgate);
     const NormArgs A = norm_args(d);
     const unsigned grid = norm_grid(d, s, norm_bwd_grid(d, s));
     float* parts = cols ? (float*)workspace : nullptr;

@@ -113,12 +113,12 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
     }
 }
 
-template <typename E, int V, bool S>
+template <typename E, int V, bool RAG>
 __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const void* __restrict__ q, const void* __restrict__ kv, const void* __restrict__ a,
                                                             const float* __restrict__ h0, const float* __restrict__ states, const void* __restrict__ dy,
                                                             const float* __restrict__ dhlast, void* __restrict__ dq, void* __restrict__ dkv,
                                                             void* __restrict__ da, float* __restrict__ dh0) {
-    const int cpr = A.C / V;
+    const int cpr = (A.C + V - 1) / V;
     const int64_t total = (int64_t)A.B * A.P * cpr;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
@@ -126,30 +126,33 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
     int c, b, p;
     walk_place(A, i, total, cpr, seq, c, b, p);
     c *= V;
+    const int nv = RAG ? min(V, A.C - c) : V;       // elements of the chunk
     const int n = live_tokens(A, b);
     const int64_t in0 = b * A.sb + p * A.sp + c, g0 = b * A.gb + p * A.gp + c;
     const int64_t yt = (int64_t)A.P * A.C, y0 = (int64_t)b * A.T * yt + (int64_t)p * A.C + c;
     const unsigned char* rs = A.resets ? A.resets + (int64_t)b * A.T : nullptr;
     float back[V], zero[V];                         // what h_{t+1} passes back to h_t
 #pragma unroll
-    for (int k = 0; k < V; ++k) { back[k] = dhlast ? dhlast[seq * A.C + c + k] : 0.f; zero[k] = 0.f; }
+    for (int k = 0; k < V; ++k) { back[k] = dhlast && k < nv ? dhlast[seq * A.C + c + k] : 0.f; zero[k] = 0.f; }
     for (int t = n; t < A.T; ++t) {
         const int64_t at = g0 + t * A.gt;
-        RowVec<E, V>::template store<S>(dq, at, zero); RowVec<E, V>::template store<S>(dkv, at, zero); RowVec<E, V>::template store<S>(da, at, zero);
+        RowVec<E, V, RAG>::store(dq, at, zero, nv); RowVec<E, V, RAG>::store(dkv, at, zero, nv); RowVec<E, V, RAG>::store(da, at, zero, nv);
     }
     for (int blk = (n + LOOP_STEPS - 1) / LOOP_STEPS - 1; blk >= 0; --blk) {
         const int t0 = blk * LOOP_STEPS;
-        RowVec<E, V> vq[LOOP_STEPS], vk[LOOP_STEPS], va[LOOP_STEPS], vy[LOOP_STEPS];
+        RowVec<E, V, RAG> vq[LOOP_STEPS], vk[LOOP_STEPS], va[LOOP_STEPS], vy[LOOP_STEPS];
 #pragma unroll
         for (int s = 0; s < LOOP_STEPS; ++s)
             if (t0 + s < n) {
                 const int64_t at = in0 + (t0 + s) * A.st;
-                vk[s].template load<S>(kv, at); va[s].template load<S>(a, at); vq[s].template load<S>(q, at); vy[s].template load<S>(dy, y0 + (t0 + s) * yt);
-            }
+                vk[s].load(kv, at, nv); va[s].load(a, at, nv); vq[s].load(q, at, nv); vy[s].load(dy, y0 + (t0 + s) * yt, nv);
+            } else { vk[s].clear(); va[s].clear(); vq[s].clear(); vy[s].clear(); }
+#pragma unroll
+        for (int s = 0; s < LOOP_STEPS; ++s) { vk[s].settle(nv); va[s].settle(nv); vq[s].settle(nv); vy[s].settle(nv); }
         float h[LOOP_STEPS + 1][V];                 // h[s] = state before token t0 + s
         const float* hin = blk > 0 ? states + (((int64_t)b * A.nstate + blk - 1) * A.P + p) * A.C + c : (h0 ? h0 + seq * A.C + c : nullptr);
 #pragma unroll
-        for (int k = 0; k < V; ++k) h[0][k] = hin ? hin[k] : 0.f;
+        for (int k = 0; k < V; ++k) h[0][k] = hin && k < nv ? hin[k] : 0.f;
 #pragma unroll
         for (int s = 0; s < LOOP_STEPS; ++s)
             if (t0 + s < n) {
@@ -176,12 +179,12 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
                     back[k] = cut ? 0.f : g * d;
                 }
                 const int64_t at = g0 + (t0 + s) * A.gt;
-                RowVec<E, V>::template store<S>(dq, at, oq); RowVec<E, V>::template store<S>(dkv, at, ok); RowVec<E, V>::template store<S>(da, at, oa);
+                RowVec<E, V, RAG>::store(dq, at, oq, nv); RowVec<E, V, RAG>::store(dkv, at, ok, nv); RowVec<E, V, RAG>::store(da, at, oa, nv);
             }
     }
     if (dh0) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) dh0[seq * A.C + c + k] = back[k];
+        for (int k = 0; k < V; ++k) if (k < nv) dh0[seq * A.C + c + k] = back[k];
     }
 }
 
@@ -234,7 +237,8 @@ __device__ __forceinline__ bool span_place(const SpanWork& W, int& kb, int& tile
     const unsigned x = blockIdx.x % (unsigned)W.nq;
     if (threadIdx.x == 0) drawn = __hip_atomic_fetch_add(W.ticket + 16 * x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    const unsigned lo = (unsigned)((u64)x * W.ntile / W.nq), cnt = (unsigned)((u64)(x + 1) * W.ntile / W.nq) - lo;
+    const unsigned each = (unsigned)W.ntile / (unsigned)W.nq, more = (unsigned)W.ntile % (unsigned)W.nq;      // the first `more` queues hold one tile more
+    const unsigned cnt = each + (x < more), lo = each * x + min(x, more);
     kb = (int)(drawn / cnt); tile = (int)(lo + drawn % cnt);
     return kb < W.nblk;
 }
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(256) void span_clear_kernel(u64* p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
-template <typename E, int V, int CL, int WAVES, int TW, bool CUTS, bool S>
+template <typename E, int V, bool RAG, int CL, int WAVES, int TW, bool CUTS, bool S>
 __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* h0, void* __restrict__ y, float* hlast,
                                                                    float* __restrict__ states) {
@@ -343,17 +347,19 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
     const int n = live_tokens(A, b), b0 = kb * SPAN, t0 = b0 + row * L;
     const int c = ct * NCH + cl * V;
     const bool cok = c < A.C, whole = b0 + SPAN <= n;         // whole: every token of the block exists
-    const int cc = cok ? c : 0;
+    const int cc = cok ? c : 0, nv = RAG ? min(V, A.C - cc) : V;      // elements of the chunk
 
-    RowVec<E, V> vq[L], vk[L], va[L];
+    RowVec<E, V, RAG> vq[L], vk[L], va[L];
     unsigned cuts = 0;
     if (b0 < n) {
         const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
 #pragma unroll
         for (int i = 0; i < L; ++i) {                         // rows behind the last token are not read: the last one stands in for them
             const int64_t at = in0 + (int64_t)min(t0 + i, n - 1) * A.st;
-            va[i].template load<S>(a, at); vk[i].template load<S>(kv, at); vq[i].template load<S>(q, at);
+            va[i].template load<S>(a, at, nv); vk[i].template load<S>(kv, at, nv); vq[i].template load<S>(q, at, nv);
         }
+#pragma unroll
+        for (int i = 0; i < L; ++i) { va[i].settle(nv); vk[i].settle(nv); vq[i].settle(nv); }
         if (CUTS) {
             const unsigned char* rs = A.resets + (int64_t)b * A.T;
 #pragma unroll
@@ -403,7 +409,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
     if (states && cok && row == 0 && kb > 0 && t0 < n) {
         float* o = states + (((int64_t)b * A.nstate + kb - 1) * A.P + p) * A.C + c;
 #pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = h[k];
+        for (int k = 0; k < V; ++k) if (k < nv) o[k] = h[k];
     }
     const int64_t yt = (int64_t)A.P * A.C, y0 = ((int64_t)b * A.T * A.P + p) * A.C + c;
 #pragma unroll
@@ -420,17 +426,17 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) fq[k] = 0.f;
-        if (cok && t0 + i < A.T) RowVec<E, V>::template store<S>(y, y0 + (t0 + i) * yt, fq);
+        if (cok && t0 + i < A.T) RowVec<E, V, RAG>::template store<S>(y, y0 + (t0 + i) * yt, fq, nv);
     }
     if (hlast && cok && kb == W.nblk - 1 && row == ROWS - 1) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) hlast[(int64_t)seq * A.C + c + k] = h[k];
+        for (int k = 0; k < V; ++k) if (k < nv) hlast[(int64_t)seq * A.C + c + k] = h[k];
     }
 }
 
 // The same from the last token to the first for D.  The states in front of a block's tokens are formed again from the kept state.  Held per
 // element: m = min(g, 1 - g) with the sign of a, from which g and g (1 - g) follow without a cancellation and without another exponential.
-template <typename E, int V, int CL, int WAVES, int TW, bool CUTS, bool S>
+template <typename E, int V, bool RAG, int CL, int WAVES, int TW, bool CUTS, bool S>
 __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* __restrict__ h0, const float* __restrict__ states,
                                                                    const void* __restrict__ dy, const float* __restrict__ dhlast, void* __restrict__ dq,
@@ -447,25 +453,27 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
     const int n = live_tokens(A, b), b0 = kb * SPAN, t0 = b0 + row * L;
     const int c = ct * NCH + cl * V;
     const bool cok = c < A.C, whole = b0 + SPAN <= n;
-    const int cc = cok ? c : 0;
+    const int cc = cok ? c : 0, nv = RAG ? min(V, A.C - cc) : V;      // elements of the chunk
     const int chn = threadIdx.x % NCH, seg = threadIdx.x / NCH, chc = ct * NCH + chn;
     const bool chok = chc < A.C;
     const int64_t yt = (int64_t)A.P * A.C, y0 = ((int64_t)b * A.T * A.P + p) * A.C + cc;
 
-    RowVec<E, V> vq[L], vk[L], vy[L];
+    RowVec<E, V, RAG> vq[L], vk[L], vy[L];
     float m[L][V];
     unsigned cuts = 0;
     float hin = 0.f;                                          // kept state in front of the block, channel chn
     {
-        RowVec<E, V> va[L];
+        RowVec<E, V, RAG> va[L];
         if (b0 < n) {
             const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 const int t = min(t0 + i, n - 1);
                 const int64_t at = in0 + (int64_t)t * A.st;
-                va[i].template load<S>(a, at); vk[i].template load<S>(kv, at); vq[i].template load<S>(q, at); vy[i].template load<S>(dy, y0 + t * yt);
+                va[i].template load<S>(a, at, nv); vk[i].template load<S>(kv, at, nv); vq[i].template load<S>(q, at, nv); vy[i].template load<S>(dy, y0 + t * yt, nv);
             }
+#pragma unroll
+            for (int i = 0; i < L; ++i) { va[i].settle(nv); vk[i].settle(nv); vq[i].settle(nv); vy[i].settle(nv); }
             if (CUTS) {
                 const unsigned char* rs = A.resets + (int64_t)b * A.T;
 #pragma unroll
@@ -570,7 +578,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
         if (!whole && t0 + i >= n)
 #pragma unroll
             for (int k = 0; k < V; ++k) fy[k] = 0.f;
-        if (cok && t0 + i < A.T) RowVec<E, V>::template store<S>(dq, g0 + (t0 + i) * A.gt, fy);
+        if (cok && t0 + i < A.T) RowVec<E, V, RAG>::template store<S>(dq, g0 + (t0 + i) * A.gt, fy, nv);
     }
 #pragma unroll
     for (int i = L - 1; i >= 0; --i) {
@@ -594,12 +602,12 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, S
             for (int k = 0; k < V; ++k) { back[k] = fq[k]; fq[k] = 0.f; oa[k] = 0.f; }
         if (cok && t0 + i < A.T) {
             const int64_t at = g0 + (t0 + i) * A.gt;
-            RowVec<E, V>::template store<S>(dkv, at, fq); RowVec<E, V>::template store<S>(da, at, oa);
+            RowVec<E, V, RAG>::template store<S>(dkv, at, fq, nv); RowVec<E, V, RAG>::template store<S>(da, at, oa, nv);
         }
     }
     if (dh0 && cok && kb == 0 && row == 0) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) dh0[(int64_t)seq * A.C + c + k] = back[k];
+        for (int k = 0; k < V; ++k) if (k < nv) dh0[(int64_t)seq * A.C + c + k] = back[k];
     }
 }
 
@@ -664,10 +672,9 @@ extern "C" size_t mv2_gateloop_workspace_bytes(const mv2_gateloop_desc* d, int b
     return (size_t)words * sizeof(u64);
 }
 
-// elements of one access: a 16-byte chunk, a pair of bf16, or one
 static int loop_access(const mv2_gateloop_desc* d, bool backward, std::initializer_list<const void*> ps) {
     const int64_t es = d->dtype == MV2_BF16 ? 2 : 4, g = backward ? es : 0;
-    return (int)std::max<int64_t>(1, rows_access(ps, {d->C * es, d->in_b * es, d->in_t * es, d->in_p * es, d->grad_b * g, d->grad_t * g, d->grad_p * g}) / es);
+    return rows_access(d->dtype, d->C, ps, {d->in_b * es, d->in_t * es, d->in_p * es, d->grad_b * g, d->grad_t * g, d->grad_p * g});
 }
 
 // past the caches: large calls whose rows are whole lines (where lines are shared by tiles, the caches bring the second half: 6 x 4095 x 1000 bf16
@@ -711,25 +718,26 @@ extern "C" int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, c
     if (rc != MV2_OK) return rc;
     if (d->T > 0 && (!q || !kv || !a || !y)) return MV2_EINVAL;
     const LoopArgs A = loop_args(d, lengths, resets);
-    const int V = loop_access(d, false, {q, kv, a, y});
+    const int access = loop_access(d, false, {q, kv, a, y});
     const bool stream_past = loop_streams(d, 4);
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
+        const int V = access == 2 ? (d->dtype == MV2_BF16 ? 8 : 4) : 1;      // (ragged chunks: 4 x 17 x 1024 x 251 bf16 41 us, single elements 31)
         const int64_t n = (int64_t)d->B * d->P * (d->C / V);
         const dim3 grid((unsigned)((n + 255) / 256));
 #define GO(E, V, S) hipLaunchKernelGGL((loop_walk_fwd_kernel<E, V, S>), grid, dim3(256), 0, st, A, q, kv, a, h0, y, h_last, states)
-        if (d->dtype == MV2_BF16) { if (V == 8 && stream_past) GO(BF16, 8, true); else if (V == 8) GO(BF16, 8, false); else if (V == 2) GO(BF16, 2, false); else GO(BF16, 1, false); }
-        else { if (V == 4 && stream_past) GO(F32, 4, true); else if (V == 4) GO(F32, 4, false); else GO(F32, 1, false); }
+        if (d->dtype == MV2_BF16) { if (access == 2 && stream_past) GO(BF16, 8, true); else if (access == 2) GO(BF16, 8, false); else GO(BF16, 1, false); }
+        else { if (access == 2 && stream_past) GO(F32, 4, true); else if (access == 2) GO(F32, 4, false); else GO(F32, 1, false); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
-        rc = span_work(d, V == 4, false, workspace, workspace_bytes, st, W, grid);
+        rc = span_work(d, d->dtype == MV2_F32 && access, false, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, CL, CUTS, S) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
-#define GO2(E, V, CL, S) do { if (resets) GO(E, V, CL, true, S); else GO(E, V, CL, false, S); } while (0)
-        if (d->dtype == MV2_BF16) { if (V == 8 && stream_past) GO2(BF16, 8, 8, true); else if (V == 8) GO2(BF16, 8, 8, false); else if (V == 2) GO2(BF16, 2, 32, false); else GO2(BF16, 1, 64, false); }
-        else { if (V == 4 && stream_past) GO2(F32, 4, 8, true); else if (V == 4) GO2(F32, 4, 8, false); else GO2(F32, 1, 64, false); }
+#define GO(E, V, RAG, CL, CUTS, S) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, RAG, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
+#define GO2(E, V, RAG, CL, S) do { if (resets) GO(E, V, RAG, CL, true, S); else GO(E, V, RAG, CL, false, S); } while (0)
+        if (d->dtype == MV2_BF16) { if (access == 2 && stream_past) GO2(BF16, 8, false, 8, true); else if (access == 2) GO2(BF16, 8, false, 8, false); else if (access) GO2(BF16, 8, true, 8, false); else GO2(BF16, 1, false, 64, false); }
+        else { if (access == 2 && stream_past) GO2(F32, 4, false, 8, true); else if (access == 2) GO2(F32, 4, false, 8, false); else if (access) GO2(F32, 4, true, 8, false); else GO2(F32, 1, false, 64, false); }
 #undef GO2
 #undef GO
     }
@@ -745,26 +753,27 @@ extern "C" int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, 
     if (d->T > 0 && (!q || !kv || !a || !dy || !dq || !dkv || !da)) return MV2_EINVAL;
     const LoopArgs A = loop_args(d, lengths, resets);
     if (A.nstate > 0 && !states) return MV2_EINVAL;
-    const int V = loop_access(d, true, {q, kv, a, dy, dq, dkv, da});
+    const int access = loop_access(d, true, {q, kv, a, dy, dq, dkv, da});
     const bool stream_past = loop_streams(d, 7);
     hipStream_t st = (hipStream_t)stream;
     if (loop_walks(d)) {
-        const int64_t n = (int64_t)d->B * d->P * (d->C / (V > 2 ? V / 2 : V));
+        const int V = access ? (d->dtype == MV2_BF16 ? 4 : 2) : 1;
+        const int64_t n = (int64_t)d->B * d->P * ((d->C + V - 1) / V);
         const dim3 grid((unsigned)((n + 255) / 256));
-#define GO(E, V, S) hipLaunchKernelGGL((loop_walk_bwd_kernel<E, V, S>), grid, dim3(256), 0, st, A, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-        if (d->dtype == MV2_BF16) { if (V == 8) GO(BF16, 4, false); else if (V == 2) GO(BF16, 2, false); else GO(BF16, 1, false); }
-        else { if (V == 4) GO(F32, 2, false); else GO(F32, 1, false); }
+#define GO(E, V, RAG) hipLaunchKernelGGL((loop_walk_bwd_kernel<E, V, RAG>), grid, dim3(256), 0, st, A, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
+        if (d->dtype == MV2_BF16) { if (access == 2) GO(BF16, 4, false); else if (access) GO(BF16, 4, true); else GO(BF16, 1, false); }
+        else { if (access == 2) GO(F32, 2, false); else if (access) GO(F32, 2, true); else GO(F32, 1, false); }
 #undef GO
     } else {
         SpanWork W;
         unsigned grid;
-        rc = span_work(d, V == 4, true, workspace, workspace_bytes, st, W, grid);
+        rc = span_work(d, d->dtype == MV2_F32 && access, true, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, CL, CUTS, S)                                                                                                                                 \
-    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-#define GO2(E, V, CL, S) do { if (resets) GO(E, V, CL, true, S); else GO(E, V, CL, false, S); } while (0)
-        if (d->dtype == MV2_BF16) { if (V == 8 && stream_past) GO2(BF16, 8, 8, true); else if (V == 8) GO2(BF16, 8, 8, false); else if (V == 2) GO2(BF16, 2, 32, false); else GO2(BF16, 1, 64, false); }
-        else { if (V == 4 && stream_past) GO2(F32, 4, 8, true); else if (V == 4) GO2(F32, 4, 8, false); else GO2(F32, 1, 64, false); }
+#define GO(E, V, RAG, CL, CUTS, S)                                                                                                                                 \
+    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, RAG, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
+#define GO2(E, V, RAG, CL, S) do { if (resets) GO(E, V, RAG, CL, true, S); else GO(E, V, RAG, CL, false, S); } while (0)
+        if (d->dtype == MV2_BF16) { if (access == 2 && stream_past) GO2(BF16, 8, false, 8, true); else if (access == 2) GO2(BF16, 8, false, 8, false); else if (access) GO2(BF16, 8, true, 8, false); else GO2(BF16, 1, false, 64, false); }
+        else { if (access == 2 && stream_past) GO2(F32, 4, false, 8, true); else if (access == 2) GO2(F32, 4, false, 8, false); else if (access) GO2(F32, 4, true, 8, false); else GO2(F32, 1, false, 64, false); }
 #undef GO2
 #undef GO
     }

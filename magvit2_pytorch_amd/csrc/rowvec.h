@@ -1,60 +1,98 @@
-// Row access of the kernels that serve any width and any strides: V elements of storage type E as one access - 16 bytes where the
-// rows, strides and addresses are whole 16-byte chunks (V = E::kVec; V = E::kVec / 2: 8 bytes, half a chunk, for kernels that hold many rows
-// in registers), pairs of 16-bit elements where only 4 bytes are whole (V = 2), one element otherwise (V = 1).
+// Row access of the kernels that serve any width and any strides: V elements of storage type E as one access.
+//   RowVec<E, kVec>        16-byte chunks of rows, strides and addresses that are whole such chunks
+//   RowVec<E, kVec, true>  ragged: 16-byte accesses at any element (the memory pipe takes them at the same rate: a copy of 256 MB runs at
+//                          5.7 - 6.0 TB/s whatever the offsets); a row's last chunk holds nv < V elements and is read as the row's last V
+//                          elements, moved down, with zeros behind them, and written one by one.  Rows of V elements at least.
+//   V = kVec / 2           half of either, for kernels that hold many rows in registers
+//   V = 1                  rows shorter than a chunk
+// STREAM: past the caches, for calls that move more than the last-level cache holds (calls_stream).
 #pragma once
 #include "common.h"
 
-template <typename E, int V> struct RowVec {
-    static_assert(V == E::kVec, "a 16-byte chunk or one element");
-    i32x4 v;
-    __device__ __forceinline__ void clear() { v = i32x4{0, 0, 0, 0}; }
-    __device__ __forceinline__ void infinite() { const int w = E::kBytes == 2 ? 0x7f807f80 : 0x7f800000; v = i32x4{w, w, w, w}; }
-    // STREAM: past the caches, for calls that move more than the last-level cache holds (calls_stream)
-    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i) {
-        const i32x4* q = (const i32x4*)((const typename E::T*)p + i);
-        v = STREAM ? __builtin_nontemporal_load(q) : *q;
+template <int BYTES> struct RowBits;
+template <> struct RowBits<16> { typedef i32x4 T; typedef i32x4 __attribute__((aligned(2))) Any; };
+template <> struct RowBits<8> { typedef i32x2 T; typedef i32x2 __attribute__((aligned(2))) Any; };
+
+typedef int __attribute__((aligned(2))) RowWord;
+
+// N words moved down by `bytes` (of 4 N; whole words, or half words too if HALVES), zeros behind them.  By selects: written as one wide shift this
+// becomes 64-bit shifts by a variable amount, and with the amount in a wave's last register those have given wrong results here.
+template <int N, bool HALVES, typename W> __device__ __forceinline__ W moved_down(W v, int bytes) {
+#pragma unroll
+    for (int d = 1; d < N; d *= 2) {
+        const bool by = bytes & 4 * d;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = by ? (i + d < N ? v[i + d < N ? i + d : i] : 0) : v[i];
     }
-    __device__ __forceinline__ void get(float* f) const { Chunk<E>::unpack(v, f); }
-    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) {
-        i32x4* q = (i32x4*)((typename E::T*)p + i);
-        if (STREAM) __builtin_nontemporal_store(Chunk<E>::pack(f), q);
-        else *q = Chunk<E>::pack(f);
+    if (HALVES) {
+        const bool by = bytes & 2;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = by ? (int)__builtin_amdgcn_alignbit(i + 1 < N ? v[i + 1 < N ? i + 1 : i] : 0, v[i], 16) : v[i];
     }
-};
-struct RowHalf {
-    i32x2 v;
-    __device__ __forceinline__ void clear() { v = i32x2{0, 0}; }
-    template <typename T> __device__ __forceinline__ void load_at(const void* p, int64_t i) { v = *(const i32x2*)((const T*)p + i); }
-};
-template <> struct RowVec<BF16, 4> : RowHalf {
-    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i) { load_at<unsigned short>(p, i); }
-    __device__ __forceinline__ void get(float* f) const { ld4<BF16>(&v, 0, f); }
-    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { st4<BF16>(p, i, f); }
-};
-template <> struct RowVec<F32, 2> : RowHalf {
-    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i) { load_at<float>(p, i); }
-    __device__ __forceinline__ void get(float* f) const { f[0] = __int_as_float(v[0]); f[1] = __int_as_float(v[1]); }
-    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) {
-        *(i32x2*)((float*)p + i) = i32x2{__float_as_int(f[0]), __float_as_int(f[1])};
-    }
-};
-template <> struct RowVec<BF16, 2> {
-    unsigned v;
+    return v;
+}
+
+template <typename E, int V, bool RAGGED = false> struct RowVec {
+    static constexpr int kBytes = V * E::kBytes;
+    typedef RowBits<kBytes> B;
+    typename B::T v;
     __device__ __forceinline__ void clear() { v = 0; }
-    __device__ __forceinline__ void infinite() { v = 0x7f807f80u; }
-    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i) { v = *(const unsigned*)((const unsigned short*)p + i); }
-    __device__ __forceinline__ void get(float* f) const { f[0] = __uint_as_float(v << 16); f[1] = __uint_as_float(v & 0xffff0000u); }
-    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) {
-        *(unsigned*)((unsigned short*)p + i) = (unsigned)f2bf(f[0]) | ((unsigned)f2bf(f[1]) << 16);
+    __device__ __forceinline__ void infinite() { v = E::kBytes == 2 ? 0x7f807f80 : 0x7f800000; }
+    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i, int nv = V) {
+        if (!RAGGED) {
+            const typename B::T* q = (const typename B::T*)((const typename E::T*)p + i);
+            v = STREAM ? __builtin_nontemporal_load(q) : *q;
+        } else {
+            v = *(const typename B::Any*)((const typename E::T*)p + i - (V - nv));
+        }
+    }
+    // after the loads that belong together have been asked for, before any get()
+    __device__ __forceinline__ void settle(int nv) {
+        if (RAGGED && __any(nv < V)) v = moved_down<kBytes / 4, E::kBytes == 2>(v, E::kBytes * (V - nv));
+    }
+    __device__ __forceinline__ void get(float* f) const {
+        if constexpr (kBytes == 16) Chunk<E>::unpack(v, f);
+        else if constexpr (E::kBytes == 2) ld4<BF16>(&v, 0, f);
+        else { f[0] = __int_as_float(v[0]); f[1] = __int_as_float(v[1]); }
+    }
+    static __device__ __forceinline__ typename B::T pack(const float* f) {
+        if constexpr (kBytes == 16) return Chunk<E>::pack(f);
+        else if constexpr (E::kBytes == 2) { typename B::T w; st4<BF16>(&w, 0, f); return w; }
+        else return typename B::T{__float_as_int(f[0]), __float_as_int(f[1])};
+    }
+    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f, int nv = V) {
+        if (!RAGGED) {
+            typename B::T* q = (typename B::T*)((typename E::T*)p + i);
+            if (STREAM) __builtin_nontemporal_store(pack(f), q);
+            else *q = pack(f);
+        } else if (nv == V) {
+            *(typename B::Any*)((typename E::T*)p + i) = pack(f);
+        } else {                                       // 8, 4 and 2 bytes of what there is
+            typename B::T w = pack(f);
+            char* q = (char*)((typename E::T*)p + i);
+            const int bytes = nv * E::kBytes;
+            if (kBytes == 16 && (bytes & 8)) {
+                *(typename RowBits<8>::Any*)q = i32x2{w[0], w[1]};
+                w = moved_down<kBytes / 4, false>(w, 8);
+                q += 8;
+            }
+            if (bytes & 4) {
+                *(RowWord*)q = w[0];
+                w = moved_down<kBytes / 4, false>(w, 4);
+                q += 4;
+            }
+            if (E::kBytes == 2 && (bytes & 2)) *(unsigned short*)q = (unsigned short)w[0];
+        }
     }
 };
-template <typename E> struct RowVec<E, 1> {
+template <typename E> struct RowVec<E, 1, false> {
     typename E::T v;
     __device__ __forceinline__ void clear() { v = 0; }
     __device__ __forceinline__ void infinite() { st_elem<E>(&v, 0, __uint_as_float(0x7f800000u)); }
-    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i) { v = ((const typename E::T*)p)[i]; }
+    template <bool STREAM = false> __device__ __forceinline__ void load(const void* p, int64_t i, int = 1) { v = ((const typename E::T*)p)[i]; }
+    __device__ __forceinline__ void settle(int) {}
     __device__ __forceinline__ void get(float* f) const { f[0] = ld_elem<E>(&v, 0); }
-    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { st_elem<E>(p, i, f[0]); }
+    template <bool STREAM = false> static __device__ __forceinline__ void store(void* p, int64_t i, const float* f, int = 1) { st_elem<E>(p, i, f[0]); }
 };
 
 // sigmoid(a) and its slope g (1 - g) = e / (1 + e)^2 with e = exp(-|a|): no cancellation for either sign, no overflow, NaN stays NaN.
@@ -80,12 +118,14 @@ template <typename E> __device__ __forceinline__ void sigm_slope(float a, float&
 // forward and 128 backward through the caches, 65 and 118 past them; gate loop of 8 x 2048 x 2048 59 and 114, 55 and 108.
 static inline bool calls_stream(double bytes) { return bytes >= 256.0 * 1024 * 1024; }
 
-// the widest access (16, 4 or 1 bytes) that all the addresses and all the lengths in bytes are multiples of; null pointers are
-static inline int rows_access(std::initializer_list<const void*> ps, std::initializer_list<int64_t> bytes) {
-    uintptr_t any = 0;
+// how rows of C elements are accessed: whole 16-byte chunks (2), 16 bytes at any element (1), single elements (0).  `bytes`: everything that has to
+// be whole chunks for the first.
+static inline int rows_access(int dtype, int C, std::initializer_list<const void*> ps, std::initializer_list<int64_t> bytes) {
+    const int es = dtype == MV2_BF16 ? 2 : 4;
+    uintptr_t any = (uintptr_t)C * es;
     for (const void* p : ps) any |= (uintptr_t)p;
     for (int64_t b : bytes) any |= (uintptr_t)b;
-    return any & 3 ? 1 : any & 15 ? 4 : 16;
+    return !(any & 15) ? 2 : C * es >= 16 ? 1 : 0;
 }
 
 // Sum over a group of G neighbouring lanes (a power of two up to 64), in every lane, without LDS: pairs, quads, eights and rows of 16 by DPP,
