@@ -13,11 +13,10 @@ struct LoopArgs {
     int64_t gb, gt, gp;            // dq, dkv, da
     const int32_t* lengths;
     const unsigned char* resets;
-    int nstate;                    // kept states per sequence (mv2_gateloop_states)
+    int nstate, keep;              // kept states per sequence (mv2_gateloop_states), tokens between them
 };
 
 #define LOOP_STEPS 8               // tokens between two kept states of the walking kernels
-#define SPAN_KEEP 256              // and of the spans: tokens of a workgroup
 
 __device__ __forceinline__ int live_tokens(const LoopArgs& A, int b) {
     if (!A.lengths) return A.T;
@@ -337,7 +336,6 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
                                                                    const void* __restrict__ a, const float* h0, void* __restrict__ y, float* hlast,
                                                                    float* __restrict__ states) {
     constexpr int TL = 64 / CL, L = TW / TL, NCH = CL * V, SPAN = WAVES * TW, ROWS = WAVES * TL, SEGS = WAVES * 64 / NCH;
-    static_assert(SPAN == SPAN_KEEP, "a block begins at a kept state");
     __shared__ __attribute__((aligned(16))) float rowA[ROWS][NCH], rowH[ROWS][NCH];
     __shared__ float partA[SEGS][NCH], partH[SEGS][NCH], prevA[SEGS][NCH], prevH[SEGS][NCH];
     int kb, tile;
@@ -406,8 +404,8 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
     float h[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) h[k] = rowH[row][cl * V + k];
-    if (states && cok && row == 0 && kb > 0 && t0 < n) {
-        float* o = states + (((int64_t)b * A.nstate + kb - 1) * A.P + p) * A.C + c;
+    if (states && cok && t0 > 0 && t0 < n && (t0 & (A.keep - 1)) == 0) {      // a block of the backward pass begins here
+        float* o = states + (((int64_t)b * A.nstate + t0 / A.keep - 1) * A.P + p) * A.C + c;
 #pragma unroll
         for (int k = 0; k < V; ++k) if (k < nv) o[k] = h[k];
     }
@@ -437,12 +435,11 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
 // The same from the last token to the first for D.  The states in front of a block's tokens are formed again from the kept state.  Held per
 // element: m = min(g, 1 - g) with the sign of a, from which g and g (1 - g) follow without a cancellation and without another exponential.
 template <typename E, int V, bool RAG, int CL, int WAVES, int TW, bool CUTS, bool S>
-__global__ __launch_bounds__(WAVES * 64) void loop_span_bwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
+__global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A, SpanWork W, const void* __restrict__ q, const void* __restrict__ kv,
                                                                    const void* __restrict__ a, const float* __restrict__ h0, const float* __restrict__ states,
                                                                    const void* __restrict__ dy, const float* __restrict__ dhlast, void* __restrict__ dq,
                                                                    void* __restrict__ dkv, void* __restrict__ da, float* __restrict__ dh0) {
     constexpr int TL = 64 / CL, L = TW / TL, NCH = CL * V, SPAN = WAVES * TW, ROWS = WAVES * TL, SEGS = WAVES * 64 / NCH, RPS = ROWS / SEGS;
-    static_assert(SPAN == SPAN_KEEP, "a block begins at a kept state");
     __shared__ __attribute__((aligned(16))) float rowA[ROWS][NCH], rowH[ROWS][NCH], rowU[ROWS][NCH];
     __shared__ float partA[SEGS][NCH], partH[SEGS][NCH], prevA[SEGS][NCH], prevH[SEGS][NCH];
     int back_kb, tile;
@@ -641,16 +638,26 @@ static bool loop_walks(const mv2_gateloop_desc* d) {
     return d->T <= 8 + chunks / 512;
 }
 
+// Spans are of SPAN_WAVES waves of 32 tokens forward, and backward of 16 tokens where that lets two workgroups live on a CU by their registers
+// (128 against 216 in bf16: 8 x 2048 x 2048 99 us, 112 with 32 tokens, 1 x 131072 x 512 188 and 199; fp32 fits with 32: 3 x 1023 x 776 19 us, 20
+// with 16) and for rows shorter than a chunk.
+#define SPAN_WAVES 8
+static int span_tokens(const mv2_gateloop_desc* d, bool backward) {
+    return SPAN_WAVES * (!backward || (d->dtype == MV2_F32 && d->C >= 4) ? 32 : 16);
+}
+static int loop_keep(const mv2_gateloop_desc* d) { return loop_walks(d) ? LOOP_STEPS : span_tokens(d, true); }
+
 extern "C" int64_t mv2_gateloop_states(const mv2_gateloop_desc* d) {
     const int rc = loop_check(d);
     if (rc != MV2_OK) return rc;
-    return d->T > 0 ? (d->T - 1) / (loop_walks(d) ? LOOP_STEPS : SPAN_KEEP) : 0;
+    return d->T > 0 ? (d->T - 1) / loop_keep(d) : 0;
 }
 
 struct SpanShape { int64_t nblk, ctiles, ntile, nq, words; };
 static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, bool backward) {
     SpanShape s;
-    s.nblk = (d->T + SPAN_KEEP - 1) / SPAN_KEEP;
+    const int span = span_tokens(d, backward);
+    s.nblk = (d->T + span - 1) / span;
     s.ctiles = (d->C + nch - 1) / nch;
     s.ntile = s.ctiles * d->B * d->P;
     // queues per XCD, forward: 4 x 8192 x 768 bf16 48 us against 50 from one queue, rows that are not whole lines 6 x 4095 x 1000 52 against 59;
@@ -660,8 +667,6 @@ static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, bool backward) 
     s.words = s.nblk > 1 ? 64 + (s.nblk + (s.nblk + LOOP_GROUP - 1) / LOOP_GROUP) * s.ntile * nch : 0;
     return s;
 }
-#define SPAN_WAVES 8               // waves of a workgroup and tokens of a wave
-#define SPAN_TW 32
 // channels of a workgroup: 128-byte pieces of rows (64 bf16 or, in chunks of four, 32 fp32), 64 single elements of rows that are not whole chunks
 static int span_channels(bool fours) { return fours ? 32 : 64; }
 
@@ -689,7 +694,7 @@ static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, co
     A.B = d->B; A.T = d->T; A.P = d->P; A.C = d->C;
     A.sb = d->in_b; A.st = d->in_t; A.sp = d->in_p; A.gb = d->grad_b; A.gt = d->grad_t; A.gp = d->grad_p;
     A.lengths = lengths; A.resets = resets;
-    A.nstate = (int)mv2_gateloop_states(d);
+    A.nstate = (int)mv2_gateloop_states(d); A.keep = loop_keep(d);
     return A;
 }
 
@@ -734,7 +739,7 @@ extern "C" int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, c
         unsigned grid;
         rc = span_work(d, d->dtype == MV2_F32 && access, false, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, RAG, CL, CUTS, S) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, RAG, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
+#define GO(E, V, RAG, CL, CUTS, S) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, RAG, CL, SPAN_WAVES, 32, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)
 #define GO2(E, V, RAG, CL, S) do { if (resets) GO(E, V, RAG, CL, true, S); else GO(E, V, RAG, CL, false, S); } while (0)
         if (d->dtype == MV2_BF16) { if (access == 2 && stream_past) GO2(BF16, 8, false, 8, true); else if (access == 2) GO2(BF16, 8, false, 8, false); else if (access) GO2(BF16, 8, true, 8, false); else GO2(BF16, 1, false, 64, false); }
         else { if (access == 2 && stream_past) GO2(F32, 4, false, 8, true); else if (access == 2) GO2(F32, 4, false, 8, false); else if (access) GO2(F32, 4, true, 8, false); else GO2(F32, 1, false, 64, false); }
@@ -769,11 +774,11 @@ extern "C" int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, 
         unsigned grid;
         rc = span_work(d, d->dtype == MV2_F32 && access, true, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
-#define GO(E, V, RAG, CL, CUTS, S)                                                                                                                                 \
-    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, RAG, CL, SPAN_WAVES, SPAN_TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
-#define GO2(E, V, RAG, CL, S) do { if (resets) GO(E, V, RAG, CL, true, S); else GO(E, V, RAG, CL, false, S); } while (0)
-        if (d->dtype == MV2_BF16) { if (access == 2 && stream_past) GO2(BF16, 8, false, 8, true); else if (access == 2) GO2(BF16, 8, false, 8, false); else if (access) GO2(BF16, 8, true, 8, false); else GO2(BF16, 1, false, 64, false); }
-        else { if (access == 2 && stream_past) GO2(F32, 4, false, 8, true); else if (access == 2) GO2(F32, 4, false, 8, false); else if (access) GO2(F32, 4, true, 8, false); else GO2(F32, 1, false, 64, false); }
+#define GO(E, V, RAG, CL, TW, CUTS, S)                                                                                                                                 \
+    hipLaunchKernelGGL((loop_span_bwd_kernel<E, V, RAG, CL, SPAN_WAVES, TW, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, states, dy, dh_last, dq, dkv, da, dh0)
+#define GO2(E, V, RAG, CL, TW, S) do { if (resets) GO(E, V, RAG, CL, TW, true, S); else GO(E, V, RAG, CL, TW, false, S); } while (0)
+        if (d->dtype == MV2_BF16) { if (access == 2 && stream_past) GO2(BF16, 8, false, 8, 16, true); else if (access == 2) GO2(BF16, 8, false, 8, 16, false); else if (access) GO2(BF16, 8, true, 8, 16, false); else GO2(BF16, 1, false, 64, 16, false); }
+        else { if (access == 2 && stream_past) GO2(F32, 4, false, 8, 32, true); else if (access == 2) GO2(F32, 4, false, 8, 32, false); else if (access) GO2(F32, 4, true, 8, 32, false); else GO2(F32, 1, false, 64, 16, false); }
 #undef GO2
 #undef GO
     }
