@@ -395,8 +395,10 @@ int mv2_gateloop_scan(int dtype, const void* qkva, const void* residual, void* o
  * h0 itself; otherwise outputs overlap neither inputs nor each other.  Storage is `dtype`; states, decays and sums are fp32.
  * The backward pass starts from kept states: the forward call writes them to `states` if it is given (fp32,
  * B * mv2_gateloop_states(d) * P * C floats).  dq / dkv / da are all written; dh_last and dh0 are optional.
- * Any C and any strides are served; where C and the strides are whole 16-byte chunks and the pointers 16-byte aligned, rows are moved
- * in such chunks. */
+ * Any C and any strides are served (rows that are whole, aligned 16-byte chunks fastest); T = 0 gives h_last = h0.
+ * workspace: mv2_gateloop_workspace_bytes(d, backward) bytes, 8-byte aligned, contents irrelevant (the call clears what it uses with a
+ * kernel of its own); calls that run at the same time, and captured graphs that are replayed at the same time, need one each.
+ * Sums are joined in a fixed order: results are bitwise reproducible. */
 typedef struct mv2_gateloop_desc {
     int32_t dtype;
     int32_t B, T, P, C;
@@ -426,7 +428,8 @@ int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, const void*
  * rstd (optional output of the forward call, input of the backward call): fp32 (2, rows): 1 / max(|branch|, 1e-12) with post_gamma,
  * 1 / max(|out|, 1e-12) with pre_gamma; the row of a norm that is not taken is left as it is.
  * Backward: dout (gradient of out) and dn (of normed) may be NULL (zero); dx, dbranch, dgate (dense rows, dtype) and dpost, dscale, dpre (fp32 C)
- * are each optional.  The column sums are taken in a fixed order: results are bitwise reproducible. */
+ * are each optional.  The column sums are taken in a fixed order: results are bitwise reproducible.  workspace:
+ * mv2_block_norm_workspace_bytes(d) bytes where one of dpost, dscale, dpre is asked for (contents irrelevant, one per concurrent call). */
 enum { MV2_ACT_SIGMOID = 5 };
 typedef struct mv2_block_norm_desc {
     int32_t dtype;

@@ -7,6 +7,12 @@
 // A group of G threads (a power of two) owns a row and keeps it in registers: every tensor is read once and written once.  out is not saved:
 // the backward pass forms it again from x, branch and gate, unrounded, as the forward pass had it.  Memory-bound: a workgroup walks many
 // rows with the parameters in registers, R rows at a time so that their loads and their sums' latencies overlap.
+// Measured on one MI355X, us and TB/s of the rows read and written, kernels alone (a copy in 16-byte accesses: 5.9 TB/s):
+//     16384 x 2048 bf16, all parts   forward 63 (5.3), backward 116 (4.6) + 4 for the column sums' second kernel
+//     69632 x 256 bf16, add and norm forward 25 (5.7, part of it from the last-level cache), backward 40 (4.4)
+//     65536 x 512 bf16               forward 62 (5.4), backward 109 (4.9)        8192 x 2048 fp32  forward 60 (5.6), backward 100 (5.4)
+//     16384 x 1001 bf16, ragged      forward 41 (4.0), backward 79 (3.3)         4097 x 501 fp32   forward 14, backward 23
+// Forward it is the memory; backward also the 160 to 200 registers, which leave two or three waves on a SIMD.  32 rows take 5 us: latency.
 #include <algorithm>
 #include <initializer_list>
 #include "rowvec.h"

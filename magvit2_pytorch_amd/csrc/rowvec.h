@@ -4,7 +4,7 @@
 //                          5.7 - 6.0 TB/s whatever the offsets); a row's last chunk holds nv < V elements and is read as the row's last V
 //                          elements, moved down, with zeros behind them, and written one by one.  Rows of V elements at least.
 //   V = kVec / 2           half of either, for kernels that hold many rows in registers
-//   V = 1                  rows shorter than a chunk
+//   V = 1                  single elements: rows shorter than a chunk, and kernels whose every wave would hold a row's end
 // STREAM: past the caches, for calls that move more than the last-level cache holds (calls_stream).
 #pragma once
 #include "common.h"
