@@ -83,7 +83,7 @@ def _once(backward):
 # ----------------------------------------------------------------------------------------------------------------- gated recurrence
 class _LoopPlan:
     """what follows from the arguments' shapes, strides and types"""
-    __slots__ = ('ops', 'desc', 'fused', 'copy', 'empty', 'T', 'C', 'y_shape', 'h_shape', 'states_shape', 'ws_forward', 'ws_backward')
+    __slots__ = ('ops', 'desc', 'fused', 'copy', 'empty', 'T', 'C', 'stride', 'y_shape', 'h_shape', 'states_shape', 'ws_forward', 'ws_backward')
 
 
 def _plan_loop(name, qkva, tokens, state, lengths, resets):
@@ -122,7 +122,7 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
     if plan.empty:
         return plan
     plan.copy = (first.stride(-1) != 1 and shape[-1] > 1) or any(t.stride() != first.stride() for t in parts)
-    st = torch.empty(shape, device='meta').stride() if plan.copy else first.stride()
+    st = plan.stride = torch.empty(shape, device='meta').stride() if plan.copy else first.stride()
     row = (3 if fused else 1) * C                         # gradients: one dense (B, T, P, 3C) tensor, or three dense ones
     plan.desc = GateLoopDesc(dtype=dtype, B=B, T=T, P=P, C=C, in_b=st[0] if B > 1 else 0, in_t=st[1] if tokens and T > 1 else 0,
                              in_p=st[rank - 1] if P > 1 else 0, grad_b=T * P * row, grad_t=P * row, grad_p=row)
@@ -156,6 +156,9 @@ class _GateLoop(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * (4 + len(qkva))
         plan = ctx.plan
+        if any(t.stride() != plan.stride for t in qkva):      # hooks on saved tensors may lay them out anew
+            qkva = [t.contiguous() for t in qkva]
+            plan = _plan_loop('gate_loop', qkva[0] if plan.fused else qkva, True, state, lengths, resets)
         ops, dtype = plan.ops, qkva[0].dtype
         dy = ops.zeros(plan.y_shape, dtype) if dy is None else _dense(dy)
         dh = None if dh is None else _dense(dh)
@@ -226,6 +229,8 @@ def gate_loop_step(qkva, state, *, state_out=None):
         if plan.copy:
             parts = tuple(t.contiguous() for t in parts)
         plan.ops.gateloop_forward_now(plan, parts, state, None, None, y, state_out, None)
+        if not state_out.is_inference():                  # written behind autograd's back: what saved it must not use it any more
+            torch.autograd.graph.increment_version(state_out)
     return y
 
 
@@ -241,7 +246,7 @@ def _plan_step(qkva, state, state_out):
 
 # ----------------------------------------------------------------------------------------------------------------- norms around a block
 class _NormPlan:
-    __slots__ = ('ops', 'desc', 'copy', 'cast', 'shape', 'rows', 'branch', 'normed', 'keeps', 'cols', 'ws_backward')
+    __slots__ = ('ops', 'desc', 'copy', 'cast', 'strides', 'shape', 'rows', 'branch', 'normed', 'keeps', 'cols', 'ws_backward')
 
 
 def _row_stride(shape, stride):
@@ -280,6 +285,7 @@ def _plan_norm(x, branch, gate, gate_act, *params):
     plan.copy = any(t is not None and s is None for t, s in zip((x, branch, gate), steps))
     if plan.copy:
         steps = [C, C, C]
+    plan.strides = None if plan.copy else tuple(None if t is None else t.stride() for t in (x, branch, gate))      # None: all dense
     plan.shape, plan.rows, plan.cols = tuple(x.shape), x.numel() // C, (C,)
     plan.branch, plan.normed, plan.keeps = branch is not None, pre is not None, post is not None or pre is not None
     plan.desc = BlockNormDesc(dtype=dtype, C=C, rows=plan.rows, x_stride=steps[0] or 0, branch_stride=steps[1] or 0, gate_stride=steps[2] or 0,
@@ -290,10 +296,10 @@ def _plan_norm(x, branch, gate, gate_act, *params):
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, plan, x, branch, gate, post, scale, pre):
+    def forward(ctx, plan, act, x, branch, gate, post, scale, pre):
         out, normed, rstd = _norm_forward(plan, x, branch, gate, post, scale, pre, plan.keeps)
         ctx.save_for_backward(x, branch, gate, post, scale, pre, rstd)
-        ctx.plan = plan
+        ctx.plan, ctx.act = plan, act
         ctx.set_materialize_grads(False)
         return out, normed
 
@@ -302,16 +308,19 @@ class _BlockNorm(torch.autograd.Function):
     def backward(ctx, dout, dn):
         saved = ctx.saved_tensors
         if dout is None and dn is None:
-            return (None,) * 7
+            return (None,) * 8
         plan, need = ctx.plan, ctx.needs_input_grad
+        if any(t is not None and (not t.is_contiguous() if plan.strides is None else t.stride() != plan.strides[i]) for i, t in enumerate(saved[:3])):
+            saved = tuple(None if t is None else t.contiguous() for t in saved)      # hooks on saved tensors may lay them out anew
+            plan = _plan_norm(*saved[:3], ctx.act, *saved[3:6])
         ops = plan.ops
         dtype = saved[0].dtype
         dout = None if dout is None else _dense(dout)
         dn = None if dn is None else _dense(dn)
-        rows = [ops.empty(plan.shape, dtype) if n else None for n in need[1:4]]
-        cols = [ops.empty(plan.cols, torch.float32) if n else None for n in need[4:7]]
+        rows = [ops.empty(plan.shape, dtype) if n else None for n in need[2:5]]
+        cols = [ops.empty(plan.cols, torch.float32) if n else None for n in need[5:8]]
         ops.block_norm_backward_now(plan, saved, dout, dn, rows, cols)
-        return None, *rows, *cols
+        return None, None, *rows, *cols
 
 
 def _norm_forward(plan, x, branch, gate, post, scale, pre, keep):
@@ -345,7 +354,7 @@ def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, s
     if plan.cast:
         args = args[:3] + tuple(None if t is None else t.to(torch.float32).contiguous() for t in args[3:])
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        out, normed = _BlockNorm.apply(plan, *args)
+        out, normed = _BlockNorm.apply(plan, gate_act, *args)
     else:
         out, normed, _ = _norm_forward(plan, *args, False)
     return (out if plan.branch else x), normed

@@ -1,5 +1,6 @@
 """The sequence operators without a GPU: their autograd plumbing, layouts, padding and refusals over the kernel emulation, the references of
 tests/_sequence_ref.py against autograd and against differences, and the C ABI's refusals."""
+import contextlib
 import ctypes
 
 import pytest
@@ -173,6 +174,32 @@ def test_bf16_parameters_get_bf16_gradients(emulated):
     x, w = rnd(4, 8).requires_grad_(), torch.ones(8, dtype=torch.bfloat16, requires_grad=True)
     F.block_norm(x, pre_gamma=w)[1].sum().backward()
     assert w.grad.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize('fused', [True, False])
+def test_saved_tensors_laid_out_anew(emulated, fused):
+    """hooks on saved tensors give back copies of another layout than the views that were saved"""
+    B, T, C = 2, 5, 4
+    wide, up = rnd(T, B, 3 * C + 3).requires_grad_(), rnd(B, T, C, seed=1)
+    rows, w = rnd(6, 3 * C, seed=2).requires_grad_(), torch.ones(C, requires_grad=True)
+    grads = []
+    for hooks in (False, True):
+        ctx = torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t) if hooks else contextlib.nullcontext()
+        with ctx:
+            z = wide.transpose(0, 1)[..., 2:2 + 3 * C]
+            y = F.gate_loop(z if fused else z.split(C, -1))
+            q, kv, a = rows.split(C, -1)
+            out, n = F.block_norm(q, kv, gate=a, post_gamma=w, pre_gamma=w)
+        grads.append(torch.autograd.grad((y, out, n), (wide, rows, w), (up, torch.ones_like(out), rnd(6, C, seed=3))))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_a_step_over_a_saved_state_is_noticed(emulated):
+    q, s = rnd(2, 3, 12).requires_grad_(), torch.ones(2, 4)
+    y = F.gate_loop(q, state=s)
+    F.gate_loop_step(rnd(2, 12, seed=1), s)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
 
 
 def test_refusals(emulated):

@@ -611,6 +611,50 @@ def test_outputs_past_32_bit_offsets():
     assert torch.equal(out[-100:], o2) and torch.equal(n[-100:], n2)
 
 
+def test_empty_calls():
+    s = rnd(2, 8, seed=1).cuda().requires_grad_()
+    z = torch.zeros(2, 0, 24, device='cuda', requires_grad=True)
+    y, h = F.gate_loop(z, state=s, return_state=True)
+    g = torch.autograd.grad((y, h), (z, s), (y, torch.full_like(h, 3.)))
+    assert y.shape == (2, 0, 8) and torch.equal(h, s) and g[0].shape == z.shape and (g[1] == 3).all()
+    assert F.gate_loop(torch.zeros(0, 5, 24, device='cuda')).shape == (0, 5, 8)
+    x, w = torch.zeros(0, 8, device='cuda', requires_grad=True), torch.ones(8, device='cuda', requires_grad=True)
+    out, n = F.block_norm(x, x, pre_gamma=w)
+    gw = torch.autograd.grad((out, n), (x, w), (out, n))[1]
+    assert n.shape == (0, 8) and not gw.any()
+
+
+def test_two_host_threads():
+    """calls of two threads at the same time, each on a stream of its own"""
+    import threading
+    data = [loop_inputs(1, 6000, 1, 64, torch.bfloat16, s).squeeze(2).cuda() for s in range(2)]
+    w = torch.ones(64, device='cuda')
+
+    def work(z):
+        leaf = z.clone().requires_grad_()
+        y, h = F.gate_loop(leaf, return_state=True)
+        _, n = F.block_norm(leaf[..., :64], y, gate=leaf[..., 64:128], pre_gamma=w)
+        return [t.detach() for t in (y, h, n)] + [torch.autograd.grad((y, n), leaf, (y.detach(), n.detach()))[0]]
+    want = [work(z) for z in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = work(data[i])
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_second_derivatives_are_refused():
     z = loop_inputs(1, 4, 1, 8, torch.float32).cuda().requires_grad_()
     g = torch.autograd.grad(F.gate_loop(z).square().sum(), z, create_graph=True)[0]
