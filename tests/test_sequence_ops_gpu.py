@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from magvit2_pytorch_amd import functional as F
-from magvit2_pytorch_amd.ops_hip import GateLoopDesc, HipOps
+from magvit2_pytorch_amd.ops_hip import BlockNormDesc, GateLoopDesc, HipOps
+from oracle.ndhwc_ops import CpuOps
 from tests._sequence_ref import assert_within, block_norm_ref, gate_loop_ref
 
 pytestmark = pytest.mark.gpu
@@ -609,6 +610,42 @@ def test_outputs_past_32_bit_offsets():
     out, n = F.block_norm(x, x, gate=x, post_gamma=w, pre_gamma=w)
     o2, n2 = F.block_norm(x[-100:], x[-100:], gate=x[-100:], post_gamma=w, pre_gamma=w)
     assert torch.equal(out[-100:], o2) and torch.equal(n[-100:], n2)
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_steps_match_the_emulation(dtype):
+    """the launchers' steps (arguments frozen, launched on a stream that is passed in) against the kernel emulation: the gradients of a kept forward
+    pass and the norms.  Tolerance: one rounding of the store (2^-8, 2^-24) and 2e-5 of the largest value for sums in another order."""
+    B, T, P, C, dt = 2, 40, 3, 24, 0 if dtype == torch.bfloat16 else 1
+    z, dy = loop_inputs(B, T, P, C, dtype), rnd(B, T, P, C, seed=5, dtype=dtype)
+    h0, dh = rnd(B, P, C, seed=6), rnd(B, P, C, seed=7)
+    st = (T * P * 3 * C, P * 3 * C, 3 * C)
+    d = GateLoopDesc(dtype=dt, B=B, T=T, P=P, C=C, in_b=st[0], in_t=st[1], in_p=st[2], grad_b=st[0], grad_t=st[1], grad_p=st[2])
+    x, b, g, dout, dn = (rnd(9, C, seed=10 + i, dtype=dtype) for i in range(5))
+    w = [rnd(C, seed=20 + i, mean=1.) for i in range(3)]
+    e = BlockNormDesc(dtype=dt, C=C, rows=9, x_stride=C, branch_stride=C, gate_stride=C, gate_act=2, reserved=0)
+    res = []
+    for ops in (HipOps('cuda:0'), CpuOps()):
+        m = ops.to_device
+        n, wf, wb = ops.gateloop_sizes(d)
+        ws = ops.zeros((max(wf, wb, 1),), torch.uint8)
+        zz, y, h, states = m(z), ops.empty((B, T, P, C), dtype), ops.empty((B, P, C), torch.float32), ops.empty((B, max(n, 1), P, C), torch.float32)
+        dz, d0 = ops.empty((B, T, P, 3 * C), dtype), ops.empty((B, P, C), torch.float32)
+        rows, one, vec = (lambda: ops.empty((9, C), dtype)), (lambda: ops.empty((2, 9), torch.float32)), (lambda: ops.empty((C,), torch.float32))
+        out, nn, rstd, gr, gv = rows(), rows(), one(), [rows() for _ in range(3)], [vec() for _ in range(3)]
+        nws = ops.zeros((ops.block_norm_workspace_bytes(e),), torch.uint8)
+        par = [m(t) for t in w]
+        steps = [ops.gateloop_forward(d, *zz.split(C, -1), m(h0), None, None, y, h, states, ws),
+                 ops.gateloop_backward(d, *zz.split(C, -1), m(h0), None, None, states, m(dy), m(dh), *dz.split(C, -1), d0, ws),
+                 ops.block_norm_forward(e, m(x), m(b), m(g), *par, out, nn, rstd),
+                 ops.block_norm_backward(e, m(x), m(b), m(g), *par, rstd, m(dout), m(dn), *gr, *gv, nws)]
+        for step in steps:
+            step(ops.current_stream())
+        ops.synchronize()
+        res.append([t.double().cpu() for t in (y, h, dz, d0, out, nn, *gr, *gv)])
+    for i, (a, r) in enumerate(zip(*res)):
+        half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+        assert ((a - r).abs() <= 2 * half * r.abs() + 2e-5 * r.abs().max()).all(), i
 
 
 def test_empty_calls():
