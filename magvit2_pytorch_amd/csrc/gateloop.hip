@@ -629,15 +629,19 @@ static int loop_check(const mv2_gateloop_desc* d) {
 }
 
 // Which form runs: one thread per chunk where the tokens are few for that many channels, spans otherwise.  A function of the sizes alone (the
-// backward pass finds the states that the forward pass kept).  A walk takes 0.36 us a token (backward 0.65) until the memory is busy,
-// a span of up to 256 tokens some 5 us (8) and as much again for every 4096 (2048) chunks.  Measured, bf16, us forward / backward, walk : span:
-//     512 chunks, 8 tokens 5.7 / 7.5 : 5.2 / 7.8     16 tokens 8.9 / 12.6 : 5.2 / 7.8
-//   16384 chunks, 33 tokens 18 / 33 : 22 / 56        64 tokens 31 / 61 : 24 / 59
-//   65536 chunks, 128 tokens 107 / 236 : 125 / 303   256 tokens 212 / 473 : 228 / 484
+// backward pass finds the states that the forward pass kept), counted in the spans' tiles of 8 chunks, which rows shorter than a tile leave partly
+// empty.  A walk takes 0.35 us a token (backward 0.65) until the memory is busy, a span of up to 256 tokens some 5 us and as much again for every 512
+// (256) tiles.  Above 8192 tiles walks reach the memory's rate at any length.  Measured, bf16, us forward / backward, walk : span:
+//     64 tiles, 8 tokens 4.8 / 6.9 : 5.2 / 5.8        16 tokens 7.2 / 12 : 5.2 / 5.8
+//   2048 tiles, 40 tokens 16 / 31 : 22 / 27           48 tokens 18 / 37 : 23 / 27
+//   6144 tiles, 96 tokens 55 / 131 : 71 / 118         200 tokens 108 / 270 : 132 / 245
+//   8192 tiles, 192 tokens 136 / 285 : 156 / 320      1024 tokens 741 / 1516 : 874 / 1539
+//   4096 rows of 8 channels, 40 tokens 15 / 29 : 39 / 48, 200 tokens 58 / 142 : 48 / 120
+//  16384 rows of 5 channels, 200 tokens 44 / 161 : 445 / 589, 1000 tokens 291 / 1177 : 2092 / 2665
 static bool loop_walks(const mv2_gateloop_desc* d) {
-    const int kvec = d->dtype == MV2_BF16 ? 8 : 4;
-    const double chunks = (double)d->B * d->P * ((d->C + kvec - 1) / kvec);
-    return d->T <= 8 + chunks / 512;
+    const int nch = d->dtype == MV2_BF16 ? 64 : 32;
+    const int64_t tiles = (int64_t)d->B * d->P * ((d->C + nch - 1) / nch);
+    return tiles >= 8192 || d->T <= 8 + tiles / 64;
 }
 
 // Spans are of SPAN_WAVES waves of 32 tokens forward, and backward of 16 tokens where that lets two workgroups live on a CU by their registers

@@ -720,3 +720,15 @@ def test_step_kernels_leave_neighbours_alone():
             F.gate_loop_step(z, state)
             assert (pool[:32] == 7).all() and (pool[32 + B * C:] == 7).all()
             assert torch.equal(state, z[:, C:2 * C].float())
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('B,T,P,C', [(2, 150, 5000, 5), (1, 264, 8192, 8), (1, 264, 8191, 3), (3, 20, 256, 1), (3, 21, 256, 1)])
+def test_many_narrow_rows(dtype, B, T, P, C):
+    """rows shorter than a tile, on both sides of the counts that change the form, with states, lengths and document starts"""
+    z = loop_inputs(B, T, P, C, dtype).cuda()
+    n = torch.tensor([T, 0, T // 2][:B], dtype=torch.int32)
+    resets = torch.zeros(B, T, dtype=torch.bool)
+    resets[:, 7::13] = True
+    check_loop(z, C, state=rnd(B, P, C, seed=1), lengths=n, resets=resets)
+    check_loop(z, C)
