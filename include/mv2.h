@@ -424,7 +424,7 @@ int mv2_gateloop_backward(const mv2_gateloop_desc* d, const void* q, const void*
  *   gate == NULL: 1;  scale == NULL: 1;  pre_gamma == NULL: no second norm.
  * act: MV2_ACT_NONE (the gate itself), MV2_ACT_SILU or MV2_ACT_SIGMOID.  x, branch, gate are rows of C contiguous elements of `dtype` with
  * row strides of their own (elements, up to 2^20); every tensor the calls write is dense.  post_gamma, scale, pre_gamma: fp32 (C).  Norms and sums are
- * fp32, and normed is taken from the unrounded out.  out may be x itself (same stride).  C <= 16384.
+ * fp32 (rows whose sum of squares leaves fp32, |v| >= 1.8e19, have N = 0), and normed is taken from the unrounded out.  out may be x itself (same stride).  C <= 16384.
  * rstd (optional output of the forward call, input of the backward call): fp32 (2, rows): 1 / max(|branch|, 1e-12) with post_gamma,
  * 1 / max(|out|, 1e-12) with pre_gamma; the row of a norm that is not taken is left as it is.
  * Backward: dout (gradient of out) and dn (of normed) may be NULL (zero); dx, dbranch, dgate (dense rows, dtype) and dpost, dscale, dpre (fp32 C)

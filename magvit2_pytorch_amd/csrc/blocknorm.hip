@@ -496,7 +496,7 @@ extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* 
     const int access = norm_access(d, branch, gate, {x, branch, gate, out, normed});
     const NormShape s = norm_shape(d, access, 1 + !!branch * 2 + !!gate + !!pre_gamma);
     const NormArgs A = norm_args(d);
-        const unsigned grid = norm_grid(d, s, 1024);       // 16384 x 2048: 71 us, 73 with 2048
+    const unsigned grid = norm_grid(d, s, 1024);       // 16384 x 2048: 71 us, 73 with 2048
     hipStream_t st = (hipStream_t)stream;
     NORM_CASES(block_norm_fwd_kernel, x, branch, gate, post_gamma, scale, pre_gamma, out, normed, rstd);
     MV2_LAUNCH_CHECK();

@@ -5,7 +5,7 @@
 // Everything between the loads and the stores is fp32; only y, dq, dkv, da are rounded to the storage type (on their stores, once).
 // One or two flops a byte: the work is to read every element once (4 tensors forward, 7 backward) and to keep the chip's memory busy.  A copy of
 // 256 MB in 16-byte accesses runs at 5.9 TB/s.  Measured on one MI355X, us and TB/s of those tensors, kernels alone:
-//     walks   4 x 17 tokens x 1024 x 256 bf16       forward 26 (5.5; part of it from the last-level cache), backward 55 (4.5)
+//     walks   4 x 17 tokens x 1024 x 256 bf16       forward 25 (5.7; part of it from the last-level cache), backward 55 (4.5)
 //     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 99 - 105 (4.5 - 4.8); with document starts 60 and 108
 //             1 x 131072 x 512 bf16                 forward 103 (5.2), backward 189 (5.0)
 //             6 x 4095 x 1000 bf16, rows off lines  forward 53 (3.7), backward 94 (3.7)

@@ -341,7 +341,8 @@ def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, s
     ``x``, ``branch``, ``gate``: ``(..., C)``, one shape, bf16 or fp32, any strides (a third of a fused projection is read where it lies);
     ``post_gamma``, ``scale``, ``pre_gamma``: ``(C,)``, computed with in fp32.  ``gate_act``: 'silu', 'sigmoid' or 'none' (the gate as it is).
     Left out: ``branch`` - no add, ``out`` is ``x``; ``post_gamma`` - the branch enters as it is; ``gate``, ``scale`` - ones; ``pre_gamma`` - no second
-    norm, ``normed`` is None.  C <= 16384.  Returns ``(out, normed)``.  Gradients reach every tensor; the parameters' are bitwise reproducible."""
+    norm, ``normed`` is None.  C <= 16384.  Sums of squares are fp32: N of a row with ``|v| >= 1.8e19`` is zero.
+    Returns ``(out, normed)``.  Gradients reach every tensor; the parameters' are bitwise reproducible."""
     try:
         key = ('norm', _like(x), _like(branch), _like(gate), gate_act, _like(post_gamma), _like(scale), _like(pre_gamma))
         hash(gate_act)

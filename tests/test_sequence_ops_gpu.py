@@ -732,3 +732,26 @@ def test_many_narrow_rows(dtype, B, T, P, C):
     resets[:, 7::13] = True
     check_loop(z, C, state=rnd(B, P, C, seed=1), lengths=n, resets=resets)
     check_loop(z, C)
+
+
+@pytest.mark.parametrize('C', [5, 72, 2048])
+@pytest.mark.parametrize('dtype', DT)
+def test_rows_beyond_the_norms_range(dtype, C):
+    """rows whose sum of squares leaves fp32 have a norm of zero, as documented, and finite gradients; rows below the floor stay linear: 1e-30 / 1e-12
+    sqrt(C).  Their neighbours do not see them: bitwise what they are without them."""
+    x = rnd(7, C, dtype=dtype).cuda()
+    g = rnd(C, seed=1, mean=1.).cuda().requires_grad_()
+    n0 = F.block_norm(x, pre_gamma=g)[1]
+    x2 = x.clone()
+    x2[1], x2[4] = 1e25, 1e-30
+    leaf = x2.requires_grad_()
+    out, n = F.block_norm(torch.zeros_like(x), leaf, post_gamma=g, pre_gamma=None)[0], F.block_norm(leaf, pre_gamma=g)[1]
+    rest = [0, 2, 3, 5, 6]
+    assert torch.equal(n[rest], n0[rest]) and torch.equal(out[rest], n0[rest])
+    tiny = x2[4].double() * 1e12 * C ** 0.5 * g.double()
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    for v in (out, n):
+        assert v[1].eq(0).all()
+        assert ((v[4].double() - tiny).abs() <= (half + 8 * 2.0 ** -24) * tiny.abs()).all()
+    dx, dg = torch.autograd.grad((out, n), (leaf, g), (rnd(7, C, seed=2, dtype=dtype).cuda(),) * 2)
+    assert dx.isfinite().all() and dg.isfinite().all() and dx[1].eq(0).all()
