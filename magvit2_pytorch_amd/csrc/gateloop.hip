@@ -7,7 +7,7 @@
 // 256 MB in 16-byte accesses runs at 5.9 TB/s.  Measured on one MI355X, us and TB/s of those tensors, kernels alone:
 //     walks   4 x 17 tokens x 1024 x 256 bf16       forward 25 (5.7; part of it from the last-level cache), backward 55 (4.5)
 //     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 99 - 105 (4.5 - 4.8); with document starts 60 and 108
-//             1 x 131072 x 512 bf16                 forward 103 (5.2), backward 189 (5.0)
+//             1 x 131072 x 512 bf16                 forward 106 (5.1), backward 193 (4.9); 1 x 100000 x 64 23 and 35
 //             6 x 4095 x 1000 bf16, rows off lines  forward 53 (3.7), backward 94 (3.7)
 //             3 x 1023 x 777 fp32                   forward 13, backward 17 (9.5 MB a tensor: as much latency as bandwidth)
 // and 2.5 us for a single token of 512 channels, 4.3 us for one of 192 x 2048, where launch and load latency are all there is.
@@ -195,11 +195,15 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
 // CL lanes side by side read whole 128-byte pieces of rows.  Lane rows and blocks are joined through the pair (A, H) of a span: it takes the
 // state h in front of it to A h + H, and spans join as (A1, H1) (A2, H2) -> (A1 A2, A2 H1 + H2).  Within the workgroup the pairs meet in LDS,
 // where thread (channel, segment) takes a run of lane rows, and come back as the state in front of each lane row.
-// Between workgroups: a block publishes its pair and reads the pairs of the blocks before it in its group of LOOP_GROUP blocks, and the
-// state that the last block of the group before published: always the same pairs in the same order, so results do not depend on timing.
+// Between workgroups: a block publishes its pair and reads the pairs of the blocks before it in its group; the last block of a group publishes
+// the group's pair, and groups are joined likewise in sets, whose last block publishes the state behind the set.  A block reads at most 7 pairs,
+// 7 groups' pairs and one state, always the same in the same order, so results do not depend on timing, and states are handed on once every 64
+// blocks.  bf16, us forward / backward: 1 x 100000 x 64 23 / 35, states handed on from group to group of 16 blocks 36 / 58 (1 x 131072 x 512 108 / 193
+// and 107 / 188); groups and sets of 16 21 / 34, but every block reads twice as much: 16 x 60000 x 16 68 / 140 against 65 / 136.
 // Every wait ends: a block's place in the order is the ticket it draws when it starts, blocks wait for lower tickets only - for workgroups
-// that are running - and a pair is published before its block waits for anything.
-#define LOOP_GROUP 16
+// that are running; a block's pair is published before it waits for anything, a group's before its block waits for other groups.
+#define LOOP_GROUP 8                // blocks
+#define LOOP_SET 8                  // groups
 #define LOOP_CUT 2.f               // A of a span in which a document starts (products of decays are <= 1 or NaN): nothing passes through it
 typedef unsigned long long u64;
 
@@ -227,7 +231,7 @@ template <bool CUTS> __device__ __forceinline__ void join(float& A, float& H, fl
 struct SpanWork {
     unsigned* ticket;              // one per queue, 64 bytes apart
     u64* pairs;                    // [block][tile][channel of the tile]
-    u64* states;                   // [group][tile][channel of the tile]: the state behind a whole group
+    u64* groups;                   // [1 + group][tile][channel of the tile]: the pair of the group, or behind the last group of a set the state
     int nblk, ntile, ctiles, nq;
 };
 
@@ -246,27 +250,31 @@ __device__ __forceinline__ bool span_place(const SpanWork& W, int& kb, int& tile
 
 // State of the recurrence in front of this workgroup's block for channel ch (thread = (ch, seg), SEGS threads per channel).  kb counts blocks in
 // the direction of the recurrence, (A, H) is the whole block's pair (known to the threads of the last segment, which publish it), `first` what
-// block 0 starts from (the same threads).  All threads enter; everyone gets the state.
+// block 0 starts from (the same threads).  nearA, nearH: scratch.  All threads enter; everyone gets the state.
 template <int NCH, int SEGS, bool CUTS>
 __device__ __forceinline__ float span_carry(const SpanWork& W, int kb, int tile, int ch, int seg, bool ok, float first, float A, float H,
-                                            float (*partA)[NCH], float (*partH)[NCH]) {
-    constexpr int M = LOOP_GROUP / SEGS;
-    static_assert(SEGS * M == LOOP_GROUP, "the threads of a channel share a group evenly");
+                                            float (*nearA)[NCH], float (*nearH)[NCH]) {
+    __shared__ float farA[SEGS][NCH], farH[SEGS][NCH];
     const bool tail = seg == SEGS - 1;
+    const unsigned pitch = (unsigned)W.ntile * NCH, mine = (unsigned)tile * NCH + ch;      // words: 32 bits by the launch's limit on workgroups
     if (kb == 0) {
         if (tail) {
-            partH[0][ch] = first;
+            nearH[0][ch] = first;
             // block 0 publishes a state rather than a pair: whoever depends on it does not read `first` again, which may be overwritten by then
-            if (ok && W.nblk > 1) publish(W.pairs + (int64_t)tile * NCH + ch, LOOP_CUT, pass<CUTS>(A, H, first));
+            if (ok && W.nblk > 1) publish(W.pairs + mine, LOOP_CUT, pass<CUTS>(A, H, first));
         }
         __syncthreads();
-        return partH[0][ch];
+        return nearH[0][ch];
     }
-    if (ok && tail) publish(W.pairs + ((int64_t)kb * W.ntile + tile) * NCH + ch, A, H);
-    const int grp = kb / LOOP_GROUP, in = kb % LOOP_GROUP;
-    const int lead = grp > 0 ? 1 : 0, count = lead + in;      // the state behind the group before, then the blocks of this group
-    float a = 1.f, h = 0.f;
-    if (ok) {
+    const int grp = kb / LOOP_GROUP, in = kb % LOOP_GROUP, set = grp / LOOP_SET, gin = grp % LOOP_SET;
+    const bool last = in == LOOP_GROUP - 1;
+    if (ok && tail && !last) publish(W.pairs + ((unsigned)kb * pitch + mine), A, H);
+    // waits for the entries from .. to - 1 of those at `row` of `words`, this thread's share of them, and leaves their join in (a, h)
+    float a, h;
+    auto gather = [&](auto most, const u64* words, int row, int from, int to) {
+        constexpr int M = (decltype(most)::value + SEGS - 1) / SEGS;
+        a = 1.f; h = 0.f;
+        if (!ok) return;
         u64 w[M];
 #pragma unroll
         for (int j = 0; j < M; ++j) w[j] = 0;
@@ -276,10 +284,8 @@ __device__ __forceinline__ float span_carry(const SpanWork& W, int kb, int tile,
 #pragma unroll
             for (int j = 0; j < M; ++j) {
                 const int e = seg * M + j;
-                if (e < count && !pair_there(w[j])) {
-                    const u64* p = e < lead ? W.states + ((int64_t)(grp - 1) * W.ntile + tile) * NCH
-                                            : W.pairs + ((int64_t)(grp * LOOP_GROUP + e - lead) * W.ntile + tile) * NCH;
-                    w[j] = __hip_atomic_load(p + ch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (e >= from && e < to && !pair_there(w[j])) {
+                    w[j] = __hip_atomic_load(words + ((unsigned)(row + e) * pitch + mine), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     all = all && pair_there(w[j]);
                 }
             }
@@ -287,15 +293,32 @@ __device__ __forceinline__ float span_carry(const SpanWork& W, int kb, int tile,
         } while (!all);
 #pragma unroll
         for (int j = 0; j < M; ++j)
-            if (seg * M + j < count) join<true>(a, h, pair_A(w[j]), pair_H(w[j]));
+            if (pair_there(w[j])) join<true>(a, h, pair_A(w[j]), pair_H(w[j]));
+    };
+    const bool behind = last && kb + 1 < W.nblk && ok && tail;      // publishes what lies behind the group
+    gather(std::integral_constant<int, LOOP_GROUP>(), W.pairs, grp * LOOP_GROUP, 0, in);
+    nearA[seg][ch] = a; nearH[seg][ch] = h;
+    if (last) {
+        __syncthreads();
+        if (behind && gin < LOOP_SET - 1) {
+            a = 1.f; h = 0.f;
+            for (int s = 0; s < SEGS; ++s) join<true>(a, h, nearA[s][ch], nearH[s][ch]);
+            join<true>(a, h, A, H);
+            publish(W.groups + ((unsigned)(grp + 1) * pitch + mine), a, h);
+        }
     }
-    partA[seg][ch] = a; partH[seg][ch] = h;
+    if (grp > 0) {
+        gather(std::integral_constant<int, LOOP_SET>(), W.groups, set * LOOP_SET, set > 0 ? 0 : 1, gin + 1);
+        farA[seg][ch] = a; farH[seg][ch] = h;
+    }
     __syncthreads();
-    h = partH[0][ch];                                         // the first entry is a state: nothing in front of it counts
+    h = 0.f;                                                  // the first entry of all is a state: nothing in front of it counts
+    if (grp > 0)
 #pragma unroll
-    for (int s = 1; s < SEGS; ++s) h = pass<true>(partA[s][ch], partH[s][ch], h);
-    if (ok && tail && in == LOOP_GROUP - 1 && kb + 1 < W.nblk)
-        publish(W.states + ((int64_t)grp * W.ntile + tile) * NCH + ch, LOOP_CUT, pass<CUTS>(A, H, h));
+        for (int s = 0; s < SEGS; ++s) h = pass<true>(farA[s][ch], farH[s][ch], h);
+#pragma unroll
+    for (int s = 0; s < SEGS; ++s) h = pass<true>(nearA[s][ch], nearH[s][ch], h);
+    if (behind && gin == LOOP_SET - 1) publish(W.groups + ((unsigned)(grp + 1) * pitch + mine), LOOP_CUT, pass<CUTS>(A, H, h));
     return h;
 }
 
@@ -306,12 +329,11 @@ __device__ __forceinline__ void span_join(const SpanWork& W, int kb, int tile, b
                                           float (*partA)[NCH], float (*partH)[NCH], float (*prevA)[NCH], float (*prevH)[NCH]) {
     constexpr int RPS = ROWS / SEGS;
     const int ch = threadIdx.x % NCH, seg = threadIdx.x / NCH;
-    float ra[RPS], rh[RPS], A = 1.f, H = 0.f;
+    float A = 1.f, H = 0.f;
 #pragma unroll
     for (int j = 0; j < RPS; ++j) {
         const int r = REV ? ROWS - 1 - (seg * RPS + j) : seg * RPS + j;
-        ra[j] = rowA[r][ch]; rh[j] = rowH[r][ch];
-        join<CUTS>(A, H, ra[j], rh[j]);
+        join<CUTS>(A, H, rowA[r][ch], rowH[r][ch]);
     }
     partA[seg][ch] = A; partH[seg][ch] = H;
     __syncthreads();
@@ -323,8 +345,9 @@ __device__ __forceinline__ void span_join(const SpanWork& W, int kb, int tile, b
 #pragma unroll
     for (int j = 0; j < RPS; ++j) {
         const int r = REV ? ROWS - 1 - (seg * RPS + j) : seg * RPS + j;
+        const float pA = rowA[r][ch], pH = rowH[r][ch];       // read again: held over the wait they would be 16 registers
         rowH[r][ch] = h;
-        h = pass<CUTS>(ra[j], rh[j], h);
+        h = pass<CUTS>(pA, pH, h);
     }
     __syncthreads();
 }
@@ -670,7 +693,7 @@ static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, bool backward) 
     // backward only for those (104 us against 109; whole lines 91 against 87).  Few tiles would leave XCDs idle.
     const int64_t es = d->dtype == MV2_BF16 ? 2 : 4;
     s.nq = s.ntile >= 32 && (!backward || d->in_t * es % 128 != 0) ? 8 : 1;
-    s.words = s.nblk > 1 ? 64 + (s.nblk + (s.nblk + LOOP_GROUP - 1) / LOOP_GROUP) * s.ntile * nch : 0;
+    s.words = s.nblk > 1 ? 64 + (s.nblk + s.nblk / LOOP_GROUP + 1) * s.ntile * nch : 0;
     return s;
 }
 // channels of a workgroup: 128-byte pieces of rows (64 bf16 or, in chunks of four, 32 fp32), 64 single elements of rows that are not whole chunks
@@ -712,12 +735,12 @@ static int span_work(const mv2_gateloop_desc* d, bool fours, bool backward, void
     W.nblk = (int)s.nblk; W.ntile = (int)s.ntile; W.ctiles = (int)s.ctiles;
     W.nq = (int)s.nq;
     grid = (unsigned)(s.nblk > 1 ? s.nblk * s.nq * ((s.ntile + s.nq - 1) / s.nq) : s.ntile);
-    W.ticket = nullptr; W.pairs = W.states = nullptr;
+    W.ticket = nullptr; W.pairs = W.groups = nullptr;
     if (s.words == 0) return MV2_OK;
     if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < s.words * sizeof(u64)) return MV2_EWORKSPACE;
     W.ticket = (unsigned*)workspace;
     W.pairs = (u64*)workspace + 64;
-    W.states = W.pairs + s.nblk * s.ntile * nch;
+    W.groups = W.pairs + s.nblk * s.ntile * nch;
     hipLaunchKernelGGL(span_clear_kernel, dim3((unsigned)std::min<int64_t>((s.words + 255) / 256, 2048)), dim3(256), 0, st, (u64*)workspace, s.words);
     MV2_LAUNCH_CHECK();
     return MV2_OK;

@@ -755,3 +755,33 @@ def test_rows_beyond_the_norms_range(dtype, C):
         assert ((v[4].double() - tiny).abs() <= (half + 8 * 2.0 ** -24) * tiny.abs()).all()
     dx, dg = torch.autograd.grad((out, n), (leaf, g), (rnd(7, C, seed=2, dtype=dtype).cuda(),) * 2)
     assert dx.isfinite().all() and dg.isfinite().all() and dx[1].eq(0).all()
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', [1024, 1025, 2049, 8192, 8193, 16385, 66100])
+def test_groups_and_sets_of_spans(T, dtype):
+    """spans are joined in groups of 8 and sets of 64 (of 256 tokens forward and 128 or 256 backward): lengths around them and far beyond, with decays
+    that carry a state over thousands of tokens, a first state, a length and a document start"""
+    C = 8
+    z = loop_inputs(1, T, 1, C, dtype, T)
+    z[..., 2 * C::2] += 7
+    resets = torch.zeros(1, T, dtype=torch.bool)
+    resets[0, T * 3 // 5] = True
+    check_loop(z.cuda(), C, state=100 * rnd(1, 1, C, seed=1), lengths=torch.tensor([T - 40]), resets=resets)
+    check_loop(z.cuda(), C, state=100 * rnd(1, 1, C, seed=1))
+
+
+def test_sets_of_groups_in_many_tiles():
+    """long sequences of several tiles against the same tokens in shorter calls, the state handed on"""
+    B, T, C, cut = 3, 140000, 136, (0, 20000, 64000, 140000)
+    z = loop_inputs(B, T, 1, C, torch.float32).cuda()
+    z[..., 2 * C:] += 5
+    y, h = F.gate_loop(z, return_state=True)
+    s, parts = None, []
+    for a, b in zip(cut, cut[1:]):
+        p, s = F.gate_loop(z[:, a:b], state=s, return_state=True)
+        parts.append(p)
+    ref = torch.cat(parts, 1)
+    # decays of about 1 - e^-7: a state is off by some 20 units of 2^-24 for each of the ~1100 tokens that it holds, in either call
+    tol = 2 * 1100 * 20 * 2.0 ** -24
+    assert ((y - ref).abs() <= tol * ref.abs().amax(1, keepdim=True)).all() and ((h - s).abs() <= tol * s.abs().amax()).all()
