@@ -1,5 +1,5 @@
 """
-Builds libmv2_hip.so (the C-ABI of include/mv2.h) in-tree with hipcc for gfx950.
+Builds libmv2_hip.so (the C-ABI of include/mv2.h) in-tree with hipcc for gfx950, and _calls.so (functional.py's native calls) with g++.
 
     python -m magvit2_pytorch_amd.build [--force]
 
@@ -11,6 +11,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -29,6 +30,9 @@ HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_common.h'), 
 # packed fp32 arithmetic is switched off: some forms of v_pk_{add,mul,fma}_f32 that hipcc makes of ordinary float code have given wrong
 # results now and then on these chips (the host pass does not know the feature and says so: harmless)
 NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+# the native calls of functional.py: host code over torch's C++ interface, linked with the library
+CALLS = os.path.join(HERE, '_calls.so')
+CALLS_SRC = os.path.join(CSRC, 'calls.cpp')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result', *NO_PACKED_FP32]
 
 
@@ -80,7 +84,23 @@ def build(force=False, verbose=True, experiments=False):
             raise RuntimeError(f'link failed:\n{r.stdout}\n{r.stderr}')
         if verbose:
             print(f'[mv2 build] linked {lib}', flush=True)
+    if not experiments and (force or _stale(CALLS, [CALLS_SRC, HEADERS[-1]])):
+        _build_calls(verbose)
     return lib
+
+
+def _build_calls(verbose):
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{sysconfig.get_paths()["include"]}', f'-I{root}/include',
+           f'-I{os.environ.get("ROCM_PATH", "/opt/rocm")}/include', CALLS_SRC, '-o', CALLS, f'-L{root}/lib', '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip',
+           f'-L{HERE}', f'-l:{os.path.basename(LIB)}', '-Wl,-rpath,$ORIGIN']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f'g++ failed for {CALLS_SRC}:\n{r.stdout}\n{r.stderr}')
+    if verbose:
+        print(f'[mv2 build] linked {CALLS}', flush=True)
 
 
 if __name__ == '__main__':

@@ -83,7 +83,8 @@ def _once(backward):
 # ----------------------------------------------------------------------------------------------------------------- gated recurrence
 class _LoopPlan:
     """what follows from the arguments' shapes, strides and types"""
-    __slots__ = ('ops', 'desc', 'fused', 'copy', 'empty', 'T', 'C', 'stride', 'y_shape', 'h_shape', 'states_shape', 'ws_forward', 'ws_backward')
+    __slots__ = ('ops', 'desc', 'fused', 'copy', 'empty', 'T', 'C', 'stride', 'part_shape', 'y_shape', 'h_shape', 'states_shape', 'ws_forward',
+                 'ws_backward', 'native', 'forward', 'backward')
 
 
 def _plan_loop(name, qkva, tokens, state, lengths, resets):
@@ -117,7 +118,7 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
         _need(isinstance(resets, torch.Tensor) and tuple(resets.shape) == (B, T) and resets.dtype in (torch.bool, torch.uint8) and resets.device == dev,
               f'{name}: resets must be bool / uint8 {(B, T)} on {dev}')
     plan.ops = _ops(dev)
-    plan.T, plan.C, plan.y_shape, plan.h_shape = T, C, tuple(shape[:-1]) + (C,), h_shape
+    plan.T, plan.C, plan.part_shape, plan.y_shape, plan.h_shape = T, C, tuple(shape), tuple(shape[:-1]) + (C,), h_shape
     plan.empty = B * P == 0                               # no sequences: nothing to launch, and nothing that a gradient could reach
     if plan.empty:
         return plan
@@ -128,6 +129,7 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
                              in_p=st[rank - 1] if P > 1 else 0, grad_b=T * P * row, grad_t=P * row, grad_p=row)
     states, plan.ws_forward, plan.ws_backward = plan.ops.gateloop_sizes(plan.desc)
     plan.states_shape = (B, states, P, C) if states else None
+    plan.native, plan.forward, plan.backward = plan.ops.loop_plan(plan)
     return plan
 
 
@@ -140,10 +142,7 @@ def _check_state(state, shape, device, name, what='state'):
 class _GateLoop(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, lengths, resets, state, *qkva):
-        ops = plan.ops
-        y, h = ops.empty(plan.y_shape, qkva[0].dtype), ops.empty(plan.h_shape, torch.float32)
-        states = ops.empty(plan.states_shape, torch.float32) if plan.states_shape else None
-        ops.gateloop_forward_now(plan, qkva, state, lengths, resets, y, h, states)
+        y, h, states = plan.forward(plan.native, qkva, state, lengths, resets, None, 2)
         ctx.save_for_backward(state, lengths, resets, states, *qkva)
         ctx.plan = plan
         ctx.set_materialize_grads(False)
@@ -159,13 +158,7 @@ class _GateLoop(torch.autograd.Function):
         if any(t.stride() != plan.stride for t in qkva):      # hooks on saved tensors may lay them out anew
             qkva = [t.contiguous() for t in qkva]
             plan = _plan_loop('gate_loop', qkva[0] if plan.fused else qkva, True, state, lengths, resets)
-        ops, dtype = plan.ops, qkva[0].dtype
-        dy = ops.zeros(plan.y_shape, dtype) if dy is None else _dense(dy)
-        dh = None if dh is None else _dense(dh)
-        grads = tuple(ops.empty(t.shape, dtype) for t in qkva)
-        dstate = ops.empty(plan.h_shape, torch.float32) if ctx.needs_input_grad[3] else None
-        ops.gateloop_backward_now(plan, qkva, state, lengths, resets, states, dy, dh, grads, dstate)
-        return (None, None, None, dstate) + grads
+        return (None, None, None) + plan.backward(plan.native, tuple(qkva), state, lengths, resets, states, dy, dh, ctx.needs_input_grad[3])
 
 
 def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False):
@@ -199,9 +192,7 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
     if torch.is_grad_enabled() and (any(t.requires_grad for t in leaves) or (state is not None and state.requires_grad)):
         y, h = _GateLoop.apply(plan, lengths, resets, state, *leaves)
     else:
-        ops = plan.ops
-        y, h = ops.empty(plan.y_shape, first.dtype), ops.empty(plan.h_shape, torch.float32) if return_state else None
-        ops.gateloop_forward_now(plan, leaves, state, lengths, resets, y, h, None)
+        y, h, _ = plan.forward(plan.native, leaves, state, lengths, resets, None, 1 if return_state else 0)
     return (y, h) if return_state else y
 
 
@@ -224,13 +215,13 @@ def gate_loop_step(qkva, state, *, state_out=None):
     else:
         apart = abs(state_out.data_ptr() - state.data_ptr())
         _need(apart == 0 or apart >= 4 * state.numel(), 'gate_loop_step: state_out overlaps state')
-    y = plan.ops.empty(plan.y_shape, parts[0].dtype)
-    if not plan.empty:
-        if plan.copy:
-            parts = tuple(t.contiguous() for t in parts)
-        plan.ops.gateloop_forward_now(plan, parts, state, None, None, y, state_out, None)
-        if not state_out.is_inference():                  # written behind autograd's back: what saved it must not use it any more
-            torch.autograd.graph.increment_version(state_out)
+    if plan.empty:
+        return parts[0].new_empty(plan.y_shape)
+    if plan.copy:
+        parts = tuple(t.contiguous() for t in parts)
+    y = plan.forward(plan.native, parts, state, None, None, state_out, 0)[0]
+    if not state_out.is_inference():                      # written behind autograd's back: what saved it must not use it any more
+        torch.autograd.graph.increment_version(state_out)
     return y
 
 
@@ -246,7 +237,7 @@ def _plan_step(qkva, state, state_out):
 
 # ----------------------------------------------------------------------------------------------------------------- norms around a block
 class _NormPlan:
-    __slots__ = ('ops', 'desc', 'copy', 'cast', 'strides', 'shape', 'rows', 'branch', 'normed', 'keeps', 'cols', 'ws_backward')
+    __slots__ = ('ops', 'desc', 'copy', 'cast', 'strides', 'shape', 'rows', 'branch', 'normed', 'keeps', 'ws_backward', 'native', 'forward', 'backward')
 
 
 def _row_stride(shape, stride):
@@ -286,18 +277,19 @@ def _plan_norm(x, branch, gate, gate_act, *params):
     if plan.copy:
         steps = [C, C, C]
     plan.strides = None if plan.copy else tuple(None if t is None else t.stride() for t in (x, branch, gate))      # None: all dense
-    plan.shape, plan.rows, plan.cols = tuple(x.shape), x.numel() // C, (C,)
+    plan.shape, plan.rows = tuple(x.shape), x.numel() // C
     plan.branch, plan.normed, plan.keeps = branch is not None, pre is not None, post is not None or pre is not None
     plan.desc = BlockNormDesc(dtype=dtype, C=C, rows=plan.rows, x_stride=steps[0] or 0, branch_stride=steps[1] or 0, gate_stride=steps[2] or 0,
                               gate_act=_ACTS[gate_act] if gate is not None else 0, reserved=0)
     plan.ws_backward = plan.ops.block_norm_workspace_bytes(plan.desc)
+    plan.native, plan.forward, plan.backward = plan.ops.norm_plan(plan)
     return plan
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, act, x, branch, gate, post, scale, pre):
-        out, normed, rstd = _norm_forward(plan, x, branch, gate, post, scale, pre, plan.keeps)
+        out, normed, rstd = plan.forward(plan.native, x, branch, gate, post, scale, pre, True)
         ctx.save_for_backward(x, branch, gate, post, scale, pre, rstd)
         ctx.plan, ctx.act = plan, act
         ctx.set_materialize_grads(False)
@@ -309,27 +301,11 @@ class _BlockNorm(torch.autograd.Function):
         saved = ctx.saved_tensors
         if dout is None and dn is None:
             return (None,) * 8
-        plan, need = ctx.plan, ctx.needs_input_grad
+        plan = ctx.plan
         if any(t is not None and (not t.is_contiguous() if plan.strides is None else t.stride() != plan.strides[i]) for i, t in enumerate(saved[:3])):
             saved = tuple(None if t is None else t.contiguous() for t in saved)      # hooks on saved tensors may lay them out anew
             plan = _plan_norm(*saved[:3], ctx.act, *saved[3:6])
-        ops = plan.ops
-        dtype = saved[0].dtype
-        dout = None if dout is None else _dense(dout)
-        dn = None if dn is None else _dense(dn)
-        rows = [ops.empty(plan.shape, dtype) if n else None for n in need[2:5]]
-        cols = [ops.empty(plan.cols, torch.float32) if n else None for n in need[5:8]]
-        ops.block_norm_backward_now(plan, saved, dout, dn, rows, cols)
-        return None, None, *rows, *cols
-
-
-def _norm_forward(plan, x, branch, gate, post, scale, pre, keep):
-    ops = plan.ops
-    out = ops.empty(plan.shape, x.dtype) if plan.branch else None
-    normed = ops.empty(plan.shape, x.dtype) if plan.normed else None
-    rstd = ops.empty((2, plan.rows), torch.float32) if keep else None
-    ops.block_norm_forward_now(plan, x, branch, gate, post, scale, pre, out, normed, rstd)
-    return out, normed, rstd
+        return (None, None) + plan.backward(plan.native, *saved, dout, dn, ctx.needs_input_grad[2:])
 
 
 def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, scale=None, pre_gamma=None):
@@ -357,5 +333,5 @@ def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, s
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         out, normed = _BlockNorm.apply(plan, gate_act, *args)
     else:
-        out, normed, _ = _norm_forward(plan, *args, False)
+        out, normed, _ = plan.forward(plan.native, *args, False)
     return (out if plan.branch else x), normed

@@ -10,6 +10,7 @@ flat list of C calls that can be captured into a HIP graph.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 
 import torch
@@ -18,6 +19,7 @@ from . import pack as P
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libmv2_hip.so')
+CALLS_PATH = os.path.join(_HERE, '_calls.so')
 
 
 class Mv2Error(RuntimeError):
@@ -137,6 +139,24 @@ def load_library():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_calls = None
+
+
+def load_calls():
+    """the native calls of functional.py (csrc/calls.cpp)"""
+    global _calls
+    if _calls is None:
+        load_library()
+        if not os.path.exists(CALLS_PATH):
+            raise Mv2Error(f'{CALLS_PATH} not built: run `python -m magvit2_pytorch_amd.build`')
+        spec = importlib.util.spec_from_file_location('magvit2_pytorch_amd._calls', CALLS_PATH)
+        calls = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(calls)
+        calls.set_error(Mv2Error)
+        _calls = calls
+    return _calls
 
 
 def _ptr(t):
@@ -305,50 +325,15 @@ class HipOps:
         return _mk(self.lib.mv2_gateloop_backward, args, 'mv2_gateloop_backward',
                    (d, q, kv, a, h0, lengths, resets, states, dy, dh_last, dq, dkv, da, dh0, ws), (dq, dkv, da, dh0))
 
-    # the same at once on the current stream (functional.py), from a call's plan: (qkva,) or (q, kv, a), workspaces allocated here
-    def _now(self, fn, what, *args):
-        """on the current stream of this launcher's device, which need not be the current device"""
-        idx = self.device.index
-        stream = torch._C._cuda_getCurrentRawStream(idx)
-        if torch._C._cuda_getDevice() == idx:
-            rc = fn(*args, stream)
-        else:
-            with torch.cuda.device(idx):
-                rc = fn(*args, stream)
-        if rc != 0:
-            raise Mv2Error(f'{what} failed with code {rc}')
+    # the same at once on the current stream (functional.py), natively from a call's plan: csrc/calls.cpp allocates the results and launches
+    def loop_plan(self, p):
+        c = load_calls()
+        native = c.loop_plan(bytes(p.desc), p.fused, self.device.index, p.part_shape, p.y_shape, p.h_shape, p.states_shape or (), p.ws_forward, p.ws_backward)
+        return native, c.loop_forward, c.loop_backward
 
-    @staticmethod
-    def _loop_ptrs(plan, parts):
-        if plan.fused:
-            p = parts[0].data_ptr()
-            part = plan.C * parts[0].element_size()
-            return p, p + part, p + 2 * part
-        return tuple(t.data_ptr() for t in parts)
-
-    def gateloop_forward_now(self, plan, qkva, h0, lengths, resets, y, h_last, states):
-        n = plan.ws_forward
-        ws = self.empty((n,), torch.uint8) if n else None
-        self._now(self.lib.mv2_gateloop_forward, 'mv2_gateloop_forward', plan.desc, *self._loop_ptrs(plan, qkva), _ptr(h0), _ptr(lengths), _ptr(resets),
-                  y.data_ptr(), _ptr(h_last), _ptr(states), _ptr(ws), n)
-
-    def gateloop_backward_now(self, plan, qkva, h0, lengths, resets, states, dy, dh_last, grads, dh0):
-        n = plan.ws_backward
-        ws = self.empty((n,), torch.uint8) if n else None
-        self._now(self.lib.mv2_gateloop_backward, 'mv2_gateloop_backward', plan.desc, *self._loop_ptrs(plan, qkva), _ptr(h0), _ptr(lengths), _ptr(resets),
-                  _ptr(states), dy.data_ptr(), _ptr(dh_last), *self._loop_ptrs(plan, grads), _ptr(dh0), _ptr(ws), n)
-
-    def block_norm_forward_now(self, plan, x, branch, gate, post, scale, pre, out, normed, rstd):
-        self._now(self.lib.mv2_block_norm_forward, 'mv2_block_norm_forward', plan.desc, x.data_ptr(), _ptr(branch), _ptr(gate), _ptr(post), _ptr(scale),
-                  _ptr(pre), _ptr(out), _ptr(normed), _ptr(rstd))
-
-    def block_norm_backward_now(self, plan, saved, dout, dn, rows, cols):
-        n = 0 if cols[0] is cols[1] is cols[2] is None else plan.ws_backward
-        ws = self.empty((n,), torch.uint8) if n else None
-        x, branch, gate, post, scale, pre, rstd = saved
-        self._now(self.lib.mv2_block_norm_backward, 'mv2_block_norm_backward', plan.desc, x.data_ptr(), _ptr(branch), _ptr(gate), _ptr(post), _ptr(scale),
-                  _ptr(pre), _ptr(rstd), _ptr(dout), _ptr(dn), _ptr(rows[0]), _ptr(rows[1]), _ptr(rows[2]), _ptr(cols[0]), _ptr(cols[1]), _ptr(cols[2]),
-                  _ptr(ws), n)
+    def norm_plan(self, p):
+        c = load_calls()
+        return c.norm_plan(bytes(p.desc), self.device.index, p.shape, p.branch, p.normed, p.keeps, p.ws_backward), c.norm_forward, c.norm_backward
 
     def block_norm_workspace_bytes(self, d: BlockNormDesc) -> int:
         return int(self.lib.mv2_block_norm_workspace_bytes(C.byref(d)))

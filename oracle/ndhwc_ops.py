@@ -580,22 +580,41 @@ class CpuOps:
         step.what = 'gateloop_backward'
         return step
 
-    # at once, from a call's plan (functional.py)
+    # at once, from a call's plan (functional.py): (what the two functions are given for it, forward, backward)
+    def loop_plan(self, plan):
+        return plan, self._loop_forward_now, self._loop_backward_now
+
+    def norm_plan(self, plan):
+        return plan, self._norm_forward_now, self._norm_backward_now
+
     @staticmethod
     def _loop_parts(plan, parts):
         return parts[0].split(plan.C, -1) if plan.fused else parts
 
-    def gateloop_forward_now(self, plan, qkva, h0, lengths, resets, y, h_last, states):
-        self.gateloop_forward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, y, h_last, states, None)(0)
+    def _loop_forward_now(self, plan, qkva, h0, lengths, resets, state_out, want):
+        y, h = torch.empty(plan.y_shape, dtype=qkva[0].dtype), torch.empty(plan.h_shape) if want and state_out is None else None
+        states = torch.empty(plan.states_shape) if want > 1 and plan.states_shape else None
+        self.gateloop_forward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, y, h if state_out is None else state_out, states, None)(0)
+        return y, h, states
 
-    def gateloop_backward_now(self, plan, qkva, h0, lengths, resets, states, dy, dh_last, grads, dh0):
+    def _loop_backward_now(self, plan, qkva, h0, lengths, resets, states, dy, dh_last, wanted):
+        dy = torch.zeros(plan.y_shape, dtype=qkva[0].dtype) if dy is None else dy.contiguous()
+        dh_last = None if dh_last is None else dh_last.contiguous()
+        grads, dh0 = tuple(torch.empty(t.shape, dtype=t.dtype) for t in qkva), torch.empty(plan.h_shape) if wanted else None
         self.gateloop_backward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, states, dy, dh_last, *self._loop_parts(plan, grads), dh0, None)(0)
+        return (dh0,) + grads
 
-    def block_norm_forward_now(self, plan, *args):
-        self.block_norm_forward(plan.desc, *args)(0)
+    def _norm_forward_now(self, plan, x, branch, gate, post, scale, pre, keep):
+        rows = lambda there: torch.empty(plan.shape, dtype=x.dtype) if there else None
+        out, normed, rstd = rows(plan.branch), rows(plan.normed), torch.empty(2, plan.rows) if keep and plan.keeps else None
+        self.block_norm_forward(plan.desc, x, branch, gate, post, scale, pre, out, normed, rstd)(0)
+        return out, normed, rstd
 
-    def block_norm_backward_now(self, plan, saved, dout, dn, rows, cols):
-        self.block_norm_backward(plan.desc, *saved, dout, dn, *rows, *cols, None)(0)
+    def _norm_backward_now(self, plan, x, branch, gate, post, scale, pre, rstd, dout, dn, want):
+        grads = [torch.empty(plan.shape, dtype=x.dtype) if w else None for w in want[:3]] + [torch.empty(plan.desc.C) if w else None for w in want[3:]]
+        dout, dn = (None if g is None else g.contiguous() for g in (dout, dn))
+        self.block_norm_backward(plan.desc, x, branch, gate, post, scale, pre, rstd, dout, dn, *grads, None)(0)
+        return tuple(grads)
 
     def block_norm_workspace_bytes(self, d):
         return 4

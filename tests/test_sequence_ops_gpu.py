@@ -785,3 +785,21 @@ def test_sets_of_groups_in_many_tiles():
     # decays of about 1 - e^-7: a state is off by some 20 units of 2^-24 for each of the ~1100 tokens that it holds, in either call
     tol = 2 * 1100 * 20 * 2.0 ** -24
     assert ((y - ref).abs() <= tol * ref.abs().amax(1, keepdim=True)).all() and ((h - s).abs() <= tol * s.abs().amax()).all()
+
+
+def test_saved_tensors_that_come_back_changed_are_refused():
+    """hooks on saved tensors that hand back another type, size or device end in an error before anything is launched"""
+    C = 16
+    z, x = loop_inputs(1, 9, 1, C, torch.float32).cuda().requires_grad_(), rnd(9, C).cuda().requires_grad_()
+    s, g = rnd(1, 1, C, seed=1).cuda().requires_grad_(), torch.ones(C, device='cuda', requires_grad=True)
+    loop = lambda: F.gate_loop(z, state=s, lengths=torch.tensor([9], device='cuda', dtype=torch.int32), resets=torch.zeros(1, 9, dtype=torch.bool, device='cuda'))
+    norm = lambda: F.block_norm(x, x, gate=x, post_gamma=g, scale=g, pre_gamma=g)[1]
+    for call, count in ((loop, 5), (norm, 7)):                # state, lengths, resets, kept states (none for 9 tokens), qkva; x .. pre_gamma, norms
+        for change in (torch.Tensor.double, torch.Tensor.cpu, lambda t: t.reshape(-1)[:-1]):
+            for which in range(count - (call is loop)):
+                n = iter(range(count))
+                with torch.autograd.graph.saved_tensors_hooks(lambda t: (next(n), t), lambda p: change(p[1]) if p[0] == which else p[1]):
+                    y = call()
+                with pytest.raises((RuntimeError, ValueError)):
+                    y.sum().backward()
+        call().sum().backward()
