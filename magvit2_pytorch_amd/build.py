@@ -93,7 +93,7 @@ def _build_calls(verbose):
     import torch
     root = os.path.dirname(torch.__file__)
     cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
-           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{sysconfig.get_paths()["include"]}', f'-I{root}/include',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{sysconfig.get_paths()["include"]}', f'-I{root}/include', f'-I{root}/include/torch/csrc/api/include',
            f'-I{os.environ.get("ROCM_PATH", "/opt/rocm")}/include', CALLS_SRC, '-o', CALLS, f'-L{root}/lib', '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip',
            f'-L{HERE}', f'-l:{os.path.basename(LIB)}', '-Wl,-rpath,$ORIGIN']
     r = subprocess.run(cmd, capture_output=True, text=True)

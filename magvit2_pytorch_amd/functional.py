@@ -18,7 +18,6 @@ gradient nodes of a leaf to the stream of its first use: a leaf that an eager gr
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .ops_hip import BlockNormDesc, GateLoopDesc, HipOps, Mv2Error
 
@@ -71,20 +70,11 @@ def _dense(t):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _once(backward):
-    """first-order gradients: torch's guard where a graph of the gradients is asked for, without its cost where it is not"""
-    guarded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
-
-
 # ----------------------------------------------------------------------------------------------------------------- gated recurrence
 class _LoopPlan:
     """what follows from the arguments' shapes, strides and types"""
     __slots__ = ('ops', 'desc', 'fused', 'copy', 'empty', 'T', 'C', 'stride', 'part_shape', 'y_shape', 'h_shape', 'states_shape', 'ws_forward',
-                 'ws_backward', 'native', 'forward', 'backward')
+                 'ws_backward', 'native', 'forward')
 
 
 def _plan_loop(name, qkva, tokens, state, lengths, resets):
@@ -129,7 +119,7 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
                              in_p=st[rank - 1] if P > 1 else 0, grad_b=T * P * row, grad_t=P * row, grad_p=row)
     states, plan.ws_forward, plan.ws_backward = plan.ops.gateloop_sizes(plan.desc)
     plan.states_shape = (B, states, P, C) if states else None
-    plan.native, plan.forward, plan.backward = plan.ops.loop_plan(plan)
+    plan.native, plan.forward = plan.ops.loop_plan(plan)
     return plan
 
 
@@ -137,28 +127,6 @@ def _check_state(state, shape, device, name, what='state'):
     _need(isinstance(state, torch.Tensor) and tuple(state.shape) == shape, f'{name}: {what} must be a tensor of shape {shape}')
     _need(state.dtype == torch.float32, f'{name}: {what} is {state.dtype}; states are fp32')
     _need(state.device == device, f'{name}: {what} is on {state.device}, the rows on {device}')
-
-
-class _GateLoop(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, plan, lengths, resets, state, *qkva):
-        y, h, states = plan.forward(plan.native, qkva, state, lengths, resets, None, 2)
-        ctx.save_for_backward(state, lengths, resets, states, *qkva)
-        ctx.plan = plan
-        ctx.set_materialize_grads(False)
-        return y, h
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy, dh):
-        state, lengths, resets, states, *qkva = ctx.saved_tensors
-        if dy is None and dh is None:
-            return (None,) * (4 + len(qkva))
-        plan = ctx.plan
-        if any(t.stride() != plan.stride for t in qkva):      # hooks on saved tensors may lay them out anew
-            qkva = [t.contiguous() for t in qkva]
-            plan = _plan_loop('gate_loop', qkva[0] if plan.fused else qkva, True, state, lengths, resets)
-        return (None, None, None) + plan.backward(plan.native, tuple(qkva), state, lengths, resets, states, dy, dh, ctx.needs_input_grad[3])
 
 
 def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False):
@@ -189,10 +157,8 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
         lengths = _dense(lengths if lengths.dtype == torch.int32 else lengths.clamp(0, plan.T).to(torch.int32))
     if resets is not None:
         resets = _dense(resets)
-    if torch.is_grad_enabled() and (any(t.requires_grad for t in leaves) or (state is not None and state.requires_grad)):
-        y, h = _GateLoop.apply(plan, lengths, resets, state, *leaves)
-    else:
-        y, h, _ = plan.forward(plan.native, leaves, state, lengths, resets, None, 1 if return_state else 0)
+    train = torch.is_grad_enabled() and (any(t.requires_grad for t in leaves) or (state is not None and state.requires_grad))
+    y, h = plan.forward(plan.native, leaves, state, lengths, resets, None, 2 if train else 1 if return_state else 0)
     return (y, h) if return_state else y
 
 
@@ -237,7 +203,7 @@ def _plan_step(qkva, state, state_out):
 
 # ----------------------------------------------------------------------------------------------------------------- norms around a block
 class _NormPlan:
-    __slots__ = ('ops', 'desc', 'copy', 'cast', 'strides', 'shape', 'rows', 'branch', 'normed', 'keeps', 'ws_backward', 'native', 'forward', 'backward')
+    __slots__ = ('ops', 'desc', 'copy', 'cast', 'strides', 'shape', 'rows', 'branch', 'normed', 'keeps', 'ws_backward', 'native', 'forward')
 
 
 def _row_stride(shape, stride):
@@ -282,30 +248,8 @@ def _plan_norm(x, branch, gate, gate_act, *params):
     plan.desc = BlockNormDesc(dtype=dtype, C=C, rows=plan.rows, x_stride=steps[0] or 0, branch_stride=steps[1] or 0, gate_stride=steps[2] or 0,
                               gate_act=_ACTS[gate_act] if gate is not None else 0, reserved=0)
     plan.ws_backward = plan.ops.block_norm_workspace_bytes(plan.desc)
-    plan.native, plan.forward, plan.backward = plan.ops.norm_plan(plan)
+    plan.native, plan.forward = plan.ops.norm_plan(plan)
     return plan
-
-
-class _BlockNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, plan, act, x, branch, gate, post, scale, pre):
-        out, normed, rstd = plan.forward(plan.native, x, branch, gate, post, scale, pre, True)
-        ctx.save_for_backward(x, branch, gate, post, scale, pre, rstd)
-        ctx.plan, ctx.act = plan, act
-        ctx.set_materialize_grads(False)
-        return out, normed
-
-    @staticmethod
-    @_once
-    def backward(ctx, dout, dn):
-        saved = ctx.saved_tensors
-        if dout is None and dn is None:
-            return (None,) * 8
-        plan = ctx.plan
-        if any(t is not None and (not t.is_contiguous() if plan.strides is None else t.stride() != plan.strides[i]) for i, t in enumerate(saved[:3])):
-            saved = tuple(None if t is None else t.contiguous() for t in saved)      # hooks on saved tensors may lay them out anew
-            plan = _plan_norm(*saved[:3], ctx.act, *saved[3:6])
-        return (None, None) + plan.backward(plan.native, *saved, dout, dn, ctx.needs_input_grad[2:])
 
 
 def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, scale=None, pre_gamma=None):
@@ -330,8 +274,6 @@ def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, s
         args = tuple(None if t is None else t.contiguous() for t in args[:3]) + args[3:]
     if plan.cast:
         args = args[:3] + tuple(None if t is None else t.to(torch.float32).contiguous() for t in args[3:])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        out, normed = _BlockNorm.apply(plan, gate_act, *args)
-    else:
-        out, normed, _ = plan.forward(plan.native, *args, False)
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)
+    out, normed = plan.forward(plan.native, *args, train)
     return (out if plan.branch else x), normed

@@ -328,12 +328,13 @@ class HipOps:
     # the same at once on the current stream (functional.py), natively from a call's plan: csrc/calls.cpp allocates the results and launches
     def loop_plan(self, p):
         c = load_calls()
-        native = c.loop_plan(bytes(p.desc), p.fused, self.device.index, p.part_shape, p.y_shape, p.h_shape, p.states_shape or (), p.ws_forward, p.ws_backward)
-        return native, c.loop_forward, c.loop_backward
+        return c.loop_plan(bytes(p.desc), p.fused, self.device.index, p.part_shape, p.y_shape, p.h_shape, p.states_shape or (), p.stride, p.ws_forward,
+                           p.ws_backward), c.loop_forward
 
     def norm_plan(self, p):
         c = load_calls()
-        return c.norm_plan(bytes(p.desc), self.device.index, p.shape, p.branch, p.normed, p.keeps, p.ws_backward), c.norm_forward, c.norm_backward
+        strides = tuple(s or () for s in p.strides or (None,) * 3)
+        return c.norm_plan(bytes(p.desc), self.device.index, p.shape, p.branch, p.normed, p.keeps, *strides, p.ws_backward), c.norm_forward
 
     def block_norm_workspace_bytes(self, d: BlockNormDesc) -> int:
         return int(self.lib.mv2_block_norm_workspace_bytes(C.byref(d)))

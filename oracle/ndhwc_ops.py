@@ -16,6 +16,9 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
+
+from magvit2_pytorch_amd import functional as F
 
 ACT_NONE, ACT_ELU, ACT_SILU, ACT_GEGLU, ACT_LRELU = 0, 1, 2, 3, 4
 STORE_ROWS, STORE_SHUFFLE, STORE_NCTHW_F32, STORE_ROWS_F32 = 0, 1, 2, 3
@@ -580,41 +583,30 @@ class CpuOps:
         step.what = 'gateloop_backward'
         return step
 
-    # at once, from a call's plan (functional.py): (what the two functions are given for it, forward, backward)
+    # at once, from a call's plan (functional.py): (what the function is given for it, the function)
     def loop_plan(self, plan):
-        return plan, self._loop_forward_now, self._loop_backward_now
+        return plan, self._loop_now
 
     def norm_plan(self, plan):
-        return plan, self._norm_forward_now, self._norm_backward_now
+        return plan, self._norm_now
 
     @staticmethod
-    def _loop_parts(plan, parts):
+    def loop_parts(plan, parts):
         return parts[0].split(plan.C, -1) if plan.fused else parts
 
-    def _loop_forward_now(self, plan, qkva, h0, lengths, resets, state_out, want):
-        y, h = torch.empty(plan.y_shape, dtype=qkva[0].dtype), torch.empty(plan.h_shape) if want and state_out is None else None
-        states = torch.empty(plan.states_shape) if want > 1 and plan.states_shape else None
-        self.gateloop_forward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, y, h if state_out is None else state_out, states, None)(0)
-        return y, h, states
+    def _loop_now(self, plan, qkva, h0, lengths, resets, state_out, want):
+        if want == 2:
+            return _EmulatedLoop.apply(plan, lengths, resets, h0, *qkva)
+        y, h = torch.empty(plan.y_shape, dtype=qkva[0].dtype), torch.empty(plan.h_shape) if want else None
+        self.gateloop_forward(plan.desc, *self.loop_parts(plan, qkva), h0, lengths, resets, y, h if state_out is None else state_out, None, None)(0)
+        return y, h
 
-    def _loop_backward_now(self, plan, qkva, h0, lengths, resets, states, dy, dh_last, wanted):
-        dy = torch.zeros(plan.y_shape, dtype=qkva[0].dtype) if dy is None else dy.contiguous()
-        dh_last = None if dh_last is None else dh_last.contiguous()
-        grads, dh0 = tuple(torch.empty(t.shape, dtype=t.dtype) for t in qkva), torch.empty(plan.h_shape) if wanted else None
-        self.gateloop_backward(plan.desc, *self._loop_parts(plan, qkva), h0, lengths, resets, states, dy, dh_last, *self._loop_parts(plan, grads), dh0, None)(0)
-        return (dh0,) + grads
-
-    def _norm_forward_now(self, plan, x, branch, gate, post, scale, pre, keep):
-        rows = lambda there: torch.empty(plan.shape, dtype=x.dtype) if there else None
-        out, normed, rstd = rows(plan.branch), rows(plan.normed), torch.empty(2, plan.rows) if keep and plan.keeps else None
-        self.block_norm_forward(plan.desc, x, branch, gate, post, scale, pre, out, normed, rstd)(0)
-        return out, normed, rstd
-
-    def _norm_backward_now(self, plan, x, branch, gate, post, scale, pre, rstd, dout, dn, want):
-        grads = [torch.empty(plan.shape, dtype=x.dtype) if w else None for w in want[:3]] + [torch.empty(plan.desc.C) if w else None for w in want[3:]]
-        dout, dn = (None if g is None else g.contiguous() for g in (dout, dn))
-        self.block_norm_backward(plan.desc, x, branch, gate, post, scale, pre, rstd, dout, dn, *grads, None)(0)
-        return tuple(grads)
+    def _norm_now(self, plan, x, branch, gate, post, scale, pre, train):
+        if train:
+            return _EmulatedNorm.apply(plan, x, branch, gate, post, scale, pre)
+        out, normed = (torch.empty(plan.shape, dtype=x.dtype) if there else None for there in (plan.branch, plan.normed))
+        self.block_norm_forward(plan.desc, x, branch, gate, post, scale, pre, out, normed, None)(0)
+        return out, normed
 
     def block_norm_workspace_bytes(self, d):
         return 4
@@ -975,3 +967,59 @@ class CpuOps:
         step.outs = [o for o in [out] if o is not None]
         step.what = 'fsq_codes'
         return step
+
+
+class _EmulatedLoop(torch.autograd.Function):
+    """gradients of gate_loop by the emulated kernels"""
+    @staticmethod
+    def forward(ctx, plan, lengths, resets, state, *qkva):
+        y, h = torch.empty(plan.y_shape, dtype=qkva[0].dtype), torch.empty(plan.h_shape)
+        states = torch.empty(plan.states_shape) if plan.states_shape else None
+        plan.ops.gateloop_forward(plan.desc, *plan.ops.loop_parts(plan, qkva), state, lengths, resets, y, h, states, None)(0)
+        ctx.save_for_backward(state, lengths, resets, states, *qkva)
+        ctx.plan = plan
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        state, lengths, resets, states, *qkva = ctx.saved_tensors
+        plan, ops = ctx.plan, ctx.plan.ops
+        if any(t.stride() != plan.stride for t in qkva):      # hooks on saved tensors may lay them out anew
+            qkva = [t.contiguous() for t in qkva]
+            plan = F._plan_loop('gate_loop', qkva[0] if plan.fused else qkva, True, state, lengths, resets)
+        if dy is None and dh is None:
+            return (None,) * (4 + len(qkva))
+        dy = torch.zeros(plan.y_shape, dtype=qkva[0].dtype) if dy is None else dy.contiguous()
+        dh = None if dh is None else dh.contiguous()
+        grads, dstate = tuple(torch.empty(t.shape, dtype=t.dtype) for t in qkva), torch.empty(plan.h_shape) if ctx.needs_input_grad[3] else None
+        ops.gateloop_backward(plan.desc, *ops.loop_parts(plan, qkva), state, lengths, resets, states, dy, dh, *ops.loop_parts(plan, grads), dstate, None)(0)
+        return (None, None, None, dstate) + grads
+
+
+class _EmulatedNorm(torch.autograd.Function):
+    """gradients of block_norm by the emulated kernels"""
+    @staticmethod
+    def forward(ctx, plan, *args):
+        out, normed = (torch.empty(plan.shape, dtype=args[0].dtype) if there else None for there in (plan.branch, plan.normed))
+        rstd = torch.empty(2, plan.rows) if plan.keeps else None
+        plan.ops.block_norm_forward(plan.desc, *args, out, normed, rstd)(0)
+        ctx.save_for_backward(*args, rstd)
+        ctx.plan = plan
+        ctx.set_materialize_grads(False)
+        return out, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dn):
+        plan, saved, want = ctx.plan, ctx.saved_tensors, ctx.needs_input_grad[1:]
+        if any(t is not None and (not t.is_contiguous() if plan.strides is None else t.stride() != plan.strides[i]) for i, t in enumerate(saved[:3])):
+            saved = tuple(None if t is None else t.contiguous() for t in saved)      # hooks on saved tensors may lay them out anew
+            plan = F._plan_norm(*saved[:3], {0: 'none', 2: 'silu', 5: 'sigmoid'}[plan.desc.gate_act], *saved[3:6])
+        if dout is None and dn is None:
+            return (None,) * 7
+        grads = [torch.empty(plan.shape, dtype=saved[0].dtype) if w else None for w in want[:3]] + [torch.empty(plan.desc.C) if w else None for w in want[3:]]
+        dout, dn = (None if g is None else g.contiguous() for g in (dout, dn))
+        plan.ops.block_norm_backward(plan.desc, *saved, dout, dn, *grads, None)(0)
+        return (None, *grads)

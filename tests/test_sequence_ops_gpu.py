@@ -1,7 +1,10 @@
 """The sequence operators (gated recurrence, block norms) on the GPU against the 64-bit references of tests/_sequence_ref.py, within the
 running error bounds derived there."""
+import contextlib
+
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from magvit2_pytorch_amd import functional as F
 from magvit2_pytorch_amd.ops_hip import BlockNormDesc, GateLoopDesc, HipOps
@@ -803,3 +806,55 @@ def test_saved_tensors_that_come_back_changed_are_refused():
                 with pytest.raises((RuntimeError, ValueError)):
                     y.sum().backward()
         call().sum().backward()
+
+
+@pytest.mark.parametrize('fused', [True, False])
+def test_saved_tensors_laid_out_anew(fused):
+    """hooks on saved tensors give back copies of another layout than the views that were saved"""
+    B, T, C = 2, 300, 40
+    wide, up = rnd(T, B, 3 * C + 3).cuda().requires_grad_(), rnd(B, T, C, seed=1).cuda()
+    rows, w = rnd(70, 3 * C, seed=2).cuda().requires_grad_(), torch.ones(C, device='cuda', requires_grad=True)
+    grads = []
+    for pack in (None, lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.cuda()) if pack else contextlib.nullcontext():
+            z = wide.transpose(0, 1)[..., 2:2 + 3 * C]
+            y = F.gate_loop(z if fused else z.split(C, -1))
+            q, kv, a = rows.split(C, -1)
+            out, n = F.block_norm(q, kv, gate=a, post_gamma=w, pre_gamma=w)
+        grads.append(torch.autograd.grad((y, out, n), (wide, rows, w), (up, torch.ones_like(out), rnd(70, C, seed=3).cuda())))
+    for other in grads[1:]:
+        for a, b in zip(grads[0], other):                 # rows at other alignments may be summed by another kernel
+            assert ((a - b).abs() <= 64 * 2.0 ** -24 * b.abs().amax()).all()
+
+
+def test_graphs_of_gradients():
+    """gradients of some inputs only, of one output only, twice from a kept graph, added up in .grad, through a checkpoint; a released graph and
+    forward-mode derivatives are refused"""
+    C = 24
+    z, s = loop_inputs(2, 50, 1, C, torch.float32).cuda().requires_grad_(), rnd(2, 1, C, seed=1).cuda().requires_grad_()
+    x, b, w = (rnd(*n, seed=i).cuda().requires_grad_() for i, n in enumerate(((30, C), (30, C), (C,))))
+    loop, norm = lambda: F.gate_loop(z, state=s, return_state=True), lambda: F.block_norm(x, b, gate=b, post_gamma=w, scale=w, pre_gamma=w)
+    for call, leaves in ((loop, (z, s)), (norm, (x, b, w))):
+        outs = call()
+        ups = [rnd(*o.shape, seed=7 + i).cuda() for i, o in enumerate(outs)]
+        full = torch.autograd.grad(outs, leaves, ups, retain_graph=True)
+        again = torch.autograd.grad(outs, leaves, ups, retain_graph=True)
+        assert all(torch.equal(a, c) for a, c in zip(full, again))
+        for i, leaf in enumerate(leaves):
+            assert torch.equal(torch.autograd.grad(outs, leaf, ups, retain_graph=True)[0], full[i])
+        one = [torch.autograd.grad(o, leaves, u, retain_graph=True) for o, u in zip(outs, ups)]
+        zero = [torch.autograd.grad(outs, leaves, [u if i == j else torch.zeros_like(u) for j, u in enumerate(ups)], retain_graph=True) for i in range(2)]
+        for a, c in zip(one, zero):
+            assert all(torch.allclose(p, q, rtol=1e-5, atol=1e-5 * q.abs().max().item()) for p, q in zip(a, c))
+        torch.autograd.backward(outs, ups, retain_graph=True)
+        torch.autograd.backward(outs, ups)
+        assert all(torch.equal(leaf.grad, 2 * f) for leaf, f in zip(leaves, full))
+        with pytest.raises(RuntimeError):
+            torch.autograd.backward(outs, ups)
+        under = torch.utils.checkpoint.checkpoint(call, use_reentrant=False)
+        assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(under, leaves, ups), full))
+        with torch.autograd.set_detect_anomaly(True):
+            assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(call(), leaves, ups), full))
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            dual = torch.autograd.forward_ad.make_dual(leaves[0].detach(), torch.ones_like(leaves[0])).requires_grad_()
+            F.gate_loop(dual) if call is loop else F.block_norm(dual, pre_gamma=w)
