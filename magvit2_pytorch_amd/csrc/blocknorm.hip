@@ -12,6 +12,7 @@
 //     69632 x 256 bf16, add and norm forward 25 (5.7, part of it from the last-level cache), backward 40 (4.4)
 //     65536 x 512 bf16               forward 62 (5.4), backward 109 (4.9)        8192 x 2048 fp32  forward 60 (5.6), backward 100 (5.4)
 //     16384 x 1001 bf16, ragged      forward 41 (4.0), backward 79 (3.3)         4097 x 501 fp32   forward 14, backward 23
+//     6250 x 5120 bf16               forward 64 (5.0), backward 180 (2.8)        6251 x 5119 bf16, ragged  88 (3.6), 228 (2.2)
 // Forward it is the memory; backward also the 160 to 200 registers, which leave two or three waves on a SIMD.  32 rows take 5 us: latency.
 #include <algorithm>
 #include <initializer_list>
@@ -95,13 +96,15 @@ template <int NC, int V> struct Params {
     }
 };
 
+// (four waves on a SIMD: ragged rows of 3999 bf16 84 us, 103 with the 132 registers that the compiler would take)
 template <typename E, int V, bool RAG, int NC, int R, int BLOCK, bool S>
-__global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G, const void* x, const void* __restrict__ branch, const void* __restrict__ gate,
+__global__ __launch_bounds__(BLOCK, 4) void block_norm_fwd_kernel(NormArgs A, int G, const void* x, const void* __restrict__ branch, const void* __restrict__ gate,
                                                                const float* __restrict__ w1, const float* __restrict__ sc, const float* __restrict__ w2,
                                                                void* out, void* __restrict__ normed, float* __restrict__ rstd) {
     __shared__ float red[2][R][BLOCK / 64];
     GroupSum<BLOCK, R> sum{red, 0};
-    const int l = threadIdx.x & (G - 1), per = BLOCK / G;
+    // rows of more than one chunk a thread have a workgroup of their own, of G threads (whole waves), others a power of two of threads
+    const int l = NC > 1 ? threadIdx.x : threadIdx.x & (G - 1), per = NC > 1 ? 1 : BLOCK / G, mine = NC > 1 ? 0 : threadIdx.x / G;
     const int nch = (A.C + V - 1) / V;
     const Params<NC, V> p1(w1, A.root, l, G, A.C), ps(sc, 1.f, l, G, A.C), p2(w2, A.root, l, G, A.C);
     const int64_t step = (int64_t)per * R;
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs A, int G
         RowVec<E, V, RAG> vx[R][NC], vb[R][NC], vg[R][NC];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            row[i] = base + i * per + threadIdx.x / G;
+            row[i] = base + i * per + mine;
             on[i] = row[i] < A.rows;
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
@@ -206,7 +209,8 @@ __global__ __launch_bounds__(BLOCK, NC == 1 ? 3 : 1) void block_norm_bwd_kernel(
                                                                void* __restrict__ dgate, float* __restrict__ parts) {
     __shared__ float red[2][R][BLOCK / 64];
     GroupSum<BLOCK, R> sum{red, 0};
-    const int l = threadIdx.x & (G - 1), per = BLOCK / G;
+    // rows of more than one chunk a thread have a workgroup of their own, of G threads (whole waves), others a power of two of threads
+    const int l = NC > 1 ? threadIdx.x : threadIdx.x & (G - 1), per = NC > 1 ? 1 : BLOCK / G, mine = NC > 1 ? 0 : threadIdx.x / G;
     const int nch = (A.C + V - 1) / V;
     const Params<NC, V> p1(w1, A.root, l, G, A.C), ps(sc, 1.f, l, G, A.C), p2(w2, A.root, l, G, A.C);
     const int64_t step = (int64_t)per * R;
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(BLOCK, NC == 1 ? 3 : 1) void block_norm_bwd_kernel(
         float r1[R], r2[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            row[i] = base + i * per + threadIdx.x / G;
+            row[i] = base + i * per + mine;
             on[i] = row[i] < A.rows;
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
@@ -419,15 +423,19 @@ static int norm_check(const mv2_block_norm_desc* d) {
 }
 
 // threads per row G, chunks per thread NC, rows at a time R: the row's chunks spread over up to 256 threads first, then over two registers, then over
-// up to 1024 threads (and four registers); R > 1 once every workgroup of a full chip has that many rows
+// up to 1024 threads (and four registers); R > 1 once every workgroup of a full chip has that many rows.  Rows of more than 256 chunks take as many
+// whole waves as they fill (6250 x 5120 bf16 64 us forward, 75 with a power of two), but a power of two backward, where the registers leave one
+// workgroup on a CU either way (184 and 180)
 struct NormShape { int access, NC, R, block, G; bool stream; };
-static NormShape norm_shape(const mv2_block_norm_desc* d, int access, int tensors) {
+static NormShape norm_shape(const mv2_block_norm_desc* d, int access, int tensors, bool backward) {
     const int es = d->dtype == MV2_BF16 ? 2 : 4, V = access ? 16 / es : 1, nch = (d->C + V - 1) / V;
     NormShape s{access, 1, 1, 256, 1, access == 2 && calls_stream((double)d->rows * d->C * tensors * es)};
     while (s.G < nch && s.G < 256) s.G *= 2;
     if (nch > 256) {
         s.NC = nch <= 2048 ? 2 : 4;
-        while (s.G * s.NC < nch) s.block = s.G *= 2;
+        s.G = ((nch + s.NC - 1) / s.NC + 63) / 64 * 64;
+        while (backward && (s.G < 256 || (s.G & (s.G - 1)))) s.G += 64;
+        s.block = s.G;
     }
     if (s.NC == 1 && d->rows / (s.block / s.G) >= (int64_t)NORM_R * NORM_GROUPS) s.R = NORM_R;
     return s;
@@ -472,7 +480,7 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
     } while (0)
 #define NORM_ACCESS(KERNEL, E, V, ...)                                                                            \
         if (s.access == 2 && s.stream && s.NC == 1 && s.R > 1) NORM_GO(KERNEL, E, V, false, 1, NORM_R, 256, true, __VA_ARGS__);         \
-        else if (s.access == 2 && s.stream && s.NC == 2 && s.block == 256) NORM_GO(KERNEL, E, V, false, 2, 1, 256, true, __VA_ARGS__);  \
+        else if (s.access == 2 && s.stream && s.NC == 2 && s.block <= 256) NORM_GO(KERNEL, E, V, false, 2, 1, 256, true, __VA_ARGS__);  \
         else if (s.access == 2) { NORM_SHAPES(KERNEL, E, V, false, true, __VA_ARGS__) }                           \
         else if (s.access == 1) { NORM_SHAPES(KERNEL, E, V, true, false, __VA_ARGS__) }                           \
         else if (s.R == 1) NORM_GO(KERNEL, E, 1, false, 1, 1, 256, false, __VA_ARGS__);                           \
@@ -480,11 +488,11 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
 #define NORM_SHAPES(KERNEL, E, V, RAG, S, ...)                                                                    \
         if (s.NC == 1 && s.R == 1) NORM_GO(KERNEL, E, V, RAG, 1, 1, 256, false, __VA_ARGS__);                     \
         else if (s.NC == 1) NORM_GO(KERNEL, E, V, RAG, 1, NORM_R, 256, false, __VA_ARGS__);                       \
-        else if (s.block == 256) NORM_GO(KERNEL, E, V, RAG, 2, 1, 256, false, __VA_ARGS__);                       \
-        else if (s.block == 512) NORM_GO(KERNEL, E, V, RAG, 2, 1, 512, S, __VA_ARGS__);                           \
+        else if (s.block <= 256) NORM_GO(KERNEL, E, V, RAG, 2, 1, 256, false, __VA_ARGS__);                       \
+        else if (s.block <= 512) NORM_GO(KERNEL, E, V, RAG, 2, 1, 512, S, __VA_ARGS__);                           \
         else if (s.NC == 2) NORM_GO(KERNEL, E, V, RAG, 2, 1, 1024, S, __VA_ARGS__);                               \
         else NORM_GO(KERNEL, E, V, RAG, V == 4 ? 4 : 2, 1, 1024, S, __VA_ARGS__);
-#define NORM_GO(KERNEL, E, V, RAG, NC, R, BLOCK, S, ...) hipLaunchKernelGGL((KERNEL<E, V, RAG, NC, R, BLOCK, S>), dim3(grid), dim3(BLOCK), 0, st, A, s.G, __VA_ARGS__)
+#define NORM_GO(KERNEL, E, V, RAG, NC, R, BLOCK, S, ...) hipLaunchKernelGGL((KERNEL<E, V, RAG, NC, R, BLOCK, S>), dim3(grid), dim3((NC) > 1 ? s.block : BLOCK), 0, st, A, s.G, __VA_ARGS__)
 
 extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post_gamma,
                                       const float* scale, const float* pre_gamma, void* out, void* normed, float* rstd, void* stream) {
@@ -494,9 +502,12 @@ extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* 
     if (d->rows == 0) return MV2_OK;
     if (!x || (branch && !out) || (pre_gamma && !normed)) return MV2_EINVAL;
     const int access = norm_access(d, branch, gate, {x, branch, gate, out, normed});
-    const NormShape s = norm_shape(d, access, 1 + !!branch * 2 + !!gate + !!pre_gamma);
+    const NormShape s = norm_shape(d, access, 1 + !!branch * 2 + !!gate + !!pre_gamma, false);
     const NormArgs A = norm_args(d);
-    const unsigned grid = norm_grid(d, s, 1024);       // 16384 x 2048: 71 us, 73 with 2048
+    // as many workgroups as the chip holds at once: 4 waves on a SIMD by the registers of the shapes, 6 of those of aligned fp32 chunks (6250 x 5120
+    // bf16 64 us with 512 workgroups of 5 waves, 82 with 768; 16384 x 2048 71, 73 with twice as many)
+    const int held = s.NC > 1 && d->dtype == MV2_F32 && access == 2 ? 6 : 4;
+    const unsigned grid = norm_grid(d, s, 256 * std::max(1, held / ((s.block + 255) / 256)));
     hipStream_t st = (hipStream_t)stream;
     NORM_CASES(block_norm_fwd_kernel, x, branch, gate, post_gamma, scale, pre_gamma, out, normed, rstd);
     MV2_LAUNCH_CHECK();
@@ -515,7 +526,7 @@ extern "C" int mv2_block_norm_backward(const mv2_block_norm_desc* d, const void*
     const bool cols = dpost || dscale || dpre;
     if (cols && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < mv2_block_norm_workspace_bytes(d))) return MV2_EWORKSPACE;
     const int access = norm_access(d, branch, gate, {x, branch, gate, dout, dn, dx, dbranch, dgate});
-    const NormShape s = norm_shape(d, access, !!dout + !!dn * 2 + !!branch + !!gate + !!dx + !!dbranch + !!dgate);
+    const NormShape s = norm_shape(d, access, !!dout + !!dn * 2 + !!branch + !!gate + !!dx + !!dbranch + !!dgate, true);
     const NormArgs A = norm_args(d);
     const unsigned grid = norm_grid(d, s, norm_bwd_grid(d, s));
     float* parts = cols ? (float*)workspace : nullptr;

@@ -858,3 +858,17 @@ def test_graphs_of_gradients():
         with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
             dual = torch.autograd.forward_ad.make_dual(leaves[0].detach(), torch.ones_like(leaves[0])).requires_grad_()
             F.gate_loop(dual) if call is loop else F.block_norm(dual, pre_gamma=w)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('C', [1028, 1284, 1537, 2055, 2560, 3080, 5119, 5120, 6144, 7000, 7168, 10240, 12288, 14000])
+def test_block_norm_whole_waves(C, dtype):
+    """widths that fill 3 to 16 waves of a workgroup, in one row and in more rows than the chip takes at once"""
+    check_norm(3, C, dtype)
+    R = 1700
+    gen = torch.Generator('cuda').manual_seed(C)
+    x, b, g = (torch.randn(R, C, device='cuda', generator=gen).to(dtype) for _ in range(3))
+    w = [torch.rand(C, device='cuda', generator=gen) + 0.5 for _ in range(3)]
+    part = lambda i: F.block_norm(x[i], b[i], gate=g[i], post_gamma=w[0], scale=w[1], pre_gamma=w[2])
+    for whole, *parts in zip(part(slice(0, R)), *(part(slice(i, i + 100)) for i in range(0, R, 100))):
+        assert torch.equal(whole, torch.cat(parts))
