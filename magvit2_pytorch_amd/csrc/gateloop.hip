@@ -6,7 +6,7 @@
 // One or two flops a byte: the work is to read every element once (4 tensors forward, 7 backward) and to keep the chip's memory busy.  A copy of
 // 256 MB in 16-byte accesses runs at 5.9 TB/s.  Measured on one MI355X, us and TB/s of those tensors, kernels alone:
 //     walks   4 x 17 tokens x 1024 x 256 bf16       forward 25 (5.7; part of it from the last-level cache), backward 55 (4.5)
-//     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 99 - 105 (4.5 - 4.8); with document starts 60 and 108
+//     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 95 (4.9); with document starts 55 and 103
 //             1 x 131072 x 512 bf16                 forward 106 (5.1), backward 193 (4.9); 1 x 100000 x 64 23 and 35
 //             6 x 4095 x 1000 bf16, rows off lines  forward 53 (3.7), backward 94 (3.7)
 //             3 x 1023 x 777 fp32                   forward 13, backward 17 (9.5 MB a tensor: as much latency as bandwidth)
@@ -376,6 +376,10 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
     unsigned cuts = 0;
     if (b0 < n) {
         const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
+        unsigned char start[L];                               // read first: rows may still be on their way when these are needed (read behind them 60 us, 55)
+        if (CUTS)
+#pragma unroll
+            for (int i = 0; i < L; ++i) start[i] = A.resets[(int64_t)b * A.T + min(t0 + i, n - 1)];
 #pragma unroll
         for (int i = 0; i < L; ++i) {                         // rows behind the last token are not read: the last one stands in for them
             const int64_t at = in0 + (int64_t)min(t0 + i, n - 1) * A.st;
@@ -383,11 +387,9 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
         }
 #pragma unroll
         for (int i = 0; i < L; ++i) { va[i].settle(nv); vk[i].settle(nv); vq[i].settle(nv); }
-        if (CUTS) {
-            const unsigned char* rs = A.resets + (int64_t)b * A.T;
+        if (CUTS)
 #pragma unroll
-            for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && rs[min(t0 + i, n - 1)]) ? 1u << i : 0u;
-        }
+            for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && start[i]) ? 1u << i : 0u;
     } else {
 #pragma unroll
         for (int i = 0; i < L; ++i) { va[i].clear(); vk[i].clear(); vq[i].clear(); }
@@ -413,7 +415,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) ph[k] = fmaf(g[i][k], ph[k], fk[k]);
-            if (CUTS && __any(cuts >> i & 1))                 // documents start in few waves: the others do without the choice
+            if (CUTS)
 #pragma unroll
                 for (int k = 0; k < V; ++k) ph[k] = cuts >> i & 1 ? fk[k] : ph[k];
         }
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
         vk[i].get(fk); vq[i].get(fq);
 #pragma unroll
         for (int k = 0; k < V; ++k) h[k] = fmaf(g[i][k], h[k], fk[k]);
-        if (CUTS && __any(cuts >> i & 1))
+        if (CUTS)
 #pragma unroll
             for (int k = 0; k < V; ++k) h[k] = cuts >> i & 1 ? fk[k] : h[k];
 #pragma unroll
@@ -488,6 +490,10 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
         RowVec<E, V, RAG> va[L];
         if (b0 < n) {
             const int64_t in0 = (int64_t)b * A.sb + (int64_t)p * A.sp + cc;
+            unsigned char start[L];
+            if (CUTS)
+#pragma unroll
+                for (int i = 0; i < L; ++i) start[i] = A.resets[(int64_t)b * A.T + min(t0 + i, n - 1)];
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 const int t = min(t0 + i, n - 1);
@@ -496,11 +502,9 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
             }
 #pragma unroll
             for (int i = 0; i < L; ++i) { va[i].settle(nv); vk[i].settle(nv); vq[i].settle(nv); vy[i].settle(nv); }
-            if (CUTS) {
-                const unsigned char* rs = A.resets + (int64_t)b * A.T;
+            if (CUTS)
 #pragma unroll
-                for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && rs[min(t0 + i, n - 1)]) ? 1u << i : 0u;
-            }
+                for (int i = 0; i < L; ++i) cuts |= (t0 + i < n && start[i]) ? 1u << i : 0u;
             if (chok) {
                 if (kb > 0) hin = states[(((int64_t)b * A.nstate + kb - 1) * A.P + p) * A.C + chc];
                 else if (h0) hin = h0[(int64_t)seq * A.C + chc];
@@ -540,7 +544,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
                 ph[k] = fmaf(g, ph[k], fk[k]);
                 pa[k] *= g;
             }
-            if (CUTS && __any(cuts >> i & 1))                 // documents start in few waves: the others do without the choice
+            if (CUTS)
 #pragma unroll
                 for (int k = 0; k < V; ++k) ph[k] = cuts >> i & 1 ? fk[k] : ph[k];
         }
@@ -550,7 +554,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
             vq[i].get(fq); vy[i].get(fy);
 #pragma unroll
             for (int k = 0; k < V; ++k) pu[k] = decay(i, k) * fmaf(fq[k], fy[k], pu[k]);
-            if (CUTS && __any(cuts >> i & 1))
+            if (CUTS)
 #pragma unroll
                 for (int k = 0; k < V; ++k) pu[k] = cuts >> i & 1 ? 0.f : pu[k];
         }
@@ -592,7 +596,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
         vk[i].get(fk); vy[i].get(fy);
 #pragma unroll
         for (int k = 0; k < V; ++k) h[i + 1][k] = fmaf(decay(i, k), h[i][k], fk[k]);
-        if (CUTS && __any(cuts >> i & 1))
+        if (CUTS)
 #pragma unroll
             for (int k = 0; k < V; ++k) h[i + 1][k] = cuts >> i & 1 ? fk[k] : h[i + 1][k];
 #pragma unroll
@@ -613,7 +617,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
             oa[k] = fq[k] * h[i][k] * (s * (1.f - s));
             back[k] = decay(i, k) * fq[k];
         }
-        if (CUTS && __any(cuts >> i & 1))
+        if (CUTS)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 oa[k] = cuts >> i & 1 ? 0.f : oa[k];
