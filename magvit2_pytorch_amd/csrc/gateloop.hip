@@ -5,7 +5,7 @@
 // Everything between the loads and the stores is fp32; only y, dq, dkv, da are rounded to the storage type (on their stores, once).
 // One or two flops a byte: the work is to read every element once (4 tensors forward, 7 backward) and to keep the chip's memory busy.  A copy of
 // 256 MB in 16-byte accesses runs at 5.9 TB/s.  Measured on one MI355X, us and TB/s of those tensors, kernels alone:
-//     walks   4 x 17 tokens x 1024 x 256 bf16       forward 25 (5.7; part of it from the last-level cache), backward 55 (4.5)
+//     walks   4 x 17 tokens x 1024 x 256 bf16       forward 25 (5.7; part of it from the last-level cache), backward 52 (4.8)
 //     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 95 (4.9); with document starts 55 and 103
 //             1 x 131072 x 512 bf16                 forward 106 (5.1), backward 193 (4.9); 1 x 100000 x 64 23 and 35
 //             6 x 4095 x 1000 bf16, rows off lines  forward 53 (3.7), backward 94 (3.7)
@@ -48,6 +48,17 @@ __device__ __forceinline__ void walk_place(const LoopArgs& A, int64_t i, int64_t
     }
 }
 
+// the marks of 8 tokens from t on, a byte each (0 behind token T - 1).  Asked for before the tokens' rows, which may then still be on their way when
+// the marks are needed (4 x 33 x 512 x 256 bf16 28 us, read behind the rows 34)
+typedef unsigned long long Marks __attribute__((aligned(1)));
+__device__ __forceinline__ unsigned long long eight_marks(const unsigned char* rs, int t, int T) {
+    if (t + LOOP_STEPS <= T) return *(const Marks*)(rs + t);
+    unsigned long long w = 0;
+    for (int s = 0; t + s < T; ++s) w |= (unsigned long long)rs[t + s] << 8 * s;
+    return w;
+}
+__device__ __forceinline__ bool mark(unsigned long long w, int s) { return (unsigned)(w >> 8 * s) & 0xff; }
+
 template <typename E, int V, bool S>
 __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const void* __restrict__ q, const void* __restrict__ kv, const void* __restrict__ a,
                                                             const float* h0, void* __restrict__ y, float* hlast, float* __restrict__ states) {
@@ -72,13 +83,12 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
         constexpr int M = decltype(most)::value;
         constexpr bool GUARD = decltype(guard)::value;
         RowVec<E, V> vq[M], vk[M], va[M];
-        unsigned cuts = 0;
+        const unsigned long long cuts = rs ? eight_marks(rs, t, A.T) : 0;
 #pragma unroll
         for (int s = 0; s < M; ++s)
             if (!GUARD || t + s < n) {
                 const int64_t at = in0 + (t + s) * A.st;
                 vk[s].template load<S>(kv, at); va[s].template load<S>(a, at); vq[s].template load<S>(q, at);
-                if (rs) cuts |= rs[t + s] ? 1u << s : 0u;
             }
         if (states && t > 0) {
             float* o = states + (((int64_t)b * A.nstate + t / LOOP_STEPS - 1) * A.P + p) * A.C + c;
@@ -92,7 +102,7 @@ __global__ __launch_bounds__(256) void loop_walk_fwd_kernel(LoopArgs A, const vo
                 vq[s].get(fq); vk[s].get(fk); va[s].get(fa);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    h[k] = cuts >> s & 1 ? fk[k] : fmaf(sigm<E>(fa[k]), h[k], fk[k]);
+                    h[k] = mark(cuts, s) ? fk[k] : fmaf(sigm<E>(fa[k]), h[k], fk[k]);
                     fq[k] *= h[k];
                 }
                 RowVec<E, V>::template store<S>(y, y0 + (t + s) * yt, fq);
@@ -140,6 +150,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
     for (int blk = (n + LOOP_STEPS - 1) / LOOP_STEPS - 1; blk >= 0; --blk) {
         const int t0 = blk * LOOP_STEPS;
         RowVec<E, V, RAG> vq[LOOP_STEPS], vk[LOOP_STEPS], va[LOOP_STEPS], vy[LOOP_STEPS];
+        const unsigned long long cuts = rs ? eight_marks(rs, t0, A.T) : 0;
 #pragma unroll
         for (int s = 0; s < LOOP_STEPS; ++s)
             if (t0 + s < n) {
@@ -157,7 +168,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
             if (t0 + s < n) {
                 float fk[V], fa[V];
                 vk[s].get(fk); va[s].get(fa);
-                const bool cut = rs && rs[t0 + s];
+                const bool cut = mark(cuts, s);
 #pragma unroll
                 for (int k = 0; k < V; ++k) h[s + 1][k] = cut ? fk[k] : fmaf(sigm<E>(fa[k]), h[s][k], fk[k]);
             }
@@ -166,7 +177,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
             if (t0 + s < n) {
                 float fq[V], fa[V], fy[V], oq[V], oa[V], ok[V];
                 vq[s].get(fq); va[s].get(fa); vy[s].get(fy);
-                const bool cut = rs && rs[t0 + s];
+                const bool cut = mark(cuts, s);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     float g, slope;
