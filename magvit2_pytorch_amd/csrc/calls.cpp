@@ -1,7 +1,7 @@
 // The calls of the sequence operators from Python (functional.py) and their gradients' nodes: outputs and workspaces are allocated and the C ABI
 // (include/mv2.h) is called on the current stream of the tensors' device, in one native call each and without the interpreter's lock.  What the
 // arguments' shapes, strides and types lead to is in a plan: functional.py checks them and makes it.  Where the host is what a call takes, the
-// same from Python (ctypes, torch.empty, a Function of Python's) is dearer: a single token 9.1 us against 7.2, norms of 32 rows 11.9 and 8.8,
+// same from Python (ctypes, torch.empty, a Function of Python's) is dearer: a single token 9.1 us against 6.4, norms of 32 rows 11.9 and 7.2,
 // norms of 4097 x 501 fp32 and their six gradients 165 and 101 (native calls under a Function of Python's 122; torch's engine takes some 80).
 #include <Python.h>
 #include <ATen/ATen.h>
@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <cstdint>
 #include <cstring>
 #include <initializer_list>
 #include <memory>
@@ -332,6 +333,40 @@ PyObject* norm_plan(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// what a plan depends on of its arguments, as bytes: of a tensor shape, strides, type and device, of a tuple or list of tensors those of each, of a
+// text itself, of None that it is None.  None is returned for anything else (functional.py then says what is wrong with it).
+bool add_key(std::string& k, PyObject* o, int depth) {
+    const auto put = [&](int64_t v) { k.append(reinterpret_cast<const char*>(&v), sizeof v); };
+    if (o == Py_None) put(-1);
+    else if (THPVariable_Check(o)) {
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (t.layout() != at::kStrided) return false;
+        put(t.dim());
+        for (int64_t v : t.sizes()) put(v);
+        for (int64_t v : t.strides()) put(v);
+        put((int64_t)t.scalar_type() << 32 | (int64_t)(uint8_t)t.device().type() << 16 | (uint16_t)t.device().index());
+    } else if (PyUnicode_Check(o)) {
+        Py_ssize_t n;
+        const char* c = PyUnicode_AsUTF8AndSize(o, &n);
+        if (!c) { PyErr_Clear(); return false; }
+        put(-2 - n);
+        k.append(c, n);
+    } else if ((PyTuple_Check(o) || PyList_Check(o)) && depth == 0) {
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+        put(INT64_MIN + n);
+        for (Py_ssize_t i = 0; i < n; ++i) if (!add_key(k, PySequence_Fast_GET_ITEM(o, i), 1)) return false;
+    } else return false;
+    return true;
+}
+PyObject* key(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::string k;
+    k.reserve(512);
+    for (Py_ssize_t i = 0; i < nargs; ++i) if (!add_key(k, args[i], 0)) Py_RETURN_NONE;
+    return PyBytes_FromStringAndSize(k.data(), (Py_ssize_t)k.size());
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error(PyObject*, PyObject* cls) {
     Py_INCREF(cls);
     Py_XSETREF(error_class, cls);
@@ -339,7 +374,7 @@ PyObject* set_error(PyObject*, PyObject* cls) {
 }
 
 #define FAST(name) {#name, (PyCFunction)(void*)name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(loop_forward), FAST(norm_forward),
+PyMethodDef methods[] = {FAST(loop_forward), FAST(norm_forward), FAST(key),
                          {"loop_plan", loop_plan, METH_VARARGS, nullptr}, {"norm_plan", norm_plan, METH_VARARGS, nullptr},
                          {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

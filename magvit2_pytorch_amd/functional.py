@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import torch
 
-from .ops_hip import BlockNormDesc, GateLoopDesc, HipOps, Mv2Error
+from .ops_hip import BlockNormDesc, GateLoopDesc, HipOps, Mv2Error, load_calls
 
 __all__ = ['gate_loop', 'gate_loop_step', 'block_norm']
 
@@ -36,6 +36,8 @@ def _ops(device):
         if device.type != 'cuda':
             raise Mv2Error(f'tensors on {device}: these operators run on a HIP device and have no CPU fallback')
         ops = _backends[device] = HipOps(device)
+        global _key
+        _key = load_calls().key
     return ops
 
 
@@ -50,8 +52,14 @@ def _row_dtype(t, name):
     return _DTYPES[t.dtype]
 
 
-def _like(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+def _key(*args):
+    """what a plan depends on: shapes, strides, types and devices; None where arguments are not tensors (the plan says what is wrong).  On a HIP
+    device the native form of this takes its place (csrc/calls.cpp)"""
+    like = lambda t: t if t is None or isinstance(t, str) else (t.shape, t.stride(), t.dtype, t.device)
+    try:
+        return tuple(tuple(map(like, a)) if isinstance(a, (tuple, list)) else like(a) for a in args)
+    except (AttributeError, TypeError):
+        return None
 
 
 def _plan(key, make, *args):
@@ -139,11 +147,7 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
     uint8, tokens that start a new document: no state and no gradient crosses them.
     Returns ``y`` (``(B, T[, P], C)``, dense), with ``return_state`` also the last state.  Gradients reach ``qkva`` and ``state``."""
     fused = isinstance(qkva, torch.Tensor)
-    try:
-        key = ('loop', _like(qkva) if fused else tuple(map(_like, qkva)), _like(state), _like(lengths), _like(resets))
-    except (AttributeError, TypeError):                   # not tensors: the plan says what is wrong
-        key = None
-    plan = _plan(key, _plan_loop, 'gate_loop', qkva, True, state, lengths, resets)
+    plan = _plan(_key('loop', qkva, state, lengths, resets), _plan_loop, 'gate_loop', qkva, True, state, lengths, resets)
     leaves = (qkva,) if fused else tuple(qkva)
     first = leaves[0]
     if plan.empty:
@@ -167,11 +171,7 @@ def gate_loop_step(qkva, state, *, state_out=None):
     written over ``state``, or into ``state_out`` (dense fp32, the same shape; apart from ``state``, or ``state`` itself).  Returns ``y`` ``(B[, P], C)``.
     For inference: it has no gradient."""
     fused = isinstance(qkva, torch.Tensor)
-    try:
-        key = ('step', _like(qkva) if fused else tuple(map(_like, qkva)), _like(state), _like(state_out))
-    except (AttributeError, TypeError):
-        key = None
-    plan = _plan(key, _plan_step, qkva, state, state_out)
+    plan = _plan(_key('step', qkva, state, state_out), _plan_step, qkva, state, state_out)
     parts = (qkva,) if fused else tuple(qkva)
     if torch.is_grad_enabled():
         _need(not (state.requires_grad or (state_out is not None and state_out.requires_grad) or any(t.requires_grad for t in parts)),
@@ -263,12 +263,7 @@ def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, s
     Left out: ``branch`` - no add, ``out`` is ``x``; ``post_gamma`` - the branch enters as it is; ``gate``, ``scale`` - ones; ``pre_gamma`` - no second
     norm, ``normed`` is None.  C <= 16384.  Sums of squares are fp32: N of a row with ``|v| >= 1.8e19`` is zero.
     Returns ``(out, normed)``.  Gradients reach every tensor; the parameters' are bitwise reproducible."""
-    try:
-        key = ('norm', _like(x), _like(branch), _like(gate), gate_act, _like(post_gamma), _like(scale), _like(pre_gamma))
-        hash(gate_act)
-    except (AttributeError, TypeError):
-        key = None
-    plan = _plan(key, _plan_norm, x, branch, gate, gate_act, post_gamma, scale, pre_gamma)
+    plan = _plan(_key('norm', x, branch, gate, gate_act, post_gamma, scale, pre_gamma), _plan_norm, x, branch, gate, gate_act, post_gamma, scale, pre_gamma)
     args = (x, branch, gate, post_gamma, scale, pre_gamma)
     if plan.copy:
         args = tuple(None if t is None else t.contiguous() for t in args[:3]) + args[3:]

@@ -274,3 +274,16 @@ def test_abi_refuses_before_any_launch():
     assert nb(N(), rstd=None) == EINVAL and nb(N(), g=None) == EINVAL and nb(N(), pre=None) == EINVAL
     assert nb(N()) == EWORKSPACE and nb(N(), ws=ptr, nws=16) == EWORKSPACE
     assert lib.mv2_block_norm_workspace_bytes(ctypes.byref(N())) > 0 and lib.mv2_block_norm_workspace_bytes(ctypes.byref(N(C=0))) == 0
+
+
+def test_native_keys_tell_apart_what_the_plain_ones_do():
+    native, plain = ops_hip.load_calls().key, F._key
+    t = rnd(3, 4)
+    calls = [('loop', a, b, None) for b in (None, t, t.double(), t.t(), t[:, :2], t[None], t[0], t.expand(2, 3, 4), t.new_empty(0, 4))
+             for a in (t, (t, t), (t, t, t), (t, t, None), 'silu', None)] + [('loopt', t), ('loop', 't'), ('loop',), ('', 'loop')]
+    for a in calls:
+        for b in calls:
+            assert (native(*a) == native(*b)) == (plain(*a) == plain(*b)), (a, b)
+    assert native('norm', rnd(3, 4, seed=9)) == native('norm', t) and native('loop', [t, t]) == native('loop', (t, t))
+    for bad in (3, t.to_sparse(), object(), [[t]]):
+        assert native('loop', bad) is None
