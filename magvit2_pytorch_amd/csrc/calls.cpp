@@ -122,6 +122,7 @@ torch::autograd::variable_list first_order(torch::autograd::variable_list g, con
     auto end = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has gradients of first order only", (int64_t)g.size());
     return end->apply(std::move(g));
 }
+// whether or not the inputs require gradients: a dual tensor need not, and its tangent would be left out in silence
 void no_tangents(std::initializer_list<const at::Tensor*> ts, const char* what) {
     for (const at::Tensor* t : ts) TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
@@ -144,6 +145,7 @@ struct LoopNode : torch::autograd::Node {
         at::Tensor h0 = state.unpack(), n = lengths.unpack(), cuts = resets.unpack(), kept = states.unpack(), x[3];
         for (int i = 0; i < np; ++i) x[i] = parts[i].unpack();
         if (!up[0].defined() && !up[1].defined()) return g;
+        no_tangents({&up[0], &up[1]}, "gate_loop");
         const int64_t rows = (int64_t)p.d.B * p.d.P * p.d.C;
         mv2_gateloop_desc d = p.d;
         bool same = true;
@@ -191,6 +193,7 @@ struct NormNode : torch::autograd::Node {
         at::Tensor t[7];
         for (int i = 0; i < 7; ++i) t[i] = saved[i].unpack();
         if (!up[0].defined() && !up[1].defined()) return g;
+        no_tangents({&up[0], &up[1]}, "block_norm");
         mv2_block_norm_desc d = p.d;
         bool same = true;
         for (int i = 0; i < 3; ++i) {
@@ -230,6 +233,7 @@ PyObject* loop_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (int i = 0; i < np; ++i) x[i] = tensor(PyTuple_GET_ITEM(args[1], i));
     const at::Tensor &state = tensor(args[2]), &lengths = tensor(args[3]), &resets = tensor(args[4]);
     at::Tensor h = tensor(args[5]), y;
+    no_tangents({&state, &h, x, x + 1, x + 2}, "gate_loop");
     const bool own = !h.defined();
     const long want = PyLong_AsLong(args[6]);
     {
@@ -246,7 +250,6 @@ PyObject* loop_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                                                ptr(y), ptr<float>(h), ptr<float>(states), ptr(ws), (size_t)p->ws_forward, at.stream()));
         }
         if (want >= 2) {
-            no_tangents({&state, x, x + 1, x + 2}, "gate_loop");
             auto node = std::shared_ptr<LoopNode>(new LoopNode(), torch::autograd::deleteNode);
             if (p->fused) node->set_next_edges(torch::autograd::collect_next_edges(state, x[0]));
             else node->set_next_edges(torch::autograd::collect_next_edges(state, x[0], x[1], x[2]));
@@ -271,6 +274,7 @@ PyObject* norm_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PLAN(NormPlan, NORM);
     at::Tensor t[7], out, normed;
     for (int i = 0; i < 6; ++i) t[i] = tensor(args[1 + i]);
+    no_tangents({t, t + 1, t + 2, t + 3, t + 4, t + 5}, "block_norm");
     const bool train = args[7] == Py_True;
     {
         const Unlocked unlocked;
@@ -284,7 +288,6 @@ PyObject* norm_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                                                    ptr(out), ptr(normed), ptr<float>(t[6]), at.stream()));
         }
         if (train) {
-            no_tangents({t, t + 1, t + 2, t + 3, t + 4, t + 5}, "block_norm");
             auto node = std::shared_ptr<NormNode>(new NormNode(), torch::autograd::deleteNode);
             node->set_next_edges(torch::autograd::collect_next_edges(t[0], t[1], t[2], t[3], t[4], t[5]));
             node->plan = *held;

@@ -12,7 +12,7 @@ and differentiates it with autograd; ``VideoTokenizer``'s own ``gateloop_time`` 
 Tensors live on one HIP device; bf16 or fp32 rows, fp32 states and parameters.  Calls enqueue on the current stream of that device, allocate
 their outputs and workspaces from torch's allocator and can be captured into a HIP graph.  As with every torch operator, a tensor that was
 made on another stream must be ordered and recorded (``record_stream``) by the caller.  There is no CPU path: CPU tensors raise ``Mv2Error``.
-Gradients are first order.  To capture a backward pass, capture the forward pass that belongs to it in the same graph (torch ties the
+Gradients are first order and backward mode: inputs or gradients with tangents (forward mode) are refused.  To capture a backward pass, capture the forward pass that belongs to it in the same graph (torch ties the
 gradient nodes of a leaf to the stream of its first use: a leaf that an eager graph still holds must not be captured).
 """
 from __future__ import annotations

@@ -287,3 +287,30 @@ def test_native_keys_tell_apart_what_the_plain_ones_do():
     assert native('norm', rnd(3, 4, seed=9)) == native('norm', t) and native('loop', [t, t]) == native('loop', (t, t))
     for bad in (3, t.to_sparse(), object(), [[t]]):
         assert native('loop', bad) is None
+
+
+def native_plans(B=2, C=4):
+    """plans of a token's step / a call of one token and of norms, as functional.py makes them, and the functions that take them"""
+    calls = ops_hip.load_calls()
+    d = ops_hip.GateLoopDesc(dtype=1, B=B, T=1, P=1, C=C, in_b=3 * C, in_t=0, in_p=0, grad_b=3 * C, grad_t=3 * C, grad_p=3 * C)
+    e = ops_hip.BlockNormDesc(dtype=1, C=C, rows=B, x_stride=C, branch_stride=C, gate_stride=C, gate_act=2, reserved=0)
+    loop = calls.loop_plan(bytes(d), True, 0, (B, 3 * C), (B, C), (B, C), (), (3 * C, 1), 0, 0)
+    norm = calls.norm_plan(bytes(e), 0, (B, C), True, True, True, (C, 1), (C, 1), (C, 1), 0)
+    return calls.loop_forward, loop, calls.norm_forward, norm
+
+
+def test_tangents_are_refused_before_anything_is_launched():
+    """an input with a tangent but without requires_grad: neither operator has a forward-mode derivative, and none may be left out in silence"""
+    loop_forward, loop, norm_forward, norm = native_plans()
+    z, s, x, w = rnd(2, 12), rnd(2, 4, seed=1), rnd(2, 4, seed=2), torch.ones(4)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for args in ((dual(z), s, None), (z, dual(s), None), (z, s, dual(rnd(2, 4)))):
+            for want in (0, 1, 2):
+                with pytest.raises(NotImplementedError):
+                    loop_forward(loop, args[:1], args[1], None, None, args[2], want)
+        args = (x, x, x, w, w, w)
+        for i in range(6):
+            for train in (False, True):
+                with pytest.raises(NotImplementedError):
+                    norm_forward(norm, *args[:i], dual(args[i]), *args[i + 1:], train)

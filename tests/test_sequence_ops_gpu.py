@@ -872,3 +872,26 @@ def test_block_norm_whole_waves(C, dtype):
     part = lambda i: F.block_norm(x[i], b[i], gate=g[i], post_gamma=w[0], scale=w[1], pre_gamma=w[2])
     for whole, *parts in zip(part(slice(0, R)), *(part(slice(i, i + 100)) for i in range(0, R, 100))):
         assert torch.equal(whole, torch.cat(parts))
+
+
+def test_tangents_are_refused():
+    """forward mode through every entry point, by any input, whether or not it requires grad, and by the gradients that arrive: refused, nothing written"""
+    from torch.autograd import forward_ad
+    C = 16
+    z, s, x, w = rnd(2, 40, 3 * C).cuda(), rnd(2, C, seed=1).cuda(), rnd(7, C, seed=2).cuda(), torch.ones(C, device='cuda')
+    leaf, rows = z.clone().requires_grad_(), x.clone().requires_grad_()
+    y, (out, _) = F.gate_loop(leaf), F.block_norm(rows, x, pre_gamma=w)
+    s0, new = s.clone(), torch.full_like(s, 7.)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: F.gate_loop(dual(z)), lambda: F.gate_loop(z, state=dual(s)), lambda: F.gate_loop((z[..., :C], z[..., C:2 * C], dual(z[..., 2 * C:]))),
+                     lambda: F.gate_loop_step(dual(z[:, 0]), s), lambda: F.gate_loop_step(z[:, 0], dual(s)), lambda: F.gate_loop_step(z[:, 0], s, state_out=dual(new)),
+                     lambda: F.block_norm(dual(x), pre_gamma=w), lambda: F.block_norm(x, dual(x)), lambda: F.block_norm(x, x, gate=dual(x)),
+                     lambda: F.block_norm(x, pre_gamma=dual(w)), lambda: F.block_norm(x, x, scale=dual(w)), lambda: F.block_norm(x, x, post_gamma=dual(w)),
+                     lambda: torch.autograd.grad(y, leaf, dual(torch.ones_like(y)), retain_graph=True),
+                     lambda: torch.autograd.grad(out, rows, dual(torch.ones_like(out)), retain_graph=True)):
+            for mode in (contextlib.nullcontext, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError):
+                    call()
+    assert torch.equal(s, s0) and (new == 7).all()
+    torch.autograd.grad((y, out), (leaf, rows), (torch.ones_like(y), torch.ones_like(out)))
