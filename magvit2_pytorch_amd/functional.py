@@ -117,7 +117,7 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
               f'{name}: resets must be bool / uint8 {(B, T)} on {dev}')
     plan.ops = _ops(dev)
     plan.T, plan.C, plan.part_shape, plan.y_shape, plan.h_shape = T, C, tuple(shape), tuple(shape[:-1]) + (C,), h_shape
-    plan.empty = B * P == 0                               # no sequences: nothing to launch, and nothing that a gradient could reach
+    plan.empty = B * P == 0                               # no sequences: nothing to launch
     if plan.empty:
         return plan
     plan.copy = (first.stride(-1) != 1 and shape[-1] > 1) or any(t.stride() != first.stride() for t in parts)
@@ -149,10 +149,8 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
     fused = isinstance(qkva, torch.Tensor)
     plan = _plan(_key('loop', qkva, state, lengths, resets), _plan_loop, 'gate_loop', qkva, True, state, lengths, resets)
     leaves = (qkva,) if fused else tuple(qkva)
-    first = leaves[0]
     if plan.empty:
-        y = first.new_empty(plan.y_shape)
-        return (y, first.new_empty(plan.h_shape, dtype=torch.float32)) if return_state else y
+        return _empty_loop(plan, leaves, state, return_state)
     if plan.copy:
         leaves = tuple(t.contiguous() for t in leaves)
     if state is not None:
@@ -164,6 +162,15 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
     train = torch.is_grad_enabled() and (any(t.requires_grad for t in leaves) or (state is not None and state.requires_grad))
     y, h = plan.forward(plan.native, leaves, state, lengths, resets, None, 2 if train else 1 if return_state else 0)
     return (y, h) if return_state else y
+
+
+def _empty_loop(plan, leaves, state, return_state):
+    """results without an element, tied to every input as those of the kernels are: a training step passes through a batch of no sequences"""
+    q, kv, a = leaves[0].split(plan.C, -1) if plan.fused else leaves
+    y = q + kv + a
+    if state is not None:
+        y = y + state.unsqueeze(1).to(y.dtype)
+    return (y, y.sum(1, dtype=torch.float32)) if return_state else y
 
 
 def gate_loop_step(qkva, state, *, state_out=None):

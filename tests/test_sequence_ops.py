@@ -314,3 +314,23 @@ def test_tangents_are_refused_before_anything_is_launched():
             for train in (False, True):
                 with pytest.raises(NotImplementedError):
                     norm_forward(norm, *args[:i], dual(args[i]), *args[i + 1:], train)
+
+
+@pytest.mark.parametrize('shape', [(0, 3, 2), (0, 3), (2, 3, 0), (0, 0)])
+@pytest.mark.parametrize('fused', [True, False])
+def test_an_empty_batch_keeps_its_graph(emulated, shape, fused):
+    """no sequences (B = 0 or no pixels): gradients of nothing reach every input, and what lies behind them zeros, as with torch's operators"""
+    C, w = 4, rnd(5, 12, seed=1).requires_grad_()
+    z = torch.zeros(*shape, 5) @ w
+    parts = z.split(C, -1)
+    s = torch.zeros(*shape[:1], *shape[2:], C, requires_grad=True)
+    y, h = F.gate_loop(z if fused else tuple(parts), state=s, return_state=True)
+    assert y.shape == (*shape, C) and h.shape == s.shape and y.dtype == z.dtype and h.dtype == torch.float32
+    for outs in ((y, h), (y,), (h,)):
+        got = torch.autograd.grad([o.sum() for o in outs], [s, w, *((z,) if fused else parts)], retain_graph=True)
+        assert not any(g.any() for g in got) and got[0].shape == s.shape
+    half = F.gate_loop(z.detach().bfloat16().requires_grad_(), state=s, return_state=True)
+    assert half[0].dtype == torch.bfloat16 and half[0].requires_grad and half[1].dtype == torch.float32 and half[1].requires_grad
+    with torch.no_grad():
+        assert not F.gate_loop(z, state=s).requires_grad
+    assert not F.gate_loop(z.detach()).requires_grad

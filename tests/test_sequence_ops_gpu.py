@@ -895,3 +895,16 @@ def test_tangents_are_refused():
                     call()
     assert torch.equal(s, s0) and (new == 7).all()
     torch.autograd.grad((y, out), (leaf, rows), (torch.ones_like(y), torch.ones_like(out)))
+
+
+@pytest.mark.parametrize('shape', [(0, 3, 2), (0, 3), (2, 3, 0), (2, 0), (0, 0)])
+def test_an_empty_batch_keeps_its_graph(shape):
+    """no sequences or no tokens, in a training step: gradients reach every input, and what lies behind them"""
+    C, w = 8, rnd(5, 24, seed=1).cuda().requires_grad_()
+    z, s = torch.zeros(*shape, 5, device='cuda') @ w, torch.zeros(*shape[:1], *shape[2:], C, device='cuda', requires_grad=True)
+    for rows in (z, z.bfloat16(), tuple(z.split(C, -1))):
+        y, h = F.gate_loop(rows, state=s, return_state=True)
+        g = torch.autograd.grad((y.float().sum(), h.sum()), (s, w), retain_graph=True)
+        assert y.shape == (*shape, C) and h.shape == s.shape and h.dtype == torch.float32 and g[0].shape == s.shape and not g[1].any()
+        out, n = F.block_norm(y, y, pre_gamma=torch.ones(C, device='cuda'))
+        assert not torch.autograd.grad(n.float().sum(), w, retain_graph=True)[0].any() and out.shape == y.shape
