@@ -398,7 +398,9 @@ int mv2_gateloop_scan(int dtype, const void* qkva, const void* residual, void* o
  * Any C and any strides are served (rows that are whole, aligned 16-byte chunks fastest); T = 0 gives h_last = h0.
  * workspace: mv2_gateloop_workspace_bytes(d, backward) bytes, 8-byte aligned, contents irrelevant (the call clears what it uses with a
  * kernel of its own); calls that run at the same time, and captured graphs that are replayed at the same time, need one each.
- * Sums are joined in a fixed order: results are bitwise reproducible. */
+ * Sums are joined in a fixed order: results are bitwise reproducible.
+ * An infinite state (or gradient of one) stays infinite for as long as the decays are above 0, as token by token; a decay that is computed as 0 (a below
+ * about -87) makes it NaN, a document start ends it. */
 typedef struct mv2_gateloop_desc {
     int32_t dtype;
     int32_t B, T, P, C;

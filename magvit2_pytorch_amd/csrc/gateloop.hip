@@ -225,6 +225,27 @@ __device__ __forceinline__ float pair_A(u64 w) { return __uint_as_float((unsigne
 __device__ __forceinline__ float pair_H(u64 w) { return __uint_as_float((unsigned)w); }
 __device__ __forceinline__ void publish(u64* p, float A, float H) { __hip_atomic_store(p, pair_word(A, H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+// A of two spans.  It stays above 0 where both are: a product below the smallest number, 1.4e-45, becomes that number (no further off than the rounding
+// of any product down there), so that an infinite state stays infinite as it does token by token; a decay of exactly 0 makes it NaN in either form.
+// The bits of numbers that are not negative are ordered as the numbers are, NaN highest: it stays.
+__device__ __forceinline__ float spans_decay(float A, float A2) {
+    return __uint_as_float(max(__float_as_uint(A * A2), min(min(__float_as_uint(A), __float_as_uint(A2)), 1u)));
+}
+// the same for the product of a lane's L decays, g(i, k) of channel k: looked at again only where one came out as 0
+template <int L, int V, typename G> __device__ __forceinline__ void lane_decay(float (&pa)[V], G g) {
+    unsigned least = __float_as_uint(pa[0]);
+#pragma unroll
+    for (int k = 1; k < V; ++k) least = min(least, __float_as_uint(pa[k]));
+    if (least == 0)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            unsigned low = 1;
+#pragma unroll
+            for (int i = 0; i < L; ++i) low = min(low, __float_as_uint(g(i, k)));
+            pa[k] = __uint_as_float(max(__float_as_uint(pa[k]), low));
+        }
+}
+
 // state behind a span, from the state in front of it; CUTS: may documents start in it?
 template <bool CUTS> __device__ __forceinline__ float pass(float A, float H, float h) {
     const float r = fmaf(A, h, H);
@@ -233,7 +254,7 @@ template <bool CUTS> __device__ __forceinline__ float pass(float A, float H, flo
 // (A, H) := (A, H) then (A2, H2)
 template <bool CUTS> __device__ __forceinline__ void join(float& A, float& H, float A2, float H2) {
     H = pass<CUTS>(A2, H2, H);
-    const float r = A * A2;
+    const float r = spans_decay(A, A2);
     A = CUTS && (A == LOOP_CUT || A2 == LOOP_CUT) ? LOOP_CUT : r;
 }
 
@@ -430,6 +451,7 @@ __global__ __launch_bounds__(WAVES * 64) void loop_span_fwd_kernel(LoopArgs A, S
 #pragma unroll
                 for (int k = 0; k < V; ++k) ph[k] = cuts >> i & 1 ? fk[k] : ph[k];
         }
+        lane_decay<L, V>(pa, [&](int i, int k) { return g[i][k]; });
 #pragma unroll
         for (int k = 0; k < V; ++k) { rowA[row][cl * V + k] = CUTS && cuts ? LOOP_CUT : pa[k]; rowH[row][cl * V + k] = ph[k]; }
     }
@@ -569,6 +591,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
 #pragma unroll
                 for (int k = 0; k < V; ++k) pu[k] = cuts >> i & 1 ? 0.f : pu[k];
         }
+        lane_decay<L, V>(pa, decay);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             rowA[row][cl * V + k] = CUTS && cuts ? LOOP_CUT : pa[k];

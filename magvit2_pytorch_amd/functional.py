@@ -145,6 +145,7 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
     ``lengths``: ``(B,)`` int32 / int64, tokens per sample in a padded batch (values are taken into ``[0, T]``): ``y`` and the gradients are zero
     behind them, whatever the rows hold there, and the last state is the one behind the last token that exists.  ``resets``: ``(B, T)`` bool /
     uint8, tokens that start a new document: no state and no gradient crosses them.
+    An infinite state stays infinite while decays are above zero (``a`` above about -87) and is NaN behind a decay of zero; a document start ends it.
     Returns ``y`` (``(B, T[, P], C)``, dense), with ``return_state`` also the last state.  Gradients reach ``qkva`` and ``state``."""
     fused = isinstance(qkva, torch.Tensor)
     plan = _plan(_key('loop', qkva, state, lengths, resets), _plan_loop, 'gate_loop', qkva, True, state, lengths, resets)

@@ -908,3 +908,43 @@ def test_an_empty_batch_keeps_its_graph(shape):
         assert y.shape == (*shape, C) and h.shape == s.shape and h.dtype == torch.float32 and g[0].shape == s.shape and not g[1].any()
         out, n = F.block_norm(y, y, pre_gamma=torch.ones(C, device='cuda'))
         assert not torch.autograd.grad(n.float().sum(), w, retain_graph=True)[0].any() and out.shape == y.shape
+
+
+def kind(t):
+    """0 finite, 1 and 2 infinities, 3 NaN"""
+    return torch.where(t.isnan(), 3, torch.where(t.isinf(), torch.where(t > 0, 1, 2), 0)).cpu()
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('T', [8, 40, 300, 9000])
+@pytest.mark.parametrize('C', [3, 40])
+def test_infinite_states_decay_as_token_by_token(T, C, dtype):
+    """an infinite state stays infinite while the decays are above zero, however small their product gets, in every form that the sizes choose; a
+    decay of zero makes it NaN, a document start ends it.  So do infinite gradients on their way back.  Channels without one are as they were."""
+    B = 5
+    z = loop_inputs(B, T, 1, C, dtype, T)
+    z[..., 2 * C:] -= 5                                   # decays of about 0.05: products of hundreds are far below the smallest number
+    clean, s, dh = z.clone(), rnd(B, 1, C, seed=1), rnd(B, 1, C, seed=2)
+    s0, dh0 = s.clone(), dh.clone()
+    dy = rnd(B, T, 1, C, seed=3, dtype=dtype)
+    resets = torch.zeros(B, T, dtype=torch.bool)
+    s[0, :, 0], s[1, :, -1] = INF, -INF
+    z[2, T // 2, 0, C] = INF                              # kv of channel 0
+    dh[3, :, 0], dh[4, :, 0], s[4, :, 0] = INF, -INF, INF
+    z[4, T // 2, 0, 2 * C] = -INF                         # a decay of zero
+    resets[1, T - 2] = True
+    hit = torch.zeros(B, C, dtype=torch.bool)
+    for b, c in ((0, 0), (1, C - 1), (2, 0), (3, 0), (4, 0)):
+        hit[b, c] = True
+    res = []
+    for zz, ss, dd in ((z, s, dh), (clean, s0, dh0)):
+        leaf, st = zz.cuda().requires_grad_(), ss.cuda().requires_grad_()
+        y, h = F.gate_loop(leaf, state=st, resets=resets.cuda(), return_state=True)
+        g, gs = torch.autograd.grad((y, h), (leaf, st), (dy.cuda(), dd.cuda()))
+        res.append(dict(y=y, h=h[:, None], dstate=gs[:, None], **dict(zip(('dq', 'dkv', 'da'), g.split(C, -1)))))
+    ref = gate_loop_ref(*z.split(C, -1), s, None, resets, dy, dh)
+    for name, got in res[0].items():
+        want = ref[name][0].reshape(got.shape)
+        assert torch.equal(kind(got), kind(want)), name
+        rest = ~hit.cuda()[:, None, None].expand(got.shape)
+        assert torch.equal(got[rest], res[1][name][rest]), name
