@@ -77,9 +77,9 @@ template <typename T = void> T* ptr(const at::Tensor& t) { return t.defined() ? 
 // what a hook on saved tensors gave back must still be what was saved, but for the layout of rows
 void still(const at::Tensor& t, int device, at::ScalarType type, at::IntArrayRef shape, bool whole) {
     TORCH_CHECK(!t.defined() || (t.device() == c10::Device(c10::kCUDA, (c10::DeviceIndex)device) && t.scalar_type() == type && t.sizes() == shape &&
-                                 (!whole || t.is_contiguous())), "a tensor saved for the backward pass came back with another type, size, layout or device");
+                                 !t.is_neg() && (!whole || t.is_contiguous())), "a tensor saved for the backward pass came back with another type, size, layout or device");
 }
-at::Tensor dense(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
+at::Tensor dense(const at::Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }      // (a gradient may be negated lazily)
 
 PyObject* wrapped(std::initializer_list<at::Tensor> ts) {
     PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
@@ -164,7 +164,7 @@ struct LoopNode : torch::autograd::Node {
         still(n, p.device, at::kInt, {p.d.B}, true);
         if (cuts.defined()) still(cuts, p.device, cuts.scalar_type() == at::kBool ? at::kBool : at::kByte, {p.d.B, p.d.T}, true);
         const Device at(p.device);
-        const at::Tensor dy = up[0].defined() ? up[0].contiguous() : at.empty(p.y, type).zero_(), dh = dense(up[1]);
+        const at::Tensor dy = up[0].defined() ? dense(up[0]) : at.empty(p.y, type).zero_(), dh = dense(up[1]);
         for (int i = 0; i < np; ++i) g[1 + i] = at.empty(p.part, type);
         if (task_should_compute_output(0)) g[0] = at.empty(p.h, at::kFloat);
         const at::Tensor ws = at.workspace(p.ws_backward);
@@ -336,7 +336,7 @@ PyObject* norm_plan(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
-// what a plan depends on of its arguments, as bytes: of a tensor shape, strides, type and device, of a tuple or list of tensors those of each, of a
+// what a plan depends on of its arguments, as bytes: of a tensor shape, strides, type, device and whether it is negated lazily, of a tuple or list of tensors those of each, of a
 // text itself, of None that it is None.  None is returned for anything else (functional.py then says what is wrong with it).
 bool add_key(std::string& k, PyObject* o, int depth) {
     const auto put = [&](int64_t v) { k.append(reinterpret_cast<const char*>(&v), sizeof v); };
@@ -347,7 +347,7 @@ bool add_key(std::string& k, PyObject* o, int depth) {
         put(t.dim());
         for (int64_t v : t.sizes()) put(v);
         for (int64_t v : t.strides()) put(v);
-        put((int64_t)t.scalar_type() << 32 | (int64_t)(uint8_t)t.device().type() << 16 | (uint16_t)t.device().index());
+        put((int64_t)t.is_neg() << 40 | (int64_t)t.scalar_type() << 32 | (int64_t)(uint8_t)t.device().type() << 16 | (uint16_t)t.device().index());
     } else if (PyUnicode_Check(o)) {
         Py_ssize_t n;
         const char* c = PyUnicode_AsUTF8AndSize(o, &n);

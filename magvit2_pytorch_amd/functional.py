@@ -26,7 +26,7 @@ __all__ = ['gate_loop', 'gate_loop_step', 'block_norm']
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 _ACTS = {'none': 0, 'silu': 2, 'sigmoid': 5}
 _backends = {}                       # device -> launcher (tests put the kernel emulation here for the CPU)
-_plans = {}                          # shapes, strides, types and devices of a call's arguments -> what follows from them
+_plans = {}                          # shapes, strides, types, devices and marks of a call's arguments -> what follows from them
 _MAX_PLANS = 1024
 
 
@@ -53,9 +53,9 @@ def _row_dtype(t, name):
 
 
 def _key(*args):
-    """what a plan depends on: shapes, strides, types and devices; None where arguments are not tensors (the plan says what is wrong).  On a HIP
+    """what a plan depends on: shapes, strides, types, devices and lazy negations; None where arguments are not tensors (the plan says what is wrong).  On a HIP
     device the native form of this takes its place (csrc/calls.cpp)"""
-    like = lambda t: t if t is None or isinstance(t, str) else (t.shape, t.stride(), t.dtype, t.device)
+    like = lambda t: t if t is None or isinstance(t, str) else (t.shape, t.stride(), t.dtype, t.device, t.is_neg())
     try:
         return tuple(tuple(map(like, a)) if isinstance(a, (tuple, list)) else like(a) for a in args)
     except (AttributeError, TypeError):
@@ -76,6 +76,11 @@ def _plan(key, make, *args):
 
 def _dense(t):
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _copied(t):
+    """dense, and with the sign that a lazily negated tensor (the imaginary part of a conjugate) only carries as a mark"""
+    return t if t is None else t.resolve_neg().contiguous()
 
 
 # ----------------------------------------------------------------------------------------------------------------- gated recurrence
@@ -120,7 +125,8 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
     plan.empty = B * P == 0                               # no sequences: nothing to launch
     if plan.empty:
         return plan
-    plan.copy = (first.stride(-1) != 1 and shape[-1] > 1) or any(t.stride() != first.stride() for t in parts)
+    plan.copy = (first.stride(-1) != 1 and shape[-1] > 1) or any(t.stride() != first.stride() for t in parts) or \
+        any(t is not None and t.is_neg() for t in (*parts, state))
     st = plan.stride = torch.empty(shape, device='meta').stride() if plan.copy else first.stride()
     row = (3 if fused else 1) * C                         # gradients: one dense (B, T, P, 3C) tensor, or three dense ones
     plan.desc = GateLoopDesc(dtype=dtype, B=B, T=T, P=P, C=C, in_b=st[0] if B > 1 else 0, in_t=st[1] if tokens and T > 1 else 0,
@@ -153,7 +159,7 @@ def gate_loop(qkva, *, state=None, lengths=None, resets=None, return_state=False
     if plan.empty:
         return _empty_loop(plan, leaves, state, return_state)
     if plan.copy:
-        leaves = tuple(t.contiguous() for t in leaves)
+        leaves, state = tuple(map(_copied, leaves)), _copied(state)
     if state is not None:
         state = _dense(state)
     if lengths is not None:
@@ -192,7 +198,7 @@ def gate_loop_step(qkva, state, *, state_out=None):
     if plan.empty:
         return parts[0].new_empty(plan.y_shape)
     if plan.copy:
-        parts = tuple(t.contiguous() for t in parts)
+        parts = tuple(map(_copied, parts))
     y = plan.forward(plan.native, parts, state, None, None, state_out, 0)[0]
     if not state_out.is_inference():                      # written behind autograd's back: what saved it must not use it any more
         torch.autograd.graph.increment_version(state_out)
@@ -202,10 +208,10 @@ def gate_loop_step(qkva, state, *, state_out=None):
 def _plan_step(qkva, state, state_out):
     _need(isinstance(state, torch.Tensor), 'gate_loop_step: state must be a tensor')
     plan = _plan_loop('gate_loop_step', qkva, False, state, None, None)
-    _need(state.is_contiguous(), 'gate_loop_step: the state is updated in place and must be dense')
+    _need(state.is_contiguous() and not state.is_neg(), 'gate_loop_step: the state is updated in place and must be dense')
     if state_out is not None:
         _check_state(state_out, plan.h_shape, state.device, 'gate_loop_step', 'state_out')
-        _need(state_out.is_contiguous(), 'gate_loop_step: state_out must be dense')
+        _need(state_out.is_contiguous() and not state_out.is_neg(), 'gate_loop_step: state_out must be dense')
     return plan
 
 
@@ -245,9 +251,9 @@ def _plan_norm(x, branch, gate, gate_act, *params):
         _need(t is None or (isinstance(t, torch.Tensor) and tuple(t.shape) == (C,) and t.is_floating_point() and t.device == dev),
               f'block_norm: {name} must be a floating-point ({C},) tensor on {dev}')
     plan.ops = _ops(dev)
-    plan.cast = any(t is not None and (t.dtype != torch.float32 or not t.is_contiguous()) for t in params)
+    plan.cast = any(t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.is_neg()) for t in params)
     steps = [None if t is None else _row_stride(t.shape, t.stride()) for t in (x, branch, gate)]
-    plan.copy = any(t is not None and s is None for t, s in zip((x, branch, gate), steps))
+    plan.copy = any(t is not None and (s is None or t.is_neg()) for t, s in zip((x, branch, gate), steps))
     if plan.copy:
         steps = [C, C, C]
     plan.strides = None if plan.copy else tuple(None if t is None else t.stride() for t in (x, branch, gate))      # None: all dense
@@ -274,9 +280,9 @@ def block_norm(x, branch=None, *, gate=None, gate_act='silu', post_gamma=None, s
     plan = _plan(_key('norm', x, branch, gate, gate_act, post_gamma, scale, pre_gamma), _plan_norm, x, branch, gate, gate_act, post_gamma, scale, pre_gamma)
     args = (x, branch, gate, post_gamma, scale, pre_gamma)
     if plan.copy:
-        args = tuple(None if t is None else t.contiguous() for t in args[:3]) + args[3:]
+        args = tuple(map(_copied, args[:3])) + args[3:]
     if plan.cast:
-        args = args[:3] + tuple(None if t is None else t.to(torch.float32).contiguous() for t in args[3:])
+        args = args[:3] + tuple(None if t is None else _copied(t.to(torch.float32)) for t in args[3:])
     train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)
     out, normed = plan.forward(plan.native, *args, train)
     return (out if plan.branch else x), normed

@@ -334,3 +334,9 @@ def test_an_empty_batch_keeps_its_graph(emulated, shape, fused):
     with torch.no_grad():
         assert not F.gate_loop(z, state=s).requires_grad
     assert not F.gate_loop(z.detach()).requires_grad
+
+
+def test_keys_tell_lazily_negated_tensors_apart():
+    native, t = ops_hip.load_calls().key, rnd(3, 4)
+    for key in (native, F._key):
+        assert key('norm', torch._neg_view(t)) != key('norm', t) and key('loop', (t, torch._neg_view(t), t)) != key('loop', (t, t, t))

@@ -948,3 +948,34 @@ def test_infinite_states_decay_as_token_by_token(T, C, dtype):
         assert torch.equal(kind(got), kind(want)), name
         rest = ~hit.cuda()[:, None, None].expand(got.shape)
         assert torch.equal(got[rest], res[1][name][rest]), name
+
+
+def test_lazily_negated_tensors():
+    """imaginary parts of conjugates carry their sign as a mark on the tensor; with one channel, or taken as they are, nothing else makes a copy of them"""
+    neg = lambda t: torch.complex(torch.zeros_like(t), -t.detach()).conj().imag
+    B, T, C = 2, 30, 4
+    parts, s, up = [rnd(B, T, C, seed=i).cuda() for i in range(3)], rnd(B, C, seed=3).cuda(), rnd(B, T, C, seed=4).cuda()
+    x, b, g = (rnd(9, C, seed=5 + i).cuda() for i in range(3))
+    w, fused = rnd(C, seed=9, mean=1.).cuda(), torch.cat(parts, -1)
+    for cut, lazy in ((slice(0, C), torch._neg_view), (slice(0, 1), neg)):
+        plain = lambda t: t[..., cut].detach().clone()
+        marked = lambda t: lazy(-plain(t)) if lazy is torch._neg_view else lazy(plain(t))
+        assert marked(x).is_neg() and torch.equal(marked(x), plain(x))
+        res = []
+        for f in (plain, marked):
+            q, kv, a, st, xx, bb, gg, ww = (f(t).requires_grad_() for t in (*parts, s, x, b, g, w))
+            y, h = F.gate_loop((q, kv, a), state=st, return_state=True)
+            out, n = F.block_norm(xx, bb, gate=gg, post_gamma=ww, scale=ww, pre_gamma=ww)
+            grads = torch.autograd.grad((y, h, out, n), (q, kv, a, st, xx, bb, gg, ww), (f(up), f(s), f(x), f(b)))
+            step = plain(s)
+            res.append([y, h, out, n, *grads, F.gate_loop_step(tuple(f(t[:, 0]) for t in parts), step), step, F.gate_loop(fused if f is plain else torch._neg_view(-fused))])
+        assert all(torch.equal(p, m) for p, m in zip(*res))
+    one = torch.zeros(1, 1, device='cuda')
+    for state, new in ((neg(one), None), (one, neg(one)), (torch._neg_view(one), None)):
+        with pytest.raises(ValueError):
+            F.gate_loop_step(torch.zeros(1, 3, device='cuda'), state, state_out=new)
+    z = parts[0][..., :3].clone().requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, torch._neg_view):
+        y = F.gate_loop(z)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
