@@ -765,11 +765,14 @@ static LoopArgs loop_args(const mv2_gateloop_desc* d, const int32_t* lengths, co
     return A;
 }
 
+// threads of a launch, and with them the words' indexes: 32 bits
+static bool span_fits(const SpanShape& s) { return (double)s.nblk * (s.ntile + 8) * 64 * SPAN_WAVES <= 4294967040.0; }
+
 // the pairs' words, cleared by a kernel (a captured memset would not do: the launch may be recorded into a graph)
 static int span_work(const mv2_gateloop_desc* d, bool fours, bool backward, void* workspace, size_t workspace_bytes, hipStream_t st, SpanWork& W, unsigned& grid) {
     const int nch = span_channels(fours);
     const SpanShape s = span_shape(d, nch, backward);
-    if ((double)s.nblk * (s.ntile + 8) * 64 * SPAN_WAVES > 4294967040.0) return MV2_ETOOLARGE;
+    if (!span_fits(s)) return MV2_ETOOLARGE;
     W.nblk = (int)s.nblk; W.ntile = (int)s.ntile; W.ctiles = (int)s.ctiles;
     W.nq = (int)s.nq;
     grid = (unsigned)(s.nblk > 1 ? s.nblk * s.nq * ((s.ntile + s.nq - 1) / s.nq) : s.ntile);
@@ -804,6 +807,8 @@ extern "C" int mv2_gateloop_forward(const mv2_gateloop_desc* d, const void* q, c
     } else {
         SpanWork W;
         unsigned grid;
+        // states are kept for a backward pass, whose blocks are shorter: it is refused here rather than after the forward pass
+        if (states && !span_fits(span_shape(d, span_channels(d->dtype == MV2_F32 && (int64_t)d->C * 4 >= 16), true))) return MV2_ETOOLARGE;
         rc = span_work(d, d->dtype == MV2_F32 && access, false, workspace, workspace_bytes, st, W, grid);
         if (rc != MV2_OK) return rc;
 #define GO(E, V, RAG, CL, CUTS, S) hipLaunchKernelGGL((loop_span_fwd_kernel<E, V, RAG, CL, SPAN_WAVES, 32, CUTS, S>), dim3(grid), dim3(64 * SPAN_WAVES), 0, st, A, W, q, kv, a, h0, y, h_last, states)

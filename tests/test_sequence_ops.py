@@ -340,3 +340,13 @@ def test_keys_tell_lazily_negated_tensors_apart():
     native, t = ops_hip.load_calls().key, rnd(3, 4)
     for key in (native, F._key):
         assert key('norm', torch._neg_view(t)) != key('norm', t) and key('loop', (t, torch._neg_view(t), t)) != key('loop', (t, t, t))
+
+
+def test_a_forward_pass_whose_backward_pass_is_too_long_is_refused():
+    """one sequence of 150 million tokens: served forward (as far as the launch), but its backward pass would have more workgroups than a launch can"""
+    lib, ptr = ops_hip.load_library(), ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)
+    T, C = 150_000_000, 8
+    d = ops_hip.GateLoopDesc(dtype=0, B=1, T=T, P=1, C=C, in_b=0, in_t=3 * C, in_p=0, grad_b=0, grad_t=3 * C, grad_p=0)
+    fwd = lambda states: lib.mv2_gateloop_forward(ctypes.byref(d), ptr, ptr, ptr, None, None, None, ptr, None, states, None, 0, None)
+    assert lib.mv2_gateloop_backward(ctypes.byref(d), *[ptr] * 3, None, None, None, ptr, ptr, None, *[ptr] * 3, None, None, 0, None) == ETOOLARGE
+    assert fwd(ptr) == ETOOLARGE and fwd(None) == EWORKSPACE
