@@ -54,7 +54,9 @@ typedef unsigned long long Marks __attribute__((aligned(1)));
 __device__ __forceinline__ unsigned long long eight_marks(const unsigned char* rs, int t, int T) {
     if (t + LOOP_STEPS <= T) return *(const Marks*)(rs + t);
     unsigned long long w = 0;
-    for (int s = 0; t + s < T; ++s) w |= (unsigned long long)rs[t + s] << 8 * s;
+#pragma unroll
+    for (int s = 0; s < LOOP_STEPS; ++s)
+        if (t + s < T) w |= (unsigned long long)rs[t + s] << 8 * s;
     return w;
 }
 __device__ __forceinline__ bool mark(unsigned long long w, int s) { return (unsigned)(w >> 8 * s) & 0xff; }

@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void codes_kernel(const CodesParams p) {
             code = ((float)lv - p.half_w[li]) / p.half_w[li];
         } else {
             const int64_t id = ((const int64_t*)p.ids)[row * p.ncb + cbk];
-            code = ((id >> (p.cb_dim - 1 - li)) & 1) ? p.scale : -p.scale;
+            code = ((unsigned)id >> (p.cb_dim - 1 - li) & 1) ? p.scale : -p.scale;      // cb_dim <= CB_MAX: the low half holds every bit
         }
         scode[wave][lane] = code;
     }

@@ -2,7 +2,7 @@
 //   RowVec<E, kVec>        16-byte chunks of rows, strides and addresses that are whole such chunks
 //   RowVec<E, kVec, true>  ragged: 16-byte accesses at any element (the memory pipe takes them at the same rate: a copy of 256 MB runs at
 //                          5.7 - 6.0 TB/s whatever the offsets); a row's last chunk holds nv < V elements and is read as the row's last V
-//                          elements, moved down, with zeros behind them, and written one by one.  Rows of V elements at least.
+//                          elements, moved down, with zeros behind them, and written in pieces of 8, 4 and 2 bytes.  Rows of V elements at least.
 //   V = kVec / 2           half of either, for kernels that hold many rows in registers
 //   V = 1                  single elements: rows shorter than a chunk, and kernels whose every wave would hold a row's end
 // STREAM: past the caches, for calls that move more than the last-level cache holds (calls_stream).
@@ -16,7 +16,8 @@ template <> struct RowBits<8> { typedef i32x2 T; typedef i32x2 __attribute__((al
 typedef int __attribute__((aligned(2))) RowWord;
 
 // N words moved down by `bytes` (of 4 N; whole words, or half words too if HALVES), zeros behind them.  By selects: written as one wide shift this
-// becomes 64-bit shifts by a variable amount, and with the amount in a wave's last register those have given wrong results here.
+// becomes 64-bit shifts by a variable amount, and with the amount in a wave's last register those have given wrong results here (tools/check_spills.sh
+// counts them: no kernel of the library holds one with its amount in a vector register).
 template <int N, bool HALVES, typename W> __device__ __forceinline__ W moved_down(W v, int bytes) {
 #pragma unroll
     for (int d = 1; d < N; d *= 2) {

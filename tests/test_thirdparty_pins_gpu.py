@@ -282,3 +282,19 @@ def test_two_rank_rccl_smoke():
     assert run.returncode == 0, run.stderr[-2000:]
     line = json.loads(run.stdout.strip().splitlines()[-1])
     assert line['n_gpus'] == 2 and line['value'] > 0 and line['scaling'] == 'weak' and len(line['per_rank_ms_per_step']) == 2
+
+
+@pytest.mark.parametrize('d,ncb', [(32, 1), (31, 1), (16, 2), (1, 3)])
+def test_lfq_codes_of_wide_ids(d, ncb):
+    """ids of up to 32 bits, the topmost among them"""
+    ops, C, n = _ops(), 32, 37
+    dev, st = ops.device, ops.current_stream()
+    ids = torch.randint(0, 1 << d, (n, ncb), generator=torch.Generator().manual_seed(d))
+    ids[0], ids[1] = 0, (1 << d) - 1
+    sel = torch.eye(C)[:d * ncb].contiguous().to(dev)
+    for dt, t in ((P.MV2_F32, torch.float32), (P.MV2_BF16, torch.bfloat16)):
+        out = torch.empty(n * C, dtype=t, device=dev)
+        ops.lfq_codes(dt, ids.to(dev), sel, torch.zeros(C, device=dev), out, n, C, d, ncb, 0.5)(st)
+        ops.synchronize()
+        bits = (ids[:, :, None] >> (d - 1 - torch.arange(d))) & 1
+        assert torch.equal(out.reshape(n, C)[:, :d * ncb].cpu().float(), (bits.reshape(n, -1) * 2 - 1) * 0.5)
