@@ -33,6 +33,7 @@ NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # the native calls of functional.py: host code over torch's C++ interface, linked with the library
 CALLS = os.path.join(HERE, '_calls.so')
 CALLS_SRC = os.path.join(CSRC, 'calls.cpp')
+CALLS_FOR = os.path.join(OBJ, 'calls.for')          # the interfaces that _calls.so was built against
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result', *NO_PACKED_FP32]
 
 
@@ -84,21 +85,36 @@ def build(force=False, verbose=True, experiments=False):
             raise RuntimeError(f'link failed:\n{r.stdout}\n{r.stderr}')
         if verbose:
             print(f'[mv2 build] linked {lib}', flush=True)
-    if not experiments and (force or _stale(CALLS, [CALLS_SRC, HEADERS[-1]])):
+    if not experiments and (force or _calls_stale()):
         _build_calls(verbose)
     return lib
+
+
+def _interfaces():
+    import torch
+    return f'torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}'
+
+
+def _calls_stale():
+    """older than its sources, or built against another torch or Python (whose files may be older than it)"""
+    if _stale(CALLS, [CALLS_SRC, HEADERS[-1]]) or not os.path.exists(CALLS_FOR):
+        return True
+    with open(CALLS_FOR) as f:
+        return f.read() != _interfaces()
 
 
 def _build_calls(verbose):
     import torch
     root = os.path.dirname(torch.__file__)
-    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
+    cmd = ['g++', '-O2', f'-DMV2_BUILT_FOR="{_interfaces()}"', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{sysconfig.get_paths()["include"]}', f'-I{root}/include', f'-I{root}/include/torch/csrc/api/include',
            f'-I{os.environ.get("ROCM_PATH", "/opt/rocm")}/include', CALLS_SRC, '-o', CALLS, f'-L{root}/lib', '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip',
            f'-L{HERE}', f'-l:{os.path.basename(LIB)}', '-Wl,-rpath,$ORIGIN']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f'g++ failed for {CALLS_SRC}:\n{r.stdout}\n{r.stderr}')
+    with open(CALLS_FOR, 'w') as f:
+        f.write(_interfaces())
     if verbose:
         print(f'[mv2 build] linked {CALLS}', flush=True)
 

@@ -384,4 +384,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__calls() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__calls() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", MV2_BUILT_FOR) < 0) Py_CLEAR(m);      // ops_hip.py compares it with what is running
+    return m;
+}

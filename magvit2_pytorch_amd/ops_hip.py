@@ -152,8 +152,16 @@ def load_calls():
         if not os.path.exists(CALLS_PATH):
             raise Mv2Error(f'{CALLS_PATH} not built: run `python -m magvit2_pytorch_amd.build`')
         spec = importlib.util.spec_from_file_location('magvit2_pytorch_amd._calls', CALLS_PATH)
-        calls = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(calls)
+        again = 'run `python -m magvit2_pytorch_amd.build`'
+        try:
+            calls = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(calls)
+        except ImportError as e:                     # a symbol of another torch
+            raise Mv2Error(f'{CALLS_PATH} does not load, {again}: {e}') from e
+        from .build import _interfaces
+        here = _interfaces()
+        if calls.built_for != here:
+            raise Mv2Error(f'{CALLS_PATH} was built for {calls.built_for}, this is {here}: {again}')
         calls.set_error(Mv2Error)
         _calls = calls
     return _calls

@@ -350,3 +350,27 @@ def test_a_forward_pass_whose_backward_pass_is_too_long_is_refused():
     fwd = lambda states: lib.mv2_gateloop_forward(ctypes.byref(d), ptr, ptr, ptr, None, None, None, ptr, None, states, None, 0, None)
     assert lib.mv2_gateloop_backward(ctypes.byref(d), *[ptr] * 3, None, None, None, ptr, ptr, None, *[ptr] * 3, None, None, 0, None) == ETOOLARGE
     assert fwd(ptr) == ETOOLARGE and fwd(None) == EWORKSPACE
+
+
+def test_calls_of_another_torch_are_built_anew_and_never_used(monkeypatch, tmp_path):
+    """_calls.so holds torch's C++ interface as it was when it was built: after torch is replaced it is stale, whatever its age, and is not loaded"""
+    from magvit2_pytorch_amd import build
+    stamp = tmp_path / 'calls.for'
+    stamp.write_text(build._interfaces())
+    with monkeypatch.context() as m:
+        m.setattr(build, '_stale', lambda *a: False)
+        m.setattr(build, 'CALLS_FOR', str(stamp))
+        assert not build._calls_stale()
+        m.setattr(torch, '__version__', '9.9.9')
+        assert build._calls_stale()
+        m.setattr(ops_hip, '_calls', None)
+        with pytest.raises(Mv2Error, match='9.9.9'):
+            ops_hip.load_calls()
+    broken = tmp_path / '_calls.so'
+    broken.write_bytes(b'not a library')
+    with monkeypatch.context() as m:
+        m.setattr(ops_hip, '_calls', None)
+        m.setattr(ops_hip, 'CALLS_PATH', str(broken))
+        with pytest.raises(Mv2Error, match='does not load'):
+            ops_hip.load_calls()
+    assert ops_hip.load_calls().built_for == build._interfaces()
