@@ -12,6 +12,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -86,7 +87,13 @@ def build(force=False, verbose=True, experiments=False):
         if verbose:
             print(f'[mv2 build] linked {lib}', flush=True)
     if not experiments and (force or _calls_stale()):
-        _build_calls(verbose)
+        try:
+            _build_calls(verbose)
+        except (OSError, RuntimeError) as e:         # no g++, no headers: the library stands by itself, only functional.py needs the calls
+            for f in (CALLS, CALLS_FOR):
+                if os.path.exists(f):
+                    os.remove(f)                     # an older one would be taken for this one
+            warnings.warn(f'{os.path.basename(CALLS)} was not built, magvit2_pytorch_amd.functional will not work: {e}')
     return lib
 
 
@@ -106,7 +113,7 @@ def _calls_stale():
 def _build_calls(verbose):
     import torch
     root = os.path.dirname(torch.__file__)
-    cmd = ['g++', '-O2', f'-DMV2_BUILT_FOR="{_interfaces()}"', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
+    cmd = [os.environ.get('CXX', 'g++'), '-O2', f'-DMV2_BUILT_FOR="{_interfaces()}"', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{sysconfig.get_paths()["include"]}', f'-I{root}/include', f'-I{root}/include/torch/csrc/api/include',
            f'-I{os.environ.get("ROCM_PATH", "/opt/rocm")}/include', CALLS_SRC, '-o', CALLS, f'-L{root}/lib', '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip',
            f'-L{HERE}', f'-l:{os.path.basename(LIB)}', '-Wl,-rpath,$ORIGIN']

@@ -374,3 +374,17 @@ def test_calls_of_another_torch_are_built_anew_and_never_used(monkeypatch, tmp_p
         with pytest.raises(Mv2Error, match='does not load'):
             ops_hip.load_calls()
     assert ops_hip.load_calls().built_for == build._interfaces()
+
+
+def test_the_library_is_built_without_the_calls(monkeypatch, tmp_path):
+    """no g++ here: only functional.py needs it, so the build goes on, says so, and leaves no older calls behind"""
+    from magvit2_pytorch_amd import build
+    old = [tmp_path / n for n in ('_calls.so', 'calls.for')]
+    for f in old:
+        f.write_text('older')
+    monkeypatch.setattr(build, 'CALLS', str(old[0]))
+    monkeypatch.setattr(build, 'CALLS_FOR', str(old[1]))
+    monkeypatch.setenv('CXX', str(tmp_path / 'no-such-compiler'))
+    with pytest.warns(UserWarning, match='functional'):
+        assert build.build(verbose=False) == build.LIB
+    assert not any(f.exists() for f in old)
