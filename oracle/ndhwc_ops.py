@@ -18,8 +18,6 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from magvit2_pytorch_amd import functional as F
-
 ACT_NONE, ACT_ELU, ACT_SILU, ACT_GEGLU, ACT_LRELU = 0, 1, 2, 3, 4
 STORE_ROWS, STORE_SHUFFLE, STORE_NCTHW_F32, STORE_ROWS_F32 = 0, 1, 2, 3
 
@@ -985,16 +983,18 @@ class _EmulatedLoop(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dh):
         state, lengths, resets, states, *qkva = ctx.saved_tensors
-        plan, ops = ctx.plan, ctx.plan.ops
+        plan, ops, d = ctx.plan, ctx.plan.ops, ctx.plan.desc
         if any(t.stride() != plan.stride for t in qkva):      # hooks on saved tensors may lay them out anew
             qkva = [t.contiguous() for t in qkva]
-            plan = F._plan_loop('gate_loop', qkva[0] if plan.fused else qkva, True, state, lengths, resets)
+            row = (3 if plan.fused else 1) * d.C
+            d = type(d).from_buffer_copy(d)
+            d.in_b, d.in_t, d.in_p = d.T * d.P * row, d.P * row, row
         if dy is None and dh is None:
             return (None,) * (4 + len(qkva))
         dy = torch.zeros(plan.y_shape, dtype=qkva[0].dtype) if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         grads, dstate = tuple(torch.empty(t.shape, dtype=t.dtype) for t in qkva), torch.empty(plan.h_shape) if ctx.needs_input_grad[3] else None
-        ops.gateloop_backward(plan.desc, *ops.loop_parts(plan, qkva), state, lengths, resets, states, dy, dh, *ops.loop_parts(plan, grads), dstate, None)(0)
+        ops.gateloop_backward(d, *ops.loop_parts(plan, qkva), state, lengths, resets, states, dy, dh, *ops.loop_parts(plan, grads), dstate, None)(0)
         return (None, None, None, dstate) + grads
 
 
@@ -1013,13 +1013,14 @@ class _EmulatedNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dn):
-        plan, saved, want = ctx.plan, ctx.saved_tensors, ctx.needs_input_grad[1:]
+        plan, d, saved, want = ctx.plan, ctx.plan.desc, ctx.saved_tensors, ctx.needs_input_grad[1:]
         if any(t is not None and (not t.is_contiguous() if plan.strides is None else t.stride() != plan.strides[i]) for i, t in enumerate(saved[:3])):
             saved = tuple(None if t is None else t.contiguous() for t in saved)      # hooks on saved tensors may lay them out anew
-            plan = F._plan_norm(*saved[:3], {0: 'none', 2: 'silu', 5: 'sigmoid'}[plan.desc.gate_act], *saved[3:6])
+            d = type(d).from_buffer_copy(d)
+            d.x_stride = d.branch_stride = d.gate_stride = d.C
         if dout is None and dn is None:
             return (None,) * 7
         grads = [torch.empty(plan.shape, dtype=saved[0].dtype) if w else None for w in want[:3]] + [torch.empty(plan.desc.C) if w else None for w in want[3:]]
         dout, dn = (None if g is None else g.contiguous() for g in (dout, dn))
-        plan.ops.block_norm_backward(plan.desc, *saved, dout, dn, *grads, None)(0)
+        plan.ops.block_norm_backward(d, *saved, dout, dn, *grads, None)(0)
         return (None, *grads)
