@@ -1,6 +1,7 @@
 """The sequence operators (gated recurrence, block norms) on the GPU against the 64-bit references of tests/_sequence_ref.py, within the
 running error bounds derived there."""
 import contextlib
+import math
 
 import pytest
 import torch
@@ -979,3 +980,61 @@ def test_lazily_negated_tensors():
         y = F.gate_loop(z)
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+BF, FP = DT
+
+
+@pytest.mark.parametrize('R,C,dtype', [(4097, 501, FP), (4097, 1001, BF), (4099, 1001, FP), (4097, 2048, BF), (4097, 768, FP), (2049, 1024, FP), (131073, 3, BF), (131073, 3, FP),
+                                       (65537, 5, BF), (262145, 5, FP), (262145, 9, BF)])
+def test_block_norm_of_many_rows(R, C, dtype):
+    """rows taken two at a time (from 2048 turns of a workgroup's rows on), the last turn with one row or none in the second place: whole chunks, ragged
+    ones and single elements, every part and the plain add and norm"""
+    check_norm(R, C, dtype)
+    check_norm(R, C, dtype, branch=False)
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('R,C', [(131073, 4), (262145, 9), (4097, 784), (4097, 961), (5000, 2025), (60001, 256), (60001, 729), (3000, 2304), (1023, 5041), (257, 16384), (5, 784), (300, 961)])
+def test_column_sums_are_exact_where_every_term_is(R, C, dtype):
+    """parameter gradients to the last row: widths that are squares, rows of 4^j numbers +-1 and gradients of small whole numbers make every term and every
+    partial sum of them exact in 32 bits, in any order, so the sums have to be equal"""
+    gen = torch.Generator('cuda').manual_seed(R + C)
+    few = 4 ** int(math.log(C, 4))
+    v = torch.zeros(R, C, device='cuda')
+    at = torch.rand(R, C, device='cuda', generator=gen).topk(few, -1).indices
+    v.scatter_(1, at, torch.randint(0, 2, (R, few), device='cuda', generator=gen) * 2. - 1)
+    up = torch.randint(-2, 3, (R, C), device='cuda', generator=gen).float()
+    norm, root = few ** 0.5, round(C ** 0.5)
+    assert (v.square().sum(-1) == few).all() and root * root == C
+    sums = (v.double() * up.double()).sum(0)
+    x, d = v.to(dtype), up.to(dtype)
+    w = torch.ones(C, device='cuda', requires_grad=True)
+    zero = torch.zeros_like(x)
+    for call, want in ((lambda: F.block_norm(x, pre_gamma=w)[1], sums * root / norm), (lambda: F.block_norm(zero, x, post_gamma=w)[0], sums * root / norm),
+                       (lambda: F.block_norm(zero, x, scale=w)[0], sums)):
+        assert torch.equal(torch.autograd.grad(call(), w, d)[0].double(), want)
+
+
+def test_a_step_over_a_saved_state_is_noticed():
+    q, s = rnd(2, 3, 12).cuda().requires_grad_(), torch.ones(2, 4, device='cuda')
+    y = F.gate_loop(q, state=s)
+    F.gate_loop_step(rnd(2, 12, seed=1).cuda(), s)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    y, other = F.gate_loop(q, state=s), torch.ones(2, 4, device='cuda')
+    y2 = F.gate_loop(q, state=other)
+    F.gate_loop_step(rnd(2, 12, seed=1).cuda(), s, state_out=other)      # the state is read, its other buffer written
+    y.sum().backward()
+    with pytest.raises(RuntimeError):
+        y2.sum().backward()
+
+
+def test_bf16_parameters_get_bf16_gradients():
+    x, w = rnd(4, 8).cuda().requires_grad_(), [torch.full((8,), 1.5, device='cuda', dtype=t, requires_grad=True) for t in (torch.bfloat16, torch.float32)]
+    g = [torch.autograd.grad(F.block_norm(x, x, post_gamma=p, scale=p, pre_gamma=p), p, (x.detach(), x.detach()))[0] for p in w]
+    assert g[0].dtype == torch.bfloat16
+    # three sums, each rounded to bf16, and two sums of those: 5 half steps of the largest partial result; the sums' own size bounds it for like signs
+    parts = [torch.autograd.grad(F.block_norm(x, x, **{'post_gamma': w[1].detach(), 'scale': w[1].detach(), 'pre_gamma': w[1].detach(), k: w[1]}), w[1], (x.detach(), x.detach()))[0]
+             for k in ('post_gamma', 'scale', 'pre_gamma')]
+    assert ((g[0].float() - g[1]).abs() <= 5 * 2.0 ** -8 * sum(p.abs() for p in parts)).all()
