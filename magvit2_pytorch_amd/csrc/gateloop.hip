@@ -227,12 +227,10 @@ __device__ __forceinline__ float pair_A(u64 w) { return __uint_as_float((unsigne
 __device__ __forceinline__ float pair_H(u64 w) { return __uint_as_float((unsigned)w); }
 __device__ __forceinline__ void publish(u64* p, float A, float H) { __hip_atomic_store(p, pair_word(A, H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// A of two spans.  It stays above 0 where both are: a product below the smallest number, 1.4e-45, becomes that number (no further off than the rounding
-// of any product down there), so that an infinite state stays infinite as it does token by token; a decay of exactly 0 makes it NaN in either form.
-// The bits of numbers that are not negative are ordered as the numbers are, NaN highest: it stays.
-__device__ __forceinline__ float spans_decay(float A, float A2) {
-    return __uint_as_float(max(__float_as_uint(A * A2), min(min(__float_as_uint(A), __float_as_uint(A2)), 1u)));
-}
+// A of joined spans stays above 0 where all of theirs are (low: the least of them, as bits): a product below the smallest number, 1.4e-45, becomes that
+// number (no further off than the rounding of any product down there), so that an infinite state stays infinite as it does token by token; a decay of
+// exactly 0 makes it NaN in either form.  The bits of numbers that are not negative are ordered as the numbers are, NaN highest: it stays.
+__device__ __forceinline__ float above_zero(float A, unsigned low) { return __uint_as_float(max(__float_as_uint(A), min(low, 1u))); }
 // the same for the product of a lane's L decays, g(i, k) of channel k: looked at again only where one came out as 0
 template <int L, int V, typename G> __device__ __forceinline__ void lane_decay(float (&pa)[V], G g) {
     unsigned least = __float_as_uint(pa[0]);
@@ -244,7 +242,7 @@ template <int L, int V, typename G> __device__ __forceinline__ void lane_decay(f
             unsigned low = 1;
 #pragma unroll
             for (int i = 0; i < L; ++i) low = min(low, __float_as_uint(g(i, k)));
-            pa[k] = __uint_as_float(max(__float_as_uint(pa[k]), low));
+            pa[k] = above_zero(pa[k], low);
         }
 }
 
@@ -253,11 +251,17 @@ template <bool CUTS> __device__ __forceinline__ float pass(float A, float H, flo
     const float r = fmaf(A, h, H);
     return CUTS && A == LOOP_CUT ? H : r;
 }
-// (A, H) := (A, H) then (A2, H2)
-template <bool CUTS> __device__ __forceinline__ void join(float& A, float& H, float A2, float H2) {
+// (A, H) := (A, H) then (A2, H2).  A run of spans keeps the least A on the way and looks at the product at its end (above_zero): one step of a chain less.
+template <bool CUTS> __device__ __forceinline__ void join(float& A, float& H, float A2, float H2, unsigned& low) {
     H = pass<CUTS>(A2, H2, H);
-    const float r = spans_decay(A, A2);
+    low = min(low, __float_as_uint(A2));
+    const float r = A * A2;
     A = CUTS && (A == LOOP_CUT || A2 == LOOP_CUT) ? LOOP_CUT : r;
+}
+template <bool CUTS> __device__ __forceinline__ void join(float& A, float& H, float A2, float H2) {
+    unsigned low = __float_as_uint(A);
+    join<CUTS>(A, H, A2, H2, low);
+    A = above_zero(A, low);
 }
 
 // Tiles are dealt to `nq` queues of neighbours, workgroup i draws from queue i % nq: with 8 queues neighbouring tiles, which share cache lines
@@ -364,11 +368,13 @@ __device__ __forceinline__ void span_join(const SpanWork& W, int kb, int tile, b
     constexpr int RPS = ROWS / SEGS;
     const int ch = threadIdx.x % NCH, seg = threadIdx.x / NCH;
     float A = 1.f, H = 0.f;
+    unsigned low = 1;
 #pragma unroll
     for (int j = 0; j < RPS; ++j) {
         const int r = REV ? ROWS - 1 - (seg * RPS + j) : seg * RPS + j;
-        join<CUTS>(A, H, rowA[r][ch], rowH[r][ch]);
+        join<CUTS>(A, H, rowA[r][ch], rowH[r][ch], low);
     }
+    A = above_zero(A, low);
     partA[seg][ch] = A; partH[seg][ch] = H;
     __syncthreads();
     float fa = 1.f, fh = 0.f;                                 // everything in front of this segment
@@ -603,12 +609,13 @@ __global__ __launch_bounds__(WAVES * 64, 4) void loop_span_bwd_kernel(LoopArgs A
     __syncthreads();
     {   // states in front of the lane rows: from the kept state
         float ra[RPS], rh[RPS], pA = 1.f, pH = 0.f;
+        unsigned low = 1;
 #pragma unroll
         for (int j = 0; j < RPS; ++j) {
             ra[j] = rowA[seg * RPS + j][chn]; rh[j] = rowH[seg * RPS + j][chn];
-            join<CUTS>(pA, pH, ra[j], rh[j]);
+            join<CUTS>(pA, pH, ra[j], rh[j], low);
         }
-        prevA[seg][chn] = pA; prevH[seg][chn] = pH;
+        prevA[seg][chn] = above_zero(pA, low); prevH[seg][chn] = pH;
         __syncthreads();
         float h = hin;
         for (int s = 0; s < seg; ++s) h = pass<CUTS>(prevA[s][chn], prevH[s][chn], h);
