@@ -12,8 +12,10 @@
 //     69632 x 256 bf16, add and norm forward 25 (5.7, part of it from the last-level cache), backward 40 (4.4)
 //     65536 x 512 bf16               forward 62 (5.4), backward 109 (4.9)        8192 x 2048 fp32  forward 60 (5.6), backward 100 (5.4)
 //     16384 x 1001 bf16, ragged      forward 41 (4.0), backward 79 (3.3)         4097 x 501 fp32   forward 14, backward 23
-//     6250 x 5120 bf16               forward 64 (5.0), backward 180 (2.8)        6251 x 5119 bf16, ragged  88 (3.6), 228 (2.2)
-// Forward it is the memory; backward also the 160 to 200 registers, which leave two or three waves on a SIMD.  32 rows take 5 us: latency.
+//     6250 x 5120 bf16               forward 67 (4.8), backward 177 (2.9)        6251 x 5119 bf16, ragged  90 (3.6), 225 (2.3)
+//     2000 x 16384 bf16              forward 73 (4.5), backward 265 (2.0)
+// Forward it is the memory; backward also the 160 to 200 registers, which leave two or three waves on a SIMD, and beyond 8192 wide, where 1024 threads
+// have 128 registers each, the spills (bf16 157, ragged 212; fp32 185, ragged 306, and 189 in its ragged forward kernel; tools/check_spills.sh).  32 rows take 5 us: latency.
 #include <algorithm>
 #include <initializer_list>
 #include "rowvec.h"
@@ -96,7 +98,7 @@ template <int NC, int V> struct Params {
     }
 };
 
-// (four waves on a SIMD: ragged rows of 3999 bf16 84 us, 103 with the 132 registers that the compiler would take)
+// (four waves on a SIMD: up to 128 registers; without the bound the compiler takes at most one more in any shape)
 template <typename E, int V, bool RAG, int NC, int R, int BLOCK, bool S>
 __global__ __launch_bounds__(BLOCK, 4) void block_norm_fwd_kernel(NormArgs A, int G, const void* x, const void* __restrict__ branch, const void* __restrict__ gate,
                                                                const float* __restrict__ w1, const float* __restrict__ sc, const float* __restrict__ w2,
@@ -408,7 +410,8 @@ __global__ __launch_bounds__(512) void block_norm_cols_kernel(const float* __res
 }
 
 // --------------------------------------------------------------------------- host side
-#define NORM_R 2                   // rows at a time, one chunk per thread: 16384 x 2048 bf16 73 us forward and 126 backward, one row 75 and 147, four 91 and 188
+#define NORM_R 2                   // rows at a time, one chunk per thread: 16384 x 2048 bf16 65 us forward and 118 backward, one row 69 and 118, four 119 and 245;
+                                   // 65536 x 512 62 and 109, one row 68 and 112
 #define NORM_GROUPS 1024           // workgroups from which on rows are taken NORM_R at a time
 #define NORM_BWD_MOST 768          // workgroups of a backward pass at most
 static int norm_check(const mv2_block_norm_desc* d) {
@@ -424,8 +427,8 @@ static int norm_check(const mv2_block_norm_desc* d) {
 
 // threads per row G, chunks per thread NC, rows at a time R: the row's chunks spread over up to 256 threads first, then over two registers, then over
 // up to 1024 threads (and four registers); R > 1 once every workgroup of a full chip has that many rows.  Rows of more than 256 chunks take as many
-// whole waves as they fill (6250 x 5120 bf16 64 us forward, 75 with a power of two), but a power of two backward, where the registers leave one
-// workgroup on a CU either way (184 and 180)
+// whole waves as they fill (6250 x 5120 bf16 67 us forward, 70 with a power of two; ragged 6251 x 5119 90 and 96), but a power of two backward, where the
+// registers leave one workgroup on a CU either way (177 us, whole waves 180; ragged 225 and 239)
 struct NormShape { int access, NC, R, block, G; bool stream; };
 static NormShape norm_shape(const mv2_block_norm_desc* d, int access, int tensors, bool backward) {
     const int es = d->dtype == MV2_BF16 ? 2 : 4, V = access ? 16 / es : 1, nch = (d->C + V - 1) / V;
@@ -452,8 +455,8 @@ static unsigned norm_grid(const mv2_block_norm_desc* d, const NormShape& s, int6
 }
 
 // Workgroups of the backward pass: each leaves 3 C partial column sums, so two turns of the loop at least (1000 x 2048 bf16 25 us, one turn 28;
-// 4097 x 501 fp32 26 us, three turns 32), and no more than the chip holds at once by the registers of the shapes (up to 168 with two rows of
-// one 16-byte chunk, 200 with one row of two; 16384 x 2048 bf16 126 us with 768, 140 with 512; 8000 x 2048 70 with 768, 77 with 1280).
+// 4097 x 501 fp32 26 us, three turns 32, one 25), and no more than the chip holds at once by the registers of the shapes (up to 168 with two rows of
+// one 16-byte chunk, 200 with one row of two; 16384 x 2048 bf16 118 us with 768, 126 with 512, 132 with 1280; 8000 x 2048 70, 72, 78).
 static int64_t norm_bwd_grid(const mv2_block_norm_desc* d, const NormShape& s) {
     const int64_t most = s.block > 256 ? 256 : s.NC == 1 ? NORM_BWD_MOST : 512;
     return std::min(most, std::max<int64_t>(256, d->rows / ((int64_t)s.block / s.G * s.R) / 2));
@@ -472,7 +475,7 @@ static NormArgs norm_args(const mv2_block_norm_desc* d) {
 }
 
 // one launch of KERNEL<E, V, RAGGED, NC, R, BLOCK, S> for the shape; S, past the caches: where the call is large, and always at widths beyond 512 chunks
-// (a row of a thousand and more threads: 2000 x 16384 81 us forward, 95 through the caches)
+// (a row of a thousand and more threads: 2000 x 16384 73 us forward, 78 through the caches)
 #define NORM_CASES(KERNEL, ...)                                                                                   \
     do {                                                                                                          \
         if (d->dtype == MV2_BF16) { NORM_ACCESS(KERNEL, BF16, 8, __VA_ARGS__) }                                   \
@@ -505,7 +508,7 @@ extern "C" int mv2_block_norm_forward(const mv2_block_norm_desc* d, const void* 
     const NormShape s = norm_shape(d, access, 1 + !!branch * 2 + !!gate + !!pre_gamma, false);
     const NormArgs A = norm_args(d);
     // as many workgroups as the chip holds at once: 4 waves on a SIMD by the registers of the shapes, 6 of those of aligned fp32 chunks (6250 x 5120
-    // bf16 64 us with 512 workgroups of 5 waves, 82 with 768; 16384 x 2048 71, 73 with twice as many)
+    // bf16 67 us with 512 workgroups of 5 waves, 84 with 768; 16384 x 2048 65, and 65 with twice as many)
     const int held = s.NC > 1 && d->dtype == MV2_F32 && access == 2 ? 6 : 4;
     const unsigned grid = norm_grid(d, s, 256 * std::max(1, held / ((s.block + 255) / 256)));
     hipStream_t st = (hipStream_t)stream;

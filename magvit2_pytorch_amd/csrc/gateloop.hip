@@ -6,11 +6,12 @@
 // One or two flops a byte: the work is to read every element once (4 tensors forward, 7 backward) and to keep the chip's memory busy.  A copy of
 // 256 MB in 16-byte accesses runs at 5.9 TB/s.  Measured on one MI355X, us and TB/s of those tensors, kernels alone:
 //     walks   4 x 17 tokens x 1024 x 256 bf16       forward 25 (5.7; part of it from the last-level cache), backward 52 (4.8)
-//     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 95 (4.9); with document starts 55 and 103
-//             1 x 131072 x 512 bf16                 forward 106 (5.1), backward 193 (4.9); 1 x 100000 x 64 23 and 35
-//             6 x 4095 x 1000 bf16, rows off lines  forward 53 (3.7), backward 94 (3.7)
-//             3 x 1023 x 777 fp32                   forward 13, backward 17 (9.5 MB a tensor: as much latency as bandwidth)
-// and 2.5 us for a single token of 512 channels, 4.3 us for one of 192 x 2048, where launch and load latency are all there is.
+//     spans   8 x 2048 x 2048 bf16                  forward 55 (4.9), backward 96 (4.9); with document starts 54 and 105
+//             1 x 131072 x 512 bf16                 forward 106 (5.1), backward 193 (4.9); 1 x 100000 x 64 23 and 36
+//             6 x 4095 x 1000 bf16, rows off lines  forward 53 (3.7), backward 92 (3.7)
+//             16 x 60000 x 16 bf16                  forward 70 (1.8), backward 137 (1.6): two lanes of a row's eight hold data
+//             3 x 1023 x 777 fp32                   forward 14, backward 18 (9.5 MB a tensor: as much latency as bandwidth)
+// and 2.6 us for a single token of 512 channels, 4.4 us for one of 192 x 2048, where launch and load latency are all there is.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(256) void loop_walk_bwd_kernel(LoopArgs A, const vo
 // Between workgroups: a block publishes its pair and reads the pairs of the blocks before it in its group; the last block of a group publishes
 // the group's pair, and groups are joined likewise in sets, whose last block publishes the state behind the set.  A block reads at most 7 pairs,
 // 7 groups' pairs and one state, always the same in the same order, so results do not depend on timing, and states are handed on once every 64
-// blocks.  bf16, us forward / backward: 1 x 100000 x 64 23 / 35, states handed on from group to group of 16 blocks 36 / 58 (1 x 131072 x 512 108 / 193
+// blocks.  bf16, us forward / backward, measured in turn: 1 x 100000 x 64 23 / 35, states handed on from group to group of 16 blocks 36 / 58 (1 x 131072 x 512 108 / 193
 // and 107 / 188); groups and sets of 16 21 / 34, but every block reads twice as much: 16 x 60000 x 16 68 / 140 against 65 / 136.
 // Every wait ends: a block's place in the order is the ticket it draws when it starts, blocks wait for lower tickets only - for workgroups
 // that are running; a block's pair is published before it waits for anything, a group's before its block waits for other groups.
@@ -701,13 +702,14 @@ static int loop_check(const mv2_gateloop_desc* d) {
 // Which form runs: one thread per chunk where the tokens are few for that many channels, spans otherwise.  A function of the sizes alone (the
 // backward pass finds the states that the forward pass kept), counted in the spans' tiles of 8 chunks, which rows shorter than a tile leave partly
 // empty.  A walk takes 0.35 us a token (backward 0.65) until the memory is busy, a span of up to 256 tokens some 5 us and as much again for every 512
-// (256) tiles.  Above 8192 tiles walks reach the memory's rate at any length.  Measured, bf16, us forward / backward, walk : span:
-//     64 tiles, 8 tokens 4.8 / 6.9 : 5.2 / 5.8        16 tokens 7.2 / 12 : 5.2 / 5.8
-//   2048 tiles, 40 tokens 16 / 31 : 22 / 27           48 tokens 18 / 37 : 23 / 27
-//   6144 tiles, 96 tokens 55 / 131 : 71 / 118         200 tokens 108 / 270 : 132 / 245
-//   8192 tiles, 192 tokens 136 / 285 : 156 / 320      1024 tokens 741 / 1516 : 874 / 1539
-//   4096 rows of 8 channels, 40 tokens 15 / 29 : 39 / 48, 200 tokens 58 / 142 : 48 / 120
-//  16384 rows of 5 channels, 200 tokens 44 / 161 : 445 / 589, 1000 tokens 291 / 1177 : 2092 / 2665
+// (256) tiles.  Above 8192 tiles walks are near the memory's rate at any length.  Measured, bf16, us forward / backward, walk : span:
+//     64 tiles, 8 tokens 4.8 / 6.1 : 5.2 / 5.9        16 tokens 7.0 / 10 : 5.2 / 5.8
+//   2048 tiles, 40 tokens 16 / 27 : 22 / 27           48 tokens 18 / 34 : 22 / 28
+//   6144 tiles, 96 tokens 63 / 124 : 71 / 111         200 tokens 124 / 249 : 128 / 224
+//   8192 tiles, 192 tokens 159 / 303 : 165 / 281      1024 tokens 809 / 1570 : 721 / 1271
+//   4096 rows of 8 channels, 40 tokens 15 / 24 : 38 / 46, 200 tokens 58 / 121 : 50 / 132
+//  16384 rows of 5 channels, 200 tokens 60 / 175 : 505 / 619, 1000 tokens 285 / 871 : 2097 / 2602
+// The last bound is for the narrow rows; whole tiles of so many channels over hundreds of tokens are some 15 % slower than spans for it.
 static bool loop_walks(const mv2_gateloop_desc* d) {
     const int nch = d->dtype == MV2_BF16 ? 64 : 32;
     const int64_t tiles = (int64_t)d->B * d->P * ((d->C + nch - 1) / nch);
@@ -715,8 +717,8 @@ static bool loop_walks(const mv2_gateloop_desc* d) {
 }
 
 // Spans are of SPAN_WAVES waves of 32 tokens forward, and backward of 16 tokens where that lets two workgroups live on a CU by their registers
-// (128 against 216 in bf16: 8 x 2048 x 2048 99 us, 112 with 32 tokens, 1 x 131072 x 512 188 and 199; fp32 fits with 32: 3 x 1023 x 776 19 us, 20
-// with 16) and for rows shorter than a chunk.
+// (128 against 216 in bf16: 8 x 2048 x 2048 97 us, 106 with 32 tokens, 1 x 131072 x 512 196 and 207; fp32 fits with 32: 8 x 2048 x 1024 94 us, 96
+// with 16, 1 x 131072 x 256 169 and 177, but 3 x 1023 x 776 19.4 and 18.4) and for rows shorter than a chunk.
 #define SPAN_WAVES 8
 static int span_tokens(const mv2_gateloop_desc* d, bool backward) {
     return SPAN_WAVES * (!backward || (d->dtype == MV2_F32 && d->C >= 4) ? 32 : 16);
@@ -736,8 +738,9 @@ static SpanShape span_shape(const mv2_gateloop_desc* d, int nch, bool backward) 
     s.nblk = (d->T + span - 1) / span;
     s.ctiles = (d->C + nch - 1) / nch;
     s.ntile = s.ctiles * d->B * d->P;
-    // queues per XCD, forward: 4 x 8192 x 768 bf16 48 us against 50 from one queue, rows that are not whole lines 6 x 4095 x 1000 52 against 59;
-    // backward only for those (104 us against 109; whole lines 91 against 87).  Few tiles would leave XCDs idle.
+    // queues per XCD, forward: 4 x 8192 x 768 bf16 48 us against 50 from one queue, rows that are not whole lines 6 x 4095 x 1000 53 against 61;
+    // backward for those (92 us against 108); whole lines are drawn from one there, 1 to 4 % behind eight (8 x 2048 x 2048 97 us and 95, 4 x 8192 x
+    // 768 79 and 76).  Few tiles would leave XCDs idle.
     const int64_t es = d->dtype == MV2_BF16 ? 2 : 4;
     s.nq = s.ntile >= 32 && (!backward || d->in_t * es % 128 != 0) ? 8 : 1;
     s.words = s.nblk > 1 ? 64 + (s.nblk + s.nblk / LOOP_GROUP + 1) * s.ntile * nch : 0;

@@ -115,8 +115,8 @@ template <typename E> __device__ __forceinline__ void sigm_slope(float a, float&
 }
 
 // Does a call that moves this many bytes go past the caches (16-byte accesses only)?  From what the 256 MB last-level cache holds on: what a
-// smaller call reads may still be there, and what it writes is read there next.  Measured, whole lines: block norm of 16384 x 2048 bf16 73 us
-// forward and 128 backward through the caches, 65 and 118 past them; gate loop of 8 x 2048 x 2048 59 and 114, 55 and 108.
+// smaller call reads may still be there, and what it writes is read there next.  Measured, whole lines: block norm of 16384 x 2048 bf16 71 us
+// forward and 123 backward through the caches, 65 and 118 past them; gate loop of 8 x 2048 x 2048 59 and 101, 55 and 97.
 static inline bool calls_stream(double bytes) { return bytes >= 256.0 * 1024 * 1024; }
 
 // how rows of C elements are accessed: whole 16-byte chunks (2), 16 bytes at any element (1), single elements (0).  `bytes`: everything that has to
