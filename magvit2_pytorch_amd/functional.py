@@ -111,6 +111,8 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
     B, T = shape[0], shape[1] if tokens else 1
     pixels = len(shape) == rank + 1
     P = shape[rank - 1] if pixels else 1
+    if max(B, T, P, C) > 1 << 30:                         # descriptors hold 32 bits
+        raise NotImplementedError(f'{name}: {B} samples, {T} tokens, {P} pixels, {C} channels; up to 2^30 of each are built')
     h_shape = (B, P, C) if pixels else (B, C)
     if state is not None:
         _check_state(state, h_shape, dev, name)

@@ -384,7 +384,19 @@ def test_the_library_is_built_without_the_calls(monkeypatch, tmp_path):
         f.write_text('older')
     monkeypatch.setattr(build, 'CALLS', str(old[0]))
     monkeypatch.setattr(build, 'CALLS_FOR', str(old[1]))
+    monkeypatch.setattr(build, '_stale', lambda target, deps: target == str(old[0]))
     monkeypatch.setenv('CXX', str(tmp_path / 'no-such-compiler'))
     with pytest.warns(UserWarning, match='functional'):
         assert build.build(verbose=False) == build.LIB
     assert not any(f.exists() for f in old)
+
+
+def test_sizes_beyond_the_descriptors_are_refused(emulated):
+    """sizes that leave 32 bits (a view that repeats a row has them without the memory) are refused, not taken modulo 2^32"""
+    z = torch.zeros(1, 1, 1, 6)
+    for shape in ((1, (1 << 32) + 5, 1, 6), ((1 << 32) + 1, 1, 1, 6), (1, 1, (1 << 32) + 2, 6), (1, 1 << 31, 1, 6), (1, (1 << 30) + 1, 1, 6)):
+        with pytest.raises(NotImplementedError):
+            F._plan_loop('gate_loop', z.expand(shape), True, None, None, None)
+    with pytest.raises(NotImplementedError):
+        F._plan_loop('gate_loop', (z[..., :1].expand(1, 1, 1, (1 << 32) + 8),) * 3, True, None, None, None)
+    assert F._plan_loop('gate_loop', z.expand(1, 1 << 30, 1, 6), True, None, None, None).desc.T == 1 << 30
