@@ -46,6 +46,10 @@ def _need(cond, what):
         raise ValueError(what)
 
 
+def _strided(name, *args):
+    _need(all(t.layout is torch.strided for t in args if isinstance(t, torch.Tensor)), f'{name}: sparse tensors are not taken')
+
+
 def _row_dtype(t, name):
     if t.dtype not in _DTYPES:
         raise NotImplementedError(f'{name}: rows of {t.dtype}; bf16 and fp32 are built')
@@ -58,7 +62,7 @@ def _key(*args):
     like = lambda t: t if t is None or isinstance(t, str) else (t.shape, t.stride(), t.dtype, t.device, t.is_neg())
     try:
         return tuple(tuple(map(like, a)) if isinstance(a, (tuple, list)) else like(a) for a in args)
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, RuntimeError):     # (sparse tensors have no strides)
         return None
 
 
@@ -96,6 +100,7 @@ def _plan_loop(name, qkva, tokens, state, lengths, resets):
     parts = (qkva,) if fused else qkva
     _need(fused or (isinstance(qkva, (tuple, list)) and len(qkva) == 3 and all(isinstance(t, torch.Tensor) for t in qkva)),
           f'{name}: expected a tensor [q | kv | a] or the three tensors (q, kv, a)')
+    _strided(name, *parts, state, lengths, resets)
     first = parts[0]
     rank = 3 if tokens else 2
     shape, dev = first.shape, first.device
@@ -209,6 +214,7 @@ def gate_loop_step(qkva, state, *, state_out=None):
 
 def _plan_step(qkva, state, state_out):
     _need(isinstance(state, torch.Tensor), 'gate_loop_step: state must be a tensor')
+    _strided('gate_loop_step', state_out)
     plan = _plan_loop('gate_loop_step', qkva, False, state, None, None)
     _need(state.is_contiguous() and not state.is_neg(), 'gate_loop_step: the state is updated in place and must be dense')
     if state_out is not None:
@@ -237,6 +243,7 @@ def _row_stride(shape, stride):
 def _plan_norm(x, branch, gate, gate_act, *params):
     plan = _NormPlan()
     _need(isinstance(x, torch.Tensor) and x.dim() >= 1 and x.shape[-1] > 0, 'block_norm: x must have rows of at least one channel')
+    _strided('block_norm', x, branch, gate, *params)
     _need(gate_act in _ACTS, f'block_norm: unknown gate_act {gate_act!r}; silu, sigmoid or none')
     C, dev = x.shape[-1], x.device
     dtype = _row_dtype(x, 'block_norm')

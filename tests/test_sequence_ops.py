@@ -400,3 +400,12 @@ def test_sizes_beyond_the_descriptors_are_refused(emulated):
     with pytest.raises(NotImplementedError):
         F._plan_loop('gate_loop', (z[..., :1].expand(1, 1, 1, (1 << 32) + 8),) * 3, True, None, None, None)
     assert F._plan_loop('gate_loop', z.expand(1, 1 << 30, 1, 6), True, None, None, None).desc.T == 1 << 30
+
+
+def test_sparse_arguments_are_refused(emulated):
+    z, s, x, w = rnd(2, 4, 12), rnd(2, 4), rnd(3, 8), torch.ones(8)
+    for call in (lambda: F.gate_loop(z.to_sparse()), lambda: F.gate_loop(z, state=s.to_sparse()), lambda: F.gate_loop(z, lengths=torch.ones(2, dtype=torch.int32).to_sparse()),
+                 lambda: F.gate_loop((z, z, z.to_sparse())), lambda: F.gate_loop_step(z[:, 0], s.to_sparse()), lambda: F.block_norm(x.to_sparse(), pre_gamma=w),
+                 lambda: F.block_norm(x, x.to_sparse_csr()), lambda: F.block_norm(x, pre_gamma=w.to_sparse())):
+        with pytest.raises(ValueError):
+            call()
