@@ -33,6 +33,7 @@ HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'conv_common.h'), 
 NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # the native calls of functional.py: host code over torch's C++ interface, linked with the library
 CALLS = os.path.join(HERE, '_calls.so')
+CXX = 'g++'
 CALLS_SRC = os.path.join(CSRC, 'calls.cpp')
 CALLS_FOR = os.path.join(OBJ, 'calls.for')          # the interfaces that _calls.so was built against
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-fno-gpu-rdc', '-Wno-unused-result', *NO_PACKED_FP32]
@@ -113,7 +114,7 @@ def _calls_stale():
 def _build_calls(verbose):
     import torch
     root = os.path.dirname(torch.__file__)
-    cmd = [os.environ.get('CXX', 'g++'), '-O2', f'-DMV2_BUILT_FOR="{_interfaces()}"', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
+    cmd = [CXX, '-O2', f'-DMV2_BUILT_FOR="{_interfaces()}"', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{sysconfig.get_paths()["include"]}', f'-I{root}/include', f'-I{root}/include/torch/csrc/api/include',
            f'-I{os.environ.get("ROCM_PATH", "/opt/rocm")}/include', CALLS_SRC, '-o', CALLS, f'-L{root}/lib', '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip',
            f'-L{HERE}', f'-l:{os.path.basename(LIB)}', '-Wl,-rpath,$ORIGIN']

@@ -385,7 +385,7 @@ def test_the_library_is_built_without_the_calls(monkeypatch, tmp_path):
     monkeypatch.setattr(build, 'CALLS', str(old[0]))
     monkeypatch.setattr(build, 'CALLS_FOR', str(old[1]))
     monkeypatch.setattr(build, '_stale', lambda target, deps: target == str(old[0]))
-    monkeypatch.setenv('CXX', str(tmp_path / 'no-such-compiler'))
+    monkeypatch.setattr(build, 'CXX', str(tmp_path / 'no-such-compiler'))
     with pytest.warns(UserWarning, match='functional'):
         assert build.build(verbose=False) == build.LIB
     assert not any(f.exists() for f in old)
