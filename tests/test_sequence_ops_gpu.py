@@ -1038,3 +1038,45 @@ def test_bf16_parameters_get_bf16_gradients():
     parts = [torch.autograd.grad(F.block_norm(x, x, **{'post_gamma': w[1].detach(), 'scale': w[1].detach(), 'pre_gamma': w[1].detach(), k: w[1]}), w[1], (x.detach(), x.detach()))[0]
              for k in ('post_gamma', 'scale', 'pre_gamma')]
     assert ((g[0].float() - g[1]).abs() <= 5 * 2.0 ** -8 * sum(p.abs() for p in parts)).all()
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_a_captured_decoder_step(dtype):
+    """a token's step and norm in a graph: each replay takes the state on, in place and between two buffers; lengths of 64 bits and a copied layout in another.
+    The two forms' states differ by 14 units of 2^-24 a token and form at most, y by a step of the type then, the norm by what its gate (up to 3) makes of that and a step"""
+    B, T, C = 3, 12, 40
+    z = loop_inputs(B, T, 1, C, dtype).squeeze(2).cuda()
+    w = rnd(C, seed=9, mean=1.).cuda()
+    y0, h0 = F.gate_loop(z, return_state=True)
+    tok, state, other = torch.zeros_like(z[:, 0]), torch.zeros(B, C, device='cuda'), torch.zeros(B, C, device='cuda')
+    lengths = torch.full((B,), T, device='cuda')
+
+    def step(s, new=None):
+        y = F.gate_loop_step(tok, s, state_out=new)
+        return y, F.block_norm(tok[:, :C], y, gate=tok[:, C:2 * C], pre_gamma=w)[1]
+
+    def prompt():
+        return F.gate_loop(z.transpose(1, 2).contiguous().transpose(1, 2), lengths=lengths, return_state=True)
+    step(state.clone())
+    prompt()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for call in (lambda: step(state), lambda: step(state, other), lambda: step(other, state), prompt):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append(g)
+    for order in ([0] * T, [1, 2] * (T // 2)):
+        state.zero_()
+        for t, i in enumerate(order):
+            tok.copy_(z[:, t])
+            graphs[i].replay()
+            want, norm = y0[:, t], F.block_norm(z[:, t, :C], y0[:, t], gate=z[:, t, C:2 * C], pre_gamma=w)[1]
+            near = lambda a, b: bool(((a.float() - b.float()).abs() <= 4 * torch.finfo(dtype).eps * b.float().abs().amax()).all())
+            assert near(outs[i][0], want) and near(outs[i][1], norm)
+        assert ((state - h0).abs() <= 2 * 14 * T * 2.0 ** -24 * h0.abs().amax()).all()
+    for n in (T, 5, 0, T + 3):
+        lengths.fill_(n)
+        graphs[3].replay()
+        y, h = F.gate_loop(z, lengths=lengths, return_state=True)
+        assert torch.equal(outs[3][0], y) and torch.equal(outs[3][1], h)
